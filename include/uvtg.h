@@ -249,6 +249,42 @@ int uvtg_attention_bwd(const void* qkv, const unsigned char* kvalid, const void*
 int uvtg_sine_position(const float* vid_mask, const float* txt_mask, const float* dim_t, float* pos,
                        unsigned char* kvalid, int B, int Lv, int Lt, int d, uvtg_stream_t stream);
 
+/* ---- attention over score maps: with a learned relative position bias by buckets ("relpos"), and differential attention ("diff") ------
+ *   relpos  o_i = sum_j softmax_j(scale q_i.k_j + table[buckets[clamp(j - i - q_offset, -reach, reach) + reach], h]) v_j
+ *   diff    o_i = sum_j (softmax_j(scale q1_i.k1_j) - lam[h] softmax_j(scale q2_i.k2_j)) v_j
+ * q [B, Sq, H, (2,) D], k [B, Sk, Hkv, (2,) D], v [B, Sk, Hkv, D | 2 D] in 16 bits, addressed by the element strides below (channels
+ * contiguous; every stride in use and every address a multiple of 16 bytes; 0 repeats a row).  Head h reads key head h / (H / Hkv).
+ * o, o2, dO, dq, dk, dv are contiguous [B, S, heads, (2,) channels] of the same type; lse [B, H, (2,) Sq] fp32 is the natural logarithm of the
+ * row sums.  table [n_buckets, H], lam [H], dtable and dlam are fp32; buckets [2 reach + 1] int32 (entries outside 0 .. n_buckets - 1 are
+ * read as the nearest one inside).  kvalid [B, Sk] uint8, rows kvalid_sb bytes apart, 0 = the key is masked (its k / v rows may hold anything);
+ * NULL = no mask.  causal: query i sees keys j <= i + q_offset.  A row that sees no key: o = 0, lse = -inf, no gradient.
+ * Scores, statistics and sums are fp32; probabilities and score gradients are rounded to the operands' type for the products with v, k, q, dO.
+ * Results are bit-reproducible (no floating-point atomics on memory, fixed orders of summation).
+ * D: 32, 64, or 128 (relpos only).  ws: uvtg_attn_ws_bytes(dims, maps, backward) bytes, 16-byte aligned, no initial value, may be NULL if 0;
+ * maps = 1 relpos, 2 diff.  Calls in flight at the same time need a ws each. */
+typedef struct uvtg_attn_dims {
+  int struct_size;             /* = sizeof(uvtg_attn_dims)                                    */
+  int dtype;                   /* 0 bf16, 1 fp16                                              */
+  int B, H, Hkv, D, Sq, Sk;    /* H a multiple of Hkv                                         */
+  int causal, q_offset;        /* position of query 0 on the keys' axis                       */
+  float scale;                 /* > 0                                                         */
+  int n_buckets, reach;        /* relpos: rows of table; 1 <= reach <= 8191                   */
+  long long q_sb, q_ss, q_sh, q_sm, k_sb, k_ss, k_sh, k_sm, v_sb, v_ss, v_sh;   /* batch, position, head, map (diff) */
+  long long kvalid_sb;
+} uvtg_attn_dims;
+size_t uvtg_attn_ws_bytes(const uvtg_attn_dims* dm, int maps, int backward);
+int uvtg_relpos_attention_fwd(const uvtg_attn_dims* dm, const void* q, const void* k, const void* v, const float* table, const int* buckets,
+                              const unsigned char* kvalid, void* o, float* lse /* or NULL */, void* ws, uvtg_stream_t stream);
+int uvtg_relpos_attention_bwd(const uvtg_attn_dims* dm, const void* q, const void* k, const void* v, const float* table, const int* buckets,
+                              const unsigned char* kvalid, const void* o, const float* lse, const void* dO, void* dq, void* dk, void* dv,
+                              float* dtable /* or NULL */, void* ws, uvtg_stream_t stream);
+/* o2 [B, Sq, H, 2 D]: the second map's own output, which the backward pass reads (NULL in a forward call without one) */
+int uvtg_diff_attention_fwd(const uvtg_attn_dims* dm, const void* q, const void* k, const void* v, const float* lam, const unsigned char* kvalid,
+                            void* o, void* o2, float* lse /* or NULL */, void* ws, uvtg_stream_t stream);
+int uvtg_diff_attention_bwd(const uvtg_attn_dims* dm, const void* q, const void* k, const void* v, const float* lam, const unsigned char* kvalid,
+                            const void* o, const void* o2, const float* lse, const void* dO, void* dq, void* dk, void* dv,
+                            float* dlam /* or NULL */, void* ws, uvtg_stream_t stream);
+
 /* ---- wire format: replaces pad_sequences_1d (utils/tensor_utils.py:5-53) + the padded H2D copies of
  * prepare_batch_inputs_mr (main/dataset.py:1071-1100) for one key: only the VALID rows cross PCIe.
  * packed [sum(len), D]: the samples' rows back to back (fp32, or bf16 when src_bf16), offsets [B + 1] row offsets (device int),

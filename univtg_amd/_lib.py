@@ -23,11 +23,22 @@ class Dims(C.Structure):
         self.struct_size = C.sizeof(Dims)
 
 
+class AttnDims(C.Structure):
+    """struct uvtg_attn_dims (include/uvtg.h)."""
+    _fields_ = [(n, C.c_int) for n in ("struct_size", "dtype", "B", "H", "Hkv", "D", "Sq", "Sk", "causal", "q_offset")] + \
+               [("scale", C.c_float), ("n_buckets", C.c_int), ("reach", C.c_int)] + \
+               [(n, C.c_longlong) for n in ("q_sb", "q_ss", "q_sh", "q_sm", "k_sb", "k_ss", "k_sh", "k_sm", "v_sb", "v_ss", "v_sh", "kvalid_sb")]
+
+    def __init__(self, *a, **kw):
+        super().__init__(*a, **kw)
+        self.struct_size = C.sizeof(AttnDims)
+
+
 ABI_VERSION = 304          # uvtg_version() this binding was written against
 
 
 _P, _I, _F, _LL = C.c_void_p, C.c_int, C.c_float, C.c_longlong
-_DP = C.POINTER(Dims)
+_DP, _AP = C.POINTER(Dims), C.POINTER(AttnDims)
 # name -> (restype, argtypes); the authoritative prototypes are in include/uvtg.h
 SIGNATURES = {
     "uvtg_version": (_I, []),
@@ -63,6 +74,11 @@ SIGNATURES = {
     "uvtg_layernorm_bwd": (_I, [_P] * 8 + [_I, _I, _P]),
     "uvtg_attention_fwd": (_I, [_P] * 4 + [_I] * 5 + [_P]),
     "uvtg_attention_bwd": (_I, [_P] * 7 + [_F] + [_I] * 4 + [_P]),
+    "uvtg_attn_ws_bytes": (C.c_size_t, [_AP, _I, _I]),
+    "uvtg_relpos_attention_fwd": (_I, [_AP] + [_P] * 10),
+    "uvtg_relpos_attention_bwd": (_I, [_AP] + [_P] * 15),
+    "uvtg_diff_attention_fwd": (_I, [_AP] + [_P] * 10),
+    "uvtg_diff_attention_bwd": (_I, [_AP] + [_P] * 15),
     "uvtg_ragged_to_padded": (_I, [_P, _I, _P, _I, _I, _I, _P, _P, _P]),
     "uvtg_sine_position": (_I, [_P] * 5 + [_I] * 4 + [_P]),
     "uvtg_adamw_clip_step": (_I, [_P, _P, _P, _P, _LL, _F, _F, _F, _F, _F, _I, _F, _F, _P, _P]),

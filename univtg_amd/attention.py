@@ -1,0 +1,89 @@
+"""Differentiable attention cores beside the encoder's masked attention: `relpos_attention` (a learned relative position bias by buckets) and
+`diff_attention` (the difference of two softmax maps with a learned weight per head), forward and backward on the kernels of
+`ops.relpos_attention_fwd / _bwd` and `ops.diff_attention_fwd / _bwd`, where shapes, types and masks are documented.
+
+    buckets = ops.relpos_buckets(32, 128)                                  # once
+    o = relpos_attention(q, k, v, table, buckets, kvalid=kvalid)           # table: [32, H] parameter
+    o = diff_attention(q, k, v, lam, kvalid=kvalid)                        # lam: [H], e.g. exp(a1 . b1) - exp(a2 . b2) + lam0 of four parameters
+
+Under `torch.no_grad()`, or when nothing requires a gradient, they are the forward calls alone: a few new tokens against a cache of keys and
+values (`q_offset` = how many came before) run the kernel that splits the keys."""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+
+class _RelposAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, buckets, kvalid, opts):
+        o, lse = ops.relpos_attention_fwd(q, k, v, table, buckets, kvalid, *opts)
+        ctx.save_for_backward(q, k, v, table, buckets, kvalid, o, lse)
+        ctx.opts = opts
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, table, buckets, kvalid, o, lse = ctx.saved_tensors
+        dq, dk, dv, dtable = ops.relpos_attention_bwd(do, q, k, v, table, buckets, o, lse, kvalid, *ctx.opts, need_dtable=ctx.needs_input_grad[3])
+        return dq, dk, dv, dtable, None, None, None
+
+
+class _DiffAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lam, kvalid, opts):
+        o, lse, o2 = ops.diff_attention_fwd(q, k, v, lam, kvalid, *opts, need_o2=True)
+        ctx.save_for_backward(q, k, v, lam, kvalid, o, o2, lse)
+        ctx.opts = opts
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, lam, kvalid, o, o2, lse = ctx.saved_tensors
+        dq, dk, dv, dlam = ops.diff_attention_bwd(do, q, k, v, lam, o, o2, lse, kvalid, *ctx.opts, need_dlam=ctx.needs_input_grad[3])
+        return dq, dk, dv, dlam, None, None
+
+
+_STREAM = "univtg_amd.attention.stream"
+
+
+def _leaves_stream(tensors, stream, capturing):
+    """Notes on the gradient accumulator of every leaf the stream it was made for, and refuses a capture while one of another stream is alive.  An
+    accumulator lives as long as some autograd graph of its leaf does, and autograd's engine makes its stream wait for the backward pass: during a
+    capture that joins a stream outside it, which ends the process in capture_end, not in an error."""
+    for t in tensors:
+        if t.requires_grad and t.is_leaf:
+            note = torch.autograd.graph.get_gradient_edge(t).node.metadata
+            if note.setdefault(_STREAM, stream) != stream and capturing:
+                raise RuntimeError("attention: an autograd graph made outside this capture still holds a leaf of the captured call; release its outputs "
+                                   "before the capture, or pass the captured call leaves of its own")
+
+
+def _needs_grad(*tensors):
+    if not torch.is_grad_enabled() or not any(t.requires_grad for t in tensors):
+        return False
+    if tensors[0].is_cuda:
+        with torch.cuda.device_of(tensors[0]):
+            _leaves_stream(tensors, torch.cuda.current_stream().cuda_stream, torch.cuda.is_current_stream_capturing())
+    return True
+
+
+def relpos_attention(q, k, v, table, buckets, kvalid=None, q_offset=0, causal=False, scale=None):
+    """o [B, Sq, H, D] of ops.relpos_attention_fwd, differentiable in q, k, v and table (a table of another type is used, and gets its gradient, through
+    a cast to fp32)."""
+    opts = (q_offset, causal, scale)
+    if not _needs_grad(q, k, v, table):
+        return ops.relpos_attention_fwd(q, k, v, table, buckets, kvalid, *opts)[0]
+    return _RelposAttention.apply(q, k, v, table.float(), buckets, kvalid, opts)
+
+
+def diff_attention(q, k, v, lam, kvalid=None, q_offset=0, causal=False, scale=None):
+    """o [B, Sq, H, 2 D] of ops.diff_attention_fwd, differentiable in q, k, v and lam (a lam of another type through a cast to fp32)."""
+    opts = (q_offset, causal, scale)
+    if not _needs_grad(q, k, v, lam):
+        return ops.diff_attention_fwd(q, k, v, lam, kvalid, *opts)[0]
+    return _DiffAttention.apply(q, k, v, lam.float(), kvalid, opts)

@@ -1,0 +1,1306 @@
+// Attention over score maps: (1) one softmax map with a learned relative position bias by buckets ("relpos"), (2) differential attention, the
+// difference of two softmax maps with a learned weight per head ("diff").  Forward and backward, queries of one length over keys of another,
+// shared key / value heads, strided operands, key mask, causal mask, bf16 and fp16 operands with fp32 scores, statistics and sums.
+//
+//   relpos  x_ij = scale q_i.k_j + T[bucket(j - i - q_offset), h]     o = softmax(x) v
+//   diff    x^m_ij = scale q^m_i.k^m_j  (m = 1, 2)                    o = (softmax(x^1) - lam_h softmax(x^2)) v,  v twice as wide as a q / k map
+//
+// Every score tile is computed transposed to the operand that follows it (queries along lanes for o and dq, keys along lanes for dk and dv),
+// so that the probabilities go from the accumulators of one MFMA into the operand of the next without leaving their lane; the operand that has
+// to be transposed is read with ds_read_b64_tr_b16.  Tiles reach LDS by LDS-DMA (16 bytes per lane, no register round trip).
+#include "uvtg_kernels.h"
+#include "../../include/uvtg.h"
+#include <string.h>
+#include <math.h>
+
+namespace {
+
+typedef __attribute__((ext_vector_type(2))) _Float16 half2_t;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float ROW_OFF = 1e30f;       // "log2 of the sum" of a query row that has no probabilities: exp2(x - ROW_OFF) is an exact 0
+constexpr int PAD = 96;                // entries on either side of the bias window: the positions of a wave's 32 queries x 64 keys span 95
+constexpr int WIN = 256;               // key tiles whose masks a workgroup holds in LDS at a time
+
+struct MapArgs {
+  const bf16_t *q, *k, *v, *o, *o2, *dO;       // raw 16-bit values of either type
+  const float *table, *lam;
+  const int* buckets;
+  const unsigned char* kvalid;
+  bf16_t *out, *out2, *dq, *dk, *dv;
+  float *lse, *rvec, *part, *acc;
+  const float* lse_in;
+  long long q_sb, q_ss, q_sh, q_sm, k_sb, k_ss, k_sh, k_sm, v_sb, v_ss, v_sh, mask_sb;     // element strides
+  int B, H, Hkv, G, Sq, Sk, NB, R, off, causal;
+  float scale, c;                               // c = scale log2(e)
+  int hb, nsplit;                               // split kernel: heads packed into a row block, key ranges
+  int glo, gw;                                  // bias gradient: first reachable relative position, number of them
+};
+
+template <bool HALF> __device__ __forceinline__ f32x16 mma(s16x8 a, s16x8 b, f32x16 c) {
+  if constexpr (HALF) return mfma32h(a, b, c); else return mfma32(a, b, c);
+}
+template <bool HALF> __device__ __forceinline__ unsigned pack2(float lo, float hi) {
+  if constexpr (HALF) { const f32x2 v = {lo, hi}; return __builtin_bit_cast(unsigned, __builtin_convertvector(v, half2_t)); }
+  else return pack_bf2(lo, hi);
+}
+template <bool HALF> __device__ __forceinline__ float to_f(short x) {
+  if constexpr (HALF) return (float)__builtin_bit_cast(_Float16, x); else return bf2f((bf16_t)x);
+}
+template <bool HALF> __device__ __forceinline__ bf16_t from_f(float x) {
+  if constexpr (HALF) return __builtin_bit_cast(bf16_t, (_Float16)x); else return f2bf(x);
+}
+// eight packed values (a half of a 32 x 32 block's registers) as an MFMA operand
+__device__ __forceinline__ s16x8 frag(const unsigned* p) { return __builtin_bit_cast(s16x8, (u32x4){p[0], p[1], p[2], p[3]}); }
+__device__ __forceinline__ s16x8 cat4(s16x4 a, s16x4 b) { return (s16x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}; }
+__device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+// the other half-wave's value, without LDS
+__device__ __forceinline__ float half_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+  return __int_as_float(r[0]) + __int_as_float(r[1]);
+}
+__device__ __forceinline__ float half_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+  return fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
+}
+__device__ __forceinline__ void zero(f32x16& x) {
+#pragma unroll
+  for (int r = 0; r < 16; r++) x[r] = 0.f;
+}
+__device__ __forceinline__ unsigned long long uniform64(unsigned long long m) {
+  return (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(m & 0xffffffffull)) |
+         ((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(m >> 32)) << 32);
+}
+
+// An LDS tile of W-element rows that is read by rows (ds_read_b128) and transposed (ds_read_b64_tr_b16): 16-byte chunk c of row r is stored at
+// chunk c ^ f(r).  16 consecutive rows put one chunk index on 16 different 16-byte slots of the 256-byte bank row, and 4 consecutive rows put
+// the 64 bytes of a transposing read on 4 different quarters of it: neither kind of read has a bank conflict.
+template <int W> struct Tile {
+  __device__ static __forceinline__ int f(int r) {
+    if constexpr (W == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+    else if constexpr (W == 64) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+    else return (r >> 2) & 3;
+  }
+  __device__ static __forceinline__ int off(int r, int col) { return r * W + ((((col >> 3) ^ f(r))) << 3) + (col & 7); }
+  // the permutation is an XOR: 16-element column steps are XORs of the offset, 16 rows further it is the same, 8 rows further one bit differs
+  __device__ static __forceinline__ int cols(int base, int dcol) { return base ^ dcol; }
+  __device__ static __forceinline__ int rows8(int base) { return (base ^ 16) + 8 * W; }
+};
+
+// `rows` rows (a multiple of 64 / (W / 8)) of a strided matrix -> LDS tile; rows behind `last` repeat it.  `nw` waves share the work.
+template <int W, int ROWS, int NW> __device__ __forceinline__ void load_tile(const bf16_t* base, long long stride, int row0, int last, bf16_t* tile, int wave, int lane) {
+  constexpr int RPI = 512 / W, NI = ROWS / RPI;
+#pragma unroll
+  for (int i = 0; i < (NI + NW - 1) / NW; i++) {
+    const int n = i * NW + wave;
+    if (NI % NW == 0 || n < NI) {
+      const int r = n * RPI + lane / (W / 8), ch = (lane % (W / 8)) ^ Tile<W>::f(r);
+      const bf16_t* g = base + (long long)min(row0 + r, last) * stride + ch * 8;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)(tile + n * 512), 16, 0, 0);
+    }
+  }
+}
+// zero the rows of a landed tile whose mask bit is clear: a masked key's k / v row may hold anything, infinities and NaN included
+template <int W> __device__ __forceinline__ void clear_rows(bf16_t* tile, unsigned long long mask, int rows, int tid, int nt) {
+  for (int i = tid; i < rows * (W / 8); i += nt)
+    if (!((mask >> (i / (W / 8))) & 1)) *(u32x4*)(tile + i * 8) = (u32x4){0, 0, 0, 0};
+}
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Key masks of tiles w0 .. of 64 keys, one 64-bit word each (keys behind the last: 0)
+__device__ __forceinline__ void load_masks(const MapArgs& a, int b, int w0, int n, unsigned long long* sMask, int wave, int lane) {
+  const unsigned char* kv = a.kvalid ? a.kvalid + (size_t)b * a.mask_sb : nullptr;
+#pragma unroll 4
+  for (int t = wave; t < n; t += 4) {
+    const int key = (w0 + t) * 64 + lane;
+    const bool on = key < a.Sk && (!kv || kv[key] != 0);
+    const unsigned long long m = __builtin_amdgcn_ballot_w64(on);
+    if (lane == 0) sMask[t] = m;
+  }
+}
+// next tile of the window with a key that is not masked
+__device__ __forceinline__ int next_tile(const unsigned long long* sMask, int t, int n) {
+  while (t < n && uniform64(sMask[t]) == 0) t++;
+  return t;
+}
+
+// Bias of relative positions rlo .. rhi for one head, times log2(e): entry (rel - rlo).  Positions behind +-R take the bias of +-R.
+__device__ __forceinline__ void load_bias(const MapArgs& a, int h, int rlo, int rhi, float* sB, int tid, int nt) {
+  for (int i = tid; i <= rhi - rlo; i += nt) {
+    const int rel = min(max(rlo + i, -a.R), a.R);
+    const int bk = min(max(a.buckets[rel + a.R], 0), a.NB - 1);      // (an entry outside the table would be a read out of range)
+    sB[i] = a.table[(size_t)bk * a.H + h] * LOG2E;
+  }
+}
+
+// Window of positions whose bias a workgroup with positions lowest .. highest holds in LDS: at most PAD behind +-R, never without the position
+// at or behind an end that it reaches
+__device__ __forceinline__ void bias_window(const MapArgs& a, int lowest, int highest, int& rlo, int& rhi) {
+  rlo = min(max(lowest, -a.R - PAD), a.R);
+  rhi = min(max(highest, -a.R), a.R + PAD);
+}
+
+// 1-D grid -> (row block, batch, head).  Workgroups go round-robin over the 8 XCDs, each with an L2 of its own: XCD x takes a contiguous range
+// of the list, so that the blocks of a head, then the heads that share its keys, run on one XCD; batch before key head, because the samples of
+// a ragged batch differ in cost and a launch ends with its slowest XCD.
+__device__ __forceinline__ void block_id(int nblk, const MapArgs& a, int heads, int& blk, int& b, int& h) {
+  const int total = gridDim.x, qn = total / 8, r = total % 8, xcd = blockIdx.x % 8, idx = blockIdx.x / 8;
+  const int v = (xcd < r ? xcd * (qn + 1) : r * (qn + 1) + (xcd - r) * qn) + idx;
+  blk = v % nblk;
+  const int g = heads / a.Hkv, p = v / nblk, hi = p / g;
+  b = hi % a.B;
+  h = (hi / a.B) * g + p % g;
+}
+
+// [W / 32] accumulators (rows = channels, lane = row of the output) times a factor per lane -> 16-bit rows of W contiguous channels, through a
+// wave-private LDS slab: 16 bytes per lane, W / 8 lanes per row
+template <bool HALF, int W, typename F> __device__ __forceinline__ void store_rows(const f32x16* acc, float factor, bf16_t* slab, int lane, F&& row_ptr) {
+  constexpr int PW = W < 64 ? W : 64, STR = PW + 8, CPR = PW / 8;
+  const int l31 = lane & 31, g = lane >> 5;
+#pragma unroll
+  for (int pass = 0; pass < W / PW; pass++) {
+#pragma unroll
+    for (int i = 0; i < PW / 32; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const f32x16& x = acc[pass * (PW / 32) + i];
+        u32x2 t;
+        t[0] = pack2<HALF>(x[4 * j] * factor, x[4 * j + 1] * factor);
+        t[1] = pack2<HALF>(x[4 * j + 2] * factor, x[4 * j + 3] * factor);
+        *(u32x2*)(slab + l31 * STR + i * 32 + 8 * j + 4 * g) = t;
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < 32 * CPR / 64; i++) {
+      const int idx = lane + 64 * i, row = idx / CPR, ch = idx % CPR;
+      bf16_t* p = row_ptr(row);
+      const u32x4 v = *(const u32x4*)(slab + row * STR + ch * 8);
+      if (p) *(u32x4*)(p + pass * PW + ch * 8) = v;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// Scores of a 32-key x 32-query block held as f32x16 (register r <-> key (r & 3) + 8 (r >> 2) + 4 g, lane <-> query): -inf where the key's mask
+// bit is clear or the key is behind `lim` (the last key the lane's query sees, relative to the block)
+__device__ __forceinline__ void mask_scores(f32x16& s, unsigned mask32, int lim, int g, float off) {
+  const unsigned m = mask32 >> (4 * g);
+  const int l = lim - 4 * g;
+#pragma unroll
+  for (int r = 0; r < 16; r++) {
+    const int key = (r & 3) + 8 * (r >> 2);
+    if (!((m >> key) & 1) || key > l) s[r] = off;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// forward: one workgroup = 128 queries of one head, 4 waves of 32, 64-key tiles in two LDS stages
+// ------------------------------------------------------------------------------------------------
+template <bool HALF, int D, int MAPS>
+__global__ __launch_bounds__(256, 2) void maps_fwd_kernel(const MapArgs a) {
+  constexpr int DV = MAPS * D, KT = 64 * D, STAGE = MAPS * KT + 64 * DV, NK = D / 16, ND = DV / 32;
+  constexpr bool BIAS = MAPS == 1;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  bf16_t* stage = (bf16_t*)smem;
+  unsigned long long* sMask = (unsigned long long*)(smem + 2 * STAGE * 2);
+  float* sB = (float*)(sMask + WIN);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;
+  const int nqb = (a.Sq + 127) / 128;
+  int blk, b, h;
+  block_id(nqb, a, a.H, blk, b, h);
+  if (a.causal) blk = nqb - 1 - blk;                     // the longest rows first
+  const int kh = h / a.G, q0 = blk * 128 + wave * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1);
+  const bool live = q0 < a.Sq;
+  const bf16_t* kb_ = a.k + (long long)b * a.k_sb + (long long)kh * a.k_sh;
+  const bf16_t* vb_ = a.v + (long long)b * a.v_sb + (long long)kh * a.v_sh;
+
+  s16x8 qf[MAPS][NK];
+#pragma unroll
+  for (int m = 0; m < MAPS; m++)
+#pragma unroll
+    for (int ks = 0; ks < NK; ks++)
+      qf[m][ks] = *(const s16x8*)(a.q + (long long)b * a.q_sb + (long long)qrow * a.q_ss + (long long)h * a.q_sh + m * a.q_sm + 16 * ks + 8 * g);
+  f32x16 oacc[MAPS][ND];
+  float m_run[MAPS], l_run[MAPS];
+#pragma unroll
+  for (int m = 0; m < MAPS; m++) {
+    m_run[m] = -INFINITY; l_run[m] = 0.f;
+#pragma unroll
+    for (int i = 0; i < ND; i++) zero(oacc[m][i]);
+  }
+  const int last_q = min(blk * 128 + 127, a.Sq - 1);
+  int ntiles = (a.Sk + 63) / 64;
+  if (a.causal) ntiles = last_q + a.off < 0 ? 0 : min(ntiles, (last_q + a.off) / 64 + 1);
+  int rlo, rhi;
+  bias_window(a, -(last_q + a.off), ntiles * 64 - 1 - blk * 128 - a.off, rlo, rhi);
+  float bl = 0.f, br = 0.f;
+  if constexpr (BIAS) load_bias(a, h, rlo, rhi, sB, tid, 256);
+
+  const int koff = Tile<D>::off(l31, 8 * g);
+  const int toff0 = Tile<DV>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), toff1 = Tile<DV>::rows8(toff0);
+  auto request = [&](int kt, int buf) {
+    bf16_t* s = stage + buf * STAGE;
+#pragma unroll
+    for (int m = 0; m < MAPS; m++) load_tile<D, 64, 4>(kb_ + m * a.k_sm, a.k_ss, kt * 64, a.Sk - 1, s + m * KT, wave, lane);
+    load_tile<DV, 64, 4>(vb_, a.v_ss, kt * 64, a.Sk - 1, s + MAPS * KT, wave, lane);
+  };
+  for (int w0 = 0; w0 < ntiles; w0 += WIN) {
+    const int wn = min(WIN, ntiles - w0);
+    __syncthreads();
+    load_masks(a, b, w0, wn, sMask, wave, lane);
+    __syncthreads();
+    if constexpr (BIAS) if (w0 == 0) { bl = rlo <= -a.R ? sB[0] : 0.f; br = rhi >= a.R ? sB[rhi - rlo] : 0.f; }
+    int t = next_tile(sMask, 0, wn), buf = 0;
+    if (t < wn) request(w0 + t, 0);
+    while (t < wn) {
+      dma_wait();
+      __syncthreads();
+      const int tn = next_tile(sMask, t + 1, wn);
+      const unsigned long long mask = uniform64(sMask[t]);
+      bf16_t* sK = stage + buf * STAGE;
+      bf16_t* sV = sK + MAPS * KT;
+      if (mask != ~0ull) {
+        clear_rows<DV>(sV, mask, 64, tid, 256);
+        __syncthreads();
+      }
+      if (tn < wn) request(w0 + tn, buf ^ 1);
+      const int key0 = (w0 + t) * 64;
+      const int seen = a.causal ? q0 + min(31, a.Sq - 1 - q0) + a.off - key0 : 64;      // last key (relative) that any query of the wave sees
+      if (live && seen >= 0) {
+        const bool part = mask != ~0ull || (a.causal && q0 + a.off < key0 + 63);
+        unsigned pk[MAPS][2][8];
+#pragma unroll
+        for (int m = 0; m < MAPS; m++) {
+          f32x16 s[2];
+#pragma unroll
+          for (int kb = 0; kb < 2; kb++) {
+            zero(s[kb]);
+#pragma unroll
+            for (int ks = 0; ks < NK; ks++)
+              s[kb] = mma<HALF>(*(const s16x8*)(sK + m * KT + Tile<D>::cols(koff, 16 * ks) + kb * 32 * D), qf[m][ks], s[kb]);
+          }
+          // log2-domain scores are cc s + cb: the scale and a bias that is the same over the tile cost nothing, they ride in the exponent's FMA
+          float cc = a.c, cb = 0.f;
+          if constexpr (BIAS) {
+            const int rmin = key0 - q0 - 31 - a.off, rmax = key0 + 63 - q0 - a.off;
+            if (rmin >= a.R) cb = br;
+            else if (rmax <= -a.R) cb = bl;
+            else {
+              const float* bp = sB + (key0 - min(q_raw, last_q) - a.off + 4 * g - rlo);
+#pragma unroll
+              for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[kb][r] = fmaf(s[kb][r], a.c, bp[kb * 32 + (r & 3) + 8 * (r >> 2)]);
+              cc = 1.f;
+            }
+          }
+          if (part) {
+            const int lim = a.causal ? q_raw + a.off - key0 : 64;
+            mask_scores(s[0], (unsigned)mask, lim, g, -INFINITY);
+            mask_scores(s[1], (unsigned)(mask >> 32), lim - 32, g, -INFINITY);
+          }
+          float mx = s[0][0];
+#pragma unroll
+          for (int r = 1; r < 16; r++) mx = fmaxf(mx, s[0][r]);
+#pragma unroll
+          for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[1][r]);
+          mx = fmaf(half_max(mx), cc, cb);
+          // the reference point of the exponentials follows the running maximum only when it has fallen 8 (a factor of 256) behind: the sums are
+          // fp32 and the probabilities at most 2^8, and the accumulators are rescaled a few times per row instead of at every new maximum
+          if (__builtin_amdgcn_ballot_w64(mx > m_run[m] + 8.f)) {
+            const float mn = fmaxf(m_run[m], mx);
+            const float al = ex2(m_run[m] - (mn == -INFINITY ? 0.f : mn));
+            m_run[m] = mn; l_run[m] *= al;
+#pragma unroll
+            for (int i = 0; i < ND; i++)
+#pragma unroll
+              for (int r = 0; r < 16; r++) oacc[m][i][r] *= al;
+          }
+          const float e0 = cb - (m_run[m] == -INFINITY ? 0.f : m_run[m]);
+          float rs = 0.f;
+#pragma unroll
+          for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+              const float p0 = ex2(fmaf(s[kb][r], cc, e0)), p1 = ex2(fmaf(s[kb][r + 1], cc, e0));
+              rs += p0 + p1;
+              pk[m][kb][r / 2] = pack2<HALF>(p0, p1);
+            }
+          l_run[m] += rs;                                  // (this half-wave's keys; the halves meet at the end)
+        }
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+          for (int hf = 0; hf < 2; hf++) {
+            const int ro = (kb * 32 + 16 * hf) * DV;
+#pragma unroll
+            for (int i = 0; i < ND; i++) {
+              const s16x8 vt = cat4(lds_tr16(sV + Tile<DV>::cols(toff0, 32 * i) + ro), lds_tr16(sV + Tile<DV>::cols(toff1, 32 * i) + ro));
+#pragma unroll
+              for (int m = 0; m < MAPS; m++)
+                oacc[m][i] = mma<HALF>(vt, frag(pk[m][kb] + 4 * hf), oacc[m][i]);
+            }
+          }
+      }
+      t = tn; buf ^= 1;
+    }
+  }
+  dma_wait();                                              // no LDS-DMA may outlive the workgroup
+  __syncthreads();
+  if (!live) return;
+  float inv[MAPS];
+#pragma unroll
+  for (int m = 0; m < MAPS; m++) {
+    const float l = half_sum(l_run[m]);
+    inv[m] = l == 0.f ? 0.f : 1.f / l;
+    if (a.lse && g == 0 && q_raw < a.Sq) a.lse[(((size_t)b * a.H + h) * MAPS + m) * a.Sq + q_raw] = l == 0.f ? -INFINITY : m_run[m] * LN2 + __logf(l);
+  }
+  bf16_t* slab = stage + wave * 32 * 72;
+  auto rows = [&](bf16_t* base) {
+    return [=](int row) -> bf16_t* { return q0 + row < a.Sq ? base + (((size_t)b * a.Sq + q0 + row) * a.H + h) * DV : nullptr; };
+  };
+  if constexpr (MAPS == 2) {
+    if (a.out2) store_rows<HALF, DV>(oacc[MAPS - 1], inv[MAPS - 1], slab, lane, rows(a.out2));
+    const float w = -a.lam[h] * inv[MAPS - 1];
+#pragma unroll
+    for (int i = 0; i < ND; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) oacc[0][i][r] = fmaf(oacc[0][i][r], inv[0], w * oacc[MAPS - 1][i][r]);
+    inv[0] = 1.f;
+  }
+  store_rows<HALF, DV>(oacc[0], inv[0], slab, lane, rows(a.out));
+}
+
+// ------------------------------------------------------------------------------------------------
+// forward of few rows: one workgroup = up to 32 rows (queries of the heads that share a key head) x one range of keys; its 4 waves take 32-key
+// tiles in turn and never wait for each other before the end.  Bound by the bytes of k and v: every key row is read once per row block.
+// ------------------------------------------------------------------------------------------------
+template <bool HALF, int D, int MAPS>
+__global__ __launch_bounds__(256, 2) void maps_fwd_split_kernel(const MapArgs a) {
+  constexpr int DV = MAPS * D, KT = 32 * D, STAGE = MAPS * KT + 32 * DV, NK = D / 16, ND = DV / 32;
+  constexpr int NLK = MAPS * 32 * D / 512, NLV = 32 * DV / 512;                 // LDS-DMA instructions of a tile's k and v
+  constexpr bool BIAS = MAPS == 1;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  bf16_t* stage = (bf16_t*)smem;                                               // [4 waves][STAGE], then fp32 [4][DV][32] in the same place
+  constexpr int SB = 4 * STAGE * 2 > 4 * DV * 32 * 4 ? 4 * STAGE * 2 : 4 * DV * 32 * 4;
+  unsigned* sMask = (unsigned*)(smem + SB);                                    // [2 WIN] 32-key masks
+  float* sML = (float*)(sMask + 2 * WIN);                                      // [MAPS][2][4][32] maxima and sums of the waves
+  float* sB = sML + MAPS * 2 * 4 * 32;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;
+  // grid: x = row block (head group hg of hb heads, 32-row block qb of its hb * Sq rows), y = key range, z = batch x key head
+  const int rows_h = a.hb * a.Sq, nrb = (rows_h + 31) / 32, hg = blockIdx.x / nrb, rb = blockIdx.x % nrb;
+  const int b = blockIdx.z / a.Hkv, kh = blockIdx.z % a.Hkv;
+  const int nh = min(a.hb, a.G - hg * a.hb), nrows = min(32, nh * a.Sq - rb * 32);
+  if (nrows <= 0) return;
+  const int row = rb * 32 + min(l31, nrows - 1), hl = row / a.Sq, qi = row % a.Sq, h = kh * a.G + hg * a.hb + hl;
+  const bf16_t* kb_ = a.k + (long long)b * a.k_sb + (long long)kh * a.k_sh;
+  const bf16_t* vb_ = a.v + (long long)b * a.v_sb + (long long)kh * a.v_sh;
+
+  s16x8 qf[MAPS][NK];
+#pragma unroll
+  for (int m = 0; m < MAPS; m++)
+#pragma unroll
+    for (int ks = 0; ks < NK; ks++)
+      qf[m][ks] = *(const s16x8*)(a.q + (long long)b * a.q_sb + (long long)qi * a.q_ss + (long long)h * a.q_sh + m * a.q_sm + 16 * ks + 8 * g);
+  f32x16 oacc[MAPS][ND];
+  float m_run[MAPS], l_run[MAPS];
+#pragma unroll
+  for (int m = 0; m < MAPS; m++) {
+    m_run[m] = -INFINITY; l_run[m] = 0.f;
+#pragma unroll
+    for (int i = 0; i < ND; i++) zero(oacc[m][i]);
+  }
+  // positions of the block's queries: all of 0 .. Sq - 1 when several heads are packed, else 32 of them
+  const int qlo = a.hb > 1 ? 0 : rb * 32, qhi = a.hb > 1 ? a.Sq - 1 : min(rb * 32 + 31, a.Sq - 1);
+  int tiles = (a.Sk + 31) / 32;
+  if (a.causal) tiles = qhi + a.off < 0 ? 0 : min(tiles, (qhi + a.off) / 32 + 1);
+  const int per = (tiles + a.nsplit - 1) / a.nsplit, t0 = min(blockIdx.y * per, tiles), t1 = min(t0 + per, tiles);
+  const int rlo = min(max(t0 * 32 - qhi - a.off, -a.R), a.R), rhi = min(max(t1 * 32 - 1 - qlo - a.off, -a.R), a.R), bw = rhi - rlo + 1;
+  if constexpr (BIAS) for (int i = 0; i < nh; i++) load_bias(a, kh * a.G + hg * a.hb + i, rlo, rhi, sB + i * bw, tid, 256);
+
+  bf16_t* sK = stage + wave * STAGE;
+  bf16_t* sV = sK + MAPS * KT;
+  const int koff = Tile<D>::off(l31, 8 * g);
+  const int toff0 = Tile<DV>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), toff1 = Tile<DV>::rows8(toff0);
+  auto request_k = [&](int kt) {
+#pragma unroll
+    for (int m = 0; m < MAPS; m++) load_tile<D, 32, 1>(kb_ + m * a.k_sm, a.k_ss, kt * 32, a.Sk - 1, sK + m * KT, 0, lane);
+  };
+  auto request_v = [&](int kt) { load_tile<DV, 32, 1>(vb_, a.v_ss, kt * 32, a.Sk - 1, sV, 0, lane); };
+  const unsigned char* kv = a.kvalid ? a.kvalid + (size_t)b * a.mask_sb : nullptr;
+  for (int w0 = t0; w0 < t1; w0 += 2 * WIN) {
+    const int wn = min(2 * WIN, t1 - w0);
+    __syncthreads();
+#pragma unroll 4
+    for (int t = 2 * wave; t < wn; t += 8) {               // two 32-key masks per ballot
+      const int key = (w0 + t) * 32 + lane;
+      const unsigned long long m = __builtin_amdgcn_ballot_w64(key < a.Sk && (!kv || kv[key] != 0));
+      if (lane == 0) { sMask[t] = (unsigned)m; sMask[t + 1] = (unsigned)(m >> 32); }
+    }
+    __syncthreads();
+    auto next = [&](int t) { while (t < wn && __builtin_amdgcn_readfirstlane((int)sMask[t]) == 0) t += 4; return t; };
+    int t = next(wave);
+    if (t < wn) { request_k(w0 + t); request_v(w0 + t); }
+    while (t < wn) {
+      const int tn = next(t + 4);
+      const bool more = tn < wn;
+      const unsigned mask = (unsigned)__builtin_amdgcn_readfirstlane((int)sMask[t]);
+      const int key0 = (w0 + t) * 32;
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NLV) : "memory");          // k of this tile has landed (its v was requested behind it)
+      f32x16 s[MAPS];
+#pragma unroll
+      for (int m = 0; m < MAPS; m++) {
+        zero(s[m]);
+#pragma unroll
+        for (int ks = 0; ks < NK; ks++) s[m] = mma<HALF>(*(const s16x8*)(sK + m * KT + Tile<D>::cols(koff, 16 * ks)), qf[m][ks], s[m]);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                  // the reads of k are done: its place may be written
+      if (more) {
+        request_k(w0 + tn);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NLK) : "memory");        // v of this tile
+      } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (mask != ~0u) { clear_rows<DV>(sV, mask, 32, lane, 64); asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+      unsigned pk[MAPS][8];
+#pragma unroll
+      for (int m = 0; m < MAPS; m++) {
+        if constexpr (BIAS) {
+          const float* bp = sB + hl * bw;
+          const int rel = key0 + 4 * g - qi - a.off;
+#pragma unroll
+          for (int r = 0; r < 16; r++) s[m][r] = fmaf(s[m][r], a.c, bp[min(max(rel + (r & 3) + 8 * (r >> 2), rlo), rhi) - rlo]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; r++) s[m][r] *= a.c;
+        }
+        mask_scores(s[m], mask, a.causal ? qi + a.off - key0 : 32, g, -INFINITY);
+        float mx = s[m][0];
+#pragma unroll
+        for (int r = 1; r < 16; r++) mx = fmaxf(mx, s[m][r]);
+        mx = half_max(mx);
+        if (__builtin_amdgcn_ballot_w64(mx > m_run[m] + 8.f)) {
+          const float mn = fmaxf(m_run[m], mx);
+          const float al = ex2(m_run[m] - (mn == -INFINITY ? 0.f : mn));
+          m_run[m] = mn; l_run[m] *= al;
+#pragma unroll
+          for (int i = 0; i < ND; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) oacc[m][i][r] *= al;
+        }
+        const float e0 = m_run[m] == -INFINITY ? 0.f : -m_run[m];
+        float rs = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const float p0 = ex2(s[m][r] + e0), p1 = ex2(s[m][r + 1] + e0);
+          rs += p0 + p1;
+          pk[m][r / 2] = pack2<HALF>(p0, p1);
+        }
+        l_run[m] += rs;
+      }
+#pragma unroll
+      for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+        for (int i = 0; i < ND; i++) {
+          const int ro = 16 * hf * DV;
+          const s16x8 vt = cat4(lds_tr16(sV + Tile<DV>::cols(toff0, 32 * i) + ro), lds_tr16(sV + Tile<DV>::cols(toff1, 32 * i) + ro));
+#pragma unroll
+          for (int m = 0; m < MAPS; m++) oacc[m][i] = mma<HALF>(vt, frag(pk[m] + 4 * hf), oacc[m][i]);
+        }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (more) request_v(w0 + tn);
+      t = tn;
+    }
+  }
+  // join the four waves: factors from the common maximum, then a sum in wave order
+#pragma unroll
+  for (int m = 0; m < MAPS; m++) {
+    const float l = half_sum(l_run[m]);
+    if (g == 0) { sML[(m * 2 + 0) * 128 + wave * 32 + l31] = m_run[m]; sML[(m * 2 + 1) * 128 + wave * 32 + l31] = l; }
+  }
+  float* sO = (float*)smem;
+  const int orow = tid & 31, oc = tid >> 5;                                   // 8 threads per row, DV / 8 channels each
+  const int r2 = rb * 32 + orow, oh = kh * a.G + hg * a.hb + r2 / a.Sq, oq = r2 % a.Sq;
+  constexpr int CPT = DV / 8;
+  float res[MAPS][CPT], mt[MAPS], lt[MAPS];
+#pragma unroll
+  for (int m = 0; m < MAPS; m++) {
+    __syncthreads();                                                           // tiles read, maxima written; the other map's sums read
+    const float* M = sML + (m * 2) * 128;
+    const float mm = fmaxf(fmaxf(M[l31], M[32 + l31]), fmaxf(M[64 + l31], M[96 + l31]));
+    const float fac = ex2(m_run[m] - (mm == -INFINITY ? 0.f : mm));
+#pragma unroll
+    for (int i = 0; i < ND; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) sO[(wave * DV + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * g) * 32 + l31] = oacc[m][i][r] * fac;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < CPT; e++) {
+      float x = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; w++) x += sO[(w * DV + oc * CPT + e) * 32 + orow];
+      res[m][e] = x;
+    }
+    const float mo = fmaxf(fmaxf(M[orow], M[32 + orow]), fmaxf(M[64 + orow], M[96 + orow]));
+    float l = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) l += M[128 + w * 32 + orow] * ex2(M[w * 32 + orow] - (mo == -INFINITY ? 0.f : mo));
+    mt[m] = mo; lt[m] = l;
+  }
+  if (orow >= nrows) return;
+  const size_t orow_g = ((size_t)b * a.H + oh) * a.Sq + oq;
+  if (a.nsplit > 1) {                                                          // partial: [B, H, Sq][split][MAPS][DV + 2]
+    float* w = a.acc + (orow_g * a.nsplit + blockIdx.y) * (MAPS * (DV + 2));
+#pragma unroll
+    for (int m = 0; m < MAPS; m++) {
+#pragma unroll
+      for (int e = 0; e < CPT; e++) w[m * (DV + 2) + oc * CPT + e] = res[m][e];
+      if (oc == 0) { w[m * (DV + 2) + DV] = mt[m]; w[m * (DV + 2) + DV + 1] = lt[m]; }
+    }
+    return;
+  }
+  float inv[MAPS];
+#pragma unroll
+  for (int m = 0; m < MAPS; m++) {
+    inv[m] = lt[m] == 0.f ? 0.f : 1.f / lt[m];
+    if (a.lse && oc == 0) a.lse[(((size_t)b * a.H + oh) * MAPS + m) * a.Sq + oq] = lt[m] == 0.f ? -INFINITY : mt[m] * LN2 + __logf(lt[m]);
+  }
+  const size_t ob = (((size_t)b * a.Sq + oq) * a.H + oh) * DV + oc * CPT;
+  const float w = MAPS == 2 ? a.lam[oh] : 0.f;
+#pragma unroll
+  for (int e = 0; e < CPT; e++) {
+    float x = res[0][e] * inv[0];
+    if constexpr (MAPS == 2) {
+      const float y = res[MAPS - 1][e] * inv[MAPS - 1];
+      if (a.out2) a.out2[ob + e] = from_f<HALF>(y);
+      x -= w * y;
+    }
+    a.out[ob + e] = from_f<HALF>(x);
+  }
+}
+
+// joins the key ranges of maps_fwd_split_kernel: one wave per row, ranges in order
+template <bool HALF, int D, int MAPS>
+__global__ __launch_bounds__(256) void maps_join_kernel(const MapArgs a) {
+  constexpr int DV = MAPS * D, CPL = (DV + 63) / 64, W = MAPS * (DV + 2);
+  const int lane = threadIdx.x & 63;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);        // (b, h, query)
+  if (row >= (long long)a.B * a.H * a.Sq) return;
+  const int i = (int)(row % a.Sq);
+  const long long bh = row / a.Sq;
+  const int h = (int)(bh % a.H), b = (int)(bh / a.H);
+  const float* p = a.acc + (size_t)row * a.nsplit * W;
+  float o[MAPS][CPL];
+#pragma unroll
+  for (int m = 0; m < MAPS; m++) {
+    float mx = -INFINITY;
+    for (int s = lane; s < a.nsplit; s += 64) mx = fmaxf(mx, p[(size_t)s * W + m * (DV + 2) + DV]);
+    mx = wave_max(mx);
+    const float mu = mx == -INFINITY ? 0.f : mx;
+    float l = 0.f;
+#pragma unroll
+    for (int c = 0; c < CPL; c++) o[m][c] = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < a.nsplit; s++) {
+      const float* w = p + (size_t)s * W + m * (DV + 2);
+      const float f = ex2(w[DV] - mu);
+      l += w[DV + 1] * f;
+#pragma unroll
+      for (int c = 0; c < CPL; c++) if (DV >= 64 || lane < DV) o[m][c] += w[lane + 64 * c] * f;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int c = 0; c < CPL; c++) o[m][c] *= inv;
+    if (a.lse && lane == 0) a.lse[(bh * MAPS + m) * a.Sq + i] = l == 0.f ? -INFINITY : mx * LN2 + __logf(l);
+  }
+  const size_t ob = (((size_t)b * a.Sq + i) * a.H + h) * DV;
+#pragma unroll
+  for (int c = 0; c < CPL; c++) {
+    if (DV < 64 && lane >= DV) continue;
+    float x = o[0][c];
+    if constexpr (MAPS == 2) {
+      if (a.out2) a.out2[ob + lane + 64 * c] = from_f<HALF>(o[MAPS - 1][c]);
+      x -= a.lam[h] * o[MAPS - 1][c];
+    }
+    a.out[ob + lane + 64 * c] = from_f<HALF>(x);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// backward, queries: dq and the row sums r_i = sum_j p_ij dp_ij.  One workgroup = 128 queries of one head, as the forward.
+// ds = p (dp - r) needs r before the first key: rowsum(dO o) gives it up to the rounding of o, which is enough for dq (16 bits), and the exact
+// fp32 sum falls out of the same registers (one FMA per element): the key kernel forms ds, the bias table's and lam's gradients from that.
+// ------------------------------------------------------------------------------------------------
+template <bool HALF, int D, int MAPS>
+__global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
+  constexpr int DV = MAPS * D, KT = 64 * D, STAGE = MAPS * KT + 64 * DV, NK = D / 16, NV = DV / 16, ND = D / 32;
+  constexpr bool BIAS = MAPS == 1;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  bf16_t* stage = (bf16_t*)smem;
+  unsigned long long* sMask = (unsigned long long*)(smem + 2 * STAGE * 2);
+  float* sB = (float*)(sMask + WIN);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;
+  const int nqb = (a.Sq + 127) / 128;
+  int blk, b, h;
+  block_id(nqb, a, a.H, blk, b, h);
+  if (a.causal) blk = nqb - 1 - blk;
+  const int kh = h / a.G, q0 = blk * 128 + wave * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1);
+  const bool live = q0 < a.Sq;
+  const bf16_t* kb_ = a.k + (long long)b * a.k_sb + (long long)kh * a.k_sh;
+  const bf16_t* vb_ = a.v + (long long)b * a.v_sb + (long long)kh * a.v_sh;
+  s16x8 qf[MAPS][NK], of[NV];
+  float L[MAPS], del[MAPS], racc[MAPS];
+#pragma unroll
+  for (int m = 0; m < MAPS; m++) {
+#pragma unroll
+    for (int ks = 0; ks < NK; ks++)
+      qf[m][ks] = *(const s16x8*)(a.q + (long long)b * a.q_sb + (long long)qrow * a.q_ss + (long long)h * a.q_sh + m * a.q_sm + 16 * ks + 8 * g);
+    const float l = a.lse_in[(((size_t)b * a.H + h) * MAPS + m) * a.Sq + qrow];
+    L[m] = l == -INFINITY ? ROW_OFF : l * LOG2E;
+    del[m] = 0.f; racc[m] = 0.f;
+  }
+  const float lam = MAPS == 2 ? a.lam[h] : 0.f;
+  {
+    const size_t ro = (((size_t)b * a.Sq + qrow) * a.H + h) * DV + 8 * g;
+#pragma unroll
+    for (int ks = 0; ks < NV; ks++) {
+      of[ks] = *(const s16x8*)(a.dO + ro + 16 * ks);
+      const s16x8 x = *(const s16x8*)(a.o + ro + 16 * ks);
+      s16x8 y;
+      if constexpr (MAPS == 2) y = *(const s16x8*)(a.o2 + ro + 16 * ks);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float d = to_f<HALF>(of[ks][e]);
+        if constexpr (MAPS == 2) {
+          const float o2 = to_f<HALF>(y[e]);
+          del[0] += d * fmaf(lam, o2, to_f<HALF>(x[e]));
+          del[MAPS - 1] += d * o2;
+        } else del[0] += d * to_f<HALF>(x[e]);
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MAPS; m++) del[m] = half_sum(del[m]);
+  }
+  f32x16 acc[MAPS][ND];
+#pragma unroll
+  for (int m = 0; m < MAPS; m++)
+#pragma unroll
+    for (int i = 0; i < ND; i++) zero(acc[m][i]);
+  const int last_q = min(blk * 128 + 127, a.Sq - 1);
+  int ntiles = (a.Sk + 63) / 64;
+  if (a.causal) ntiles = last_q + a.off < 0 ? 0 : min(ntiles, (last_q + a.off) / 64 + 1);
+  int rlo, rhi;
+  bias_window(a, -(last_q + a.off), ntiles * 64 - 1 - blk * 128 - a.off, rlo, rhi);
+  float bl = 0.f, br = 0.f;
+  if constexpr (BIAS) load_bias(a, h, rlo, rhi, sB, tid, 256);
+  const int koff = Tile<D>::off(l31, 8 * g), voff = Tile<DV>::off(l31, 8 * g);
+  const int toff0 = Tile<D>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), toff1 = Tile<D>::rows8(toff0);
+  auto request = [&](int kt, int buf) {
+    bf16_t* s = stage + buf * STAGE;
+#pragma unroll
+    for (int m = 0; m < MAPS; m++) load_tile<D, 64, 4>(kb_ + m * a.k_sm, a.k_ss, kt * 64, a.Sk - 1, s + m * KT, wave, lane);
+    load_tile<DV, 64, 4>(vb_, a.v_ss, kt * 64, a.Sk - 1, s + MAPS * KT, wave, lane);
+  };
+  for (int w0 = 0; w0 < ntiles; w0 += WIN) {
+    const int wn = min(WIN, ntiles - w0);
+    __syncthreads();
+    load_masks(a, b, w0, wn, sMask, wave, lane);
+    __syncthreads();
+    if constexpr (BIAS) if (w0 == 0) { bl = rlo <= -a.R ? sB[0] : 0.f; br = rhi >= a.R ? sB[rhi - rlo] : 0.f; }
+    int t = next_tile(sMask, 0, wn), buf = 0;
+    if (t < wn) request(w0 + t, 0);
+    while (t < wn) {
+      dma_wait();
+      __syncthreads();
+      const int tn = next_tile(sMask, t + 1, wn);
+      const unsigned long long mask = uniform64(sMask[t]);
+      bf16_t* sK = stage + buf * STAGE;
+      bf16_t* sV = sK + MAPS * KT;
+      if (mask != ~0ull) {
+#pragma unroll
+        for (int m = 0; m < MAPS; m++) clear_rows<D>(sK + m * KT, mask, 64, tid, 256);
+        clear_rows<DV>(sV, mask, 64, tid, 256);
+        __syncthreads();
+      }
+      if (tn < wn) request(w0 + tn, buf ^ 1);
+      const int key0 = (w0 + t) * 64;
+      const int seen = a.causal ? q0 + min(31, a.Sq - 1 - q0) + a.off - key0 : 64;
+      if (live && seen >= 0) {
+        const bool part = mask != ~0ull || (a.causal && q0 + a.off < key0 + 63);
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++) {
+          f32x16 dp, s[MAPS];
+          zero(dp);
+#pragma unroll
+          for (int ks = 0; ks < NV; ks++) dp = mma<HALF>(*(const s16x8*)(sV + Tile<DV>::cols(voff, 16 * ks) + kb * 32 * DV), of[ks], dp);
+          unsigned pk[MAPS][8];
+#pragma unroll
+          for (int m = 0; m < MAPS; m++) {
+            zero(s[m]);
+#pragma unroll
+            for (int ks = 0; ks < NK; ks++) s[m] = mma<HALF>(*(const s16x8*)(sK + m * KT + Tile<D>::cols(koff, 16 * ks) + kb * 32 * D), qf[m][ks], s[m]);
+            float cc = a.c, cb = 0.f;
+            if constexpr (BIAS) {
+              const int rmin = key0 - q0 - 31 - a.off, rmax = key0 + 63 - q0 - a.off;
+              if (rmin >= a.R) cb = br;
+              else if (rmax <= -a.R) cb = bl;
+              else {
+                const float* bp = sB + (key0 - min(q_raw, last_q) - a.off + 4 * g - rlo);
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[m][r] = fmaf(s[m][r], a.c, bp[kb * 32 + (r & 3) + 8 * (r >> 2)]);
+                cc = 1.f;
+              }
+            }
+            if (part) mask_scores(s[m], (unsigned)(mask >> (32 * kb)), (a.causal ? q_raw + a.off - key0 : 64) - 32 * kb, g, -INFINITY);
+            const float e0 = cb - L[m];
+            const float f = m == 0 ? 1.f : -lam;
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+              const float p0 = ex2(fmaf(s[m][r], cc, e0)), p1 = ex2(fmaf(s[m][r + 1], cc, e0));
+              racc[m] = fmaf(p0, dp[r], racc[m]); racc[m] = fmaf(p1, dp[r + 1], racc[m]);
+              pk[m][r / 2] = pack2<HALF>((m ? f * p0 : p0) * (dp[r] - del[m]), (m ? f * p1 : p1) * (dp[r + 1] - del[m]));
+            }
+          }
+#pragma unroll
+          for (int m = 0; m < MAPS; m++)
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+              for (int i = 0; i < ND; i++) {
+                const int ro = m * KT + (kb * 32 + 16 * hf) * D;
+                const s16x8 kt = cat4(lds_tr16(sK + Tile<D>::cols(toff0, 32 * i) + ro), lds_tr16(sK + Tile<D>::cols(toff1, 32 * i) + ro));
+                acc[m][i] = mma<HALF>(kt, frag(pk[m] + 4 * hf), acc[m][i]);
+              }
+        }
+      }
+      t = tn; buf ^= 1;
+    }
+  }
+  dma_wait();
+  __syncthreads();
+  if (!live) return;
+#pragma unroll
+  for (int m = 0; m < MAPS; m++) {
+    const float r = half_sum(racc[m]);
+    if (g == 0 && q_raw < a.Sq) a.rvec[(((size_t)b * a.H + h) * MAPS + m) * a.Sq + q_raw] = r;
+    if (MAPS == 2 && m == MAPS - 1) {                      // lam's gradient: the wave's 32 rows, [H][B][32-row block]
+      const float w = wave_sum_dpp(g == 0 && q_raw < a.Sq ? r : 0.f);
+      const int n32 = (a.Sq + 31) / 32;
+      if (lane == 0) a.part[((size_t)h * a.B + b) * n32 + q0 / 32] = w;
+    }
+  }
+  bf16_t* slab = stage + wave * 32 * 72;
+#pragma unroll
+  for (int m = 0; m < MAPS; m++)
+    store_rows<HALF, D>(acc[m], a.scale, slab, lane, [=](int row) -> bf16_t* {
+      return q0 + row < a.Sq ? a.dq + ((((size_t)b * a.Sq + q0 + row) * a.H + h) * MAPS + m) * D : nullptr; });
+}
+
+// ------------------------------------------------------------------------------------------------
+// backward, keys: dk, dv and (relpos) the bias gradient by relative position.  One workgroup = 128 keys of one key head, 4 waves of 32; it walks
+// the queries of every head of the group in tiles of 64, so that the shared heads' gradients are summed in registers, in a fixed order.
+// ------------------------------------------------------------------------------------------------
+template <bool HALF, int D, int MAPS>
+__global__ __launch_bounds__(256, 1) void maps_bwd_k_kernel(const MapArgs a) {
+  constexpr int DV = MAPS * D, QT = 64 * D, STAGE = MAPS * QT + 64 * DV, NK = D / 16, NV = DV / 16, ND = D / 32, NDV = DV / 32;
+  constexpr bool BIAS = MAPS == 1;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  bf16_t* stage = (bf16_t*)smem;
+  float* sStat = (float*)(smem + 2 * STAGE * 2);           // [2][MAPS][2][64]: log2 of the row sums, r
+  float* sDiag = sStat + 2 * MAPS * 2 * 64;                // [4 waves][2 halves][64] sums along diagonals
+  float* sB = sDiag + 4 * 2 * 64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;
+  const int nkb = (a.Sk + 127) / 128;
+  int blk, b, kh;
+  block_id(nkb, a, a.Hkv, blk, b, kh);
+  const int k0 = blk * 128 + wave * 32, key = k0 + l31, krow = min(key, a.Sk - 1);
+  const bool kok = key < a.Sk && (!a.kvalid || a.kvalid[(size_t)b * a.mask_sb + krow] != 0);
+  const bool live = __builtin_amdgcn_ballot_w64(kok) != 0;                    // some key of the wave is not masked
+  // a masked key's row may hold anything: its fragments are zeros, its gradient rows are zeros, and it adds to no bias sum
+  s16x8 kf[MAPS][NK], vf[NV];
+  {
+    const s16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int m = 0; m < MAPS; m++)
+#pragma unroll
+      for (int ks = 0; ks < NK; ks++) {
+        const s16x8 x = *(const s16x8*)(a.k + (long long)b * a.k_sb + (long long)krow * a.k_ss + (long long)kh * a.k_sh + m * a.k_sm + 16 * ks + 8 * g);
+        kf[m][ks] = kok ? x : z;
+      }
+#pragma unroll
+    for (int ks = 0; ks < NV; ks++) {
+      const s16x8 x = *(const s16x8*)(a.v + (long long)b * a.v_sb + (long long)krow * a.v_ss + (long long)kh * a.v_sh + 16 * ks + 8 * g);
+      vf[ks] = kok ? x : z;
+    }
+  }
+  f32x16 dk[MAPS][ND], dv[NDV];
+#pragma unroll
+  for (int m = 0; m < MAPS; m++)
+#pragma unroll
+    for (int i = 0; i < ND; i++) zero(dk[m][i]);
+#pragma unroll
+  for (int i = 0; i < NDV; i++) zero(dv[i]);
+  const int qoff = Tile<D>::off(l31, 8 * g), ooff = Tile<DV>::off(l31, 8 * g);
+  const int tq0 = Tile<D>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), tq1 = Tile<D>::rows8(tq0);
+  const int to0 = Tile<DV>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), to1 = Tile<DV>::rows8(to0);
+  // queries that see a key of the workgroup; no tile at all when none does, or when no key of the workgroup is valid
+  const int any = __syncthreads_or(kok ? 1 : 0);
+  const int first = a.causal ? max(0, (blk * 128 - a.off)) / 64 : 0, nqt = any ? max(0, (a.Sq + 63) / 64 - first) : 0;
+  int rlo, rhi;
+  bias_window(a, blk * 128 - (a.Sq + 63) - a.off, blk * 128 + 127 - first * 64 - a.off, rlo, rhi);
+  const int nk32 = (a.Sk + 31) / 32;
+  float* diag = sDiag + wave * 128;
+  for (int hg = 0; hg < a.G; hg++) {
+    const int h = kh * a.G + hg;
+    const bf16_t* qb_ = a.q + (long long)b * a.q_sb + (long long)h * a.q_sh;
+    const bf16_t* ob_ = a.dO + ((size_t)b * a.Sq * a.H + h) * DV;
+    const float* lse = a.lse_in + ((size_t)b * a.H + h) * MAPS * a.Sq;
+    const float* rv = a.rvec + ((size_t)b * a.H + h) * MAPS * a.Sq;
+    const float lam = MAPS == 2 ? a.lam[h] : 0.f;
+    float fl = 0.f, fr = 0.f, bl = 0.f, br = 0.f;          // sums and bias of the positions at and behind -R / +R
+    bool open = false;                                     // diagonals of the last block are still being summed
+    int base = 0;
+    float* part = nullptr;
+    __syncthreads();                                       // the previous head's tiles, bias and statistics are read
+    if constexpr (BIAS) {
+      load_bias(a, h, rlo, rhi, sB, tid, 256);
+      if (a.part) {
+        part = a.part + (((size_t)h * a.B + b) * nk32 + k0 / 32) * a.gw;
+        if (k0 < a.Sk) for (int i = lane; i < a.gw; i += 64) part[i] = 0.f;     // (done before the first tile's wait)
+        diag[lane] = 0.f; diag[64 + lane] = 0.f;
+      }
+    }
+    float pl = 0.f;
+    auto request = [&](int qt, int buf) {
+      bf16_t* s = stage + buf * STAGE;
+#pragma unroll
+      for (int m = 0; m < MAPS; m++) load_tile<D, 64, 4>(qb_ + m * a.q_sm, a.q_ss, qt * 64, a.Sq - 1, s + m * QT, wave, lane);
+      load_tile<DV, 64, 4>(ob_, (long long)a.H * DV, qt * 64, a.Sq - 1, s + MAPS * QT, wave, lane);
+      if (tid < MAPS * 128) {                              // thread = (map, statistic, row)
+        const int m = tid >> 7, row = min(qt * 64 + (tid & 63), a.Sq - 1);
+        pl = (tid & 64 ? rv : lse)[m * a.Sq + row];
+      }
+    };
+    auto stats = [&](int qt, int buf) {
+      if (tid < MAPS * 128) sStat[buf * MAPS * 128 + tid] = tid & 64 ? pl : (qt * 64 + (tid & 63) >= a.Sq || pl == -INFINITY) ? ROW_OFF : pl * LOG2E;
+    };
+    // a finished 64-entry window of diagonal sums: relative positions base - 31 .. base + 31 at entries 0 .. 62; the upper 32 are complete and
+    // leave, the lower 31 move up for the next query block
+    auto flush = [&](int base_) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const float v = diag[lane] + diag[64 + lane];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (lane < 63) diag[lane < 31 ? lane + 32 : lane - 31] = lane < 31 ? v : 0.f;
+      diag[64 + lane] = 0.f;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      const int rel = base_ + lane - 31;
+      if (lane >= 31 && lane < 63) {
+        if (rel >= a.R) fr += v;
+        else if (rel <= -a.R) fl += v;
+        else if (rel >= a.glo && rel < a.glo + a.gw) part[rel - a.glo] = v;
+      }
+    };
+    if (nqt > 0) { request(first, 0); stats(first, 0); }
+    for (int n = 0; n < nqt; n++) {
+      const int qt = first + n, buf = n & 1;
+      dma_wait();
+      __syncthreads();
+      if (n == 0) if constexpr (BIAS) { bl = rlo <= -a.R ? sB[0] : 0.f; br = rhi >= a.R ? sB[rhi - rlo] : 0.f; }
+      if (n + 1 < nqt) request(qt + 1, buf ^ 1);
+      bf16_t* sQ = stage + buf * STAGE;
+      bf16_t* sO = sQ + MAPS * QT;
+      const float* st = sStat + buf * MAPS * 128;
+#pragma unroll 1
+      for (int qs = 0; qs < 2; qs++) {
+        const int q0 = qt * 64 + qs * 32;
+        if (q0 >= a.Sq || !live || (a.causal && q0 + 31 + a.off < k0)) continue;
+        f32x16 s[MAPS], dp;
+        zero(dp);
+#pragma unroll
+        for (int m = 0; m < MAPS; m++) {
+          zero(s[m]);
+#pragma unroll
+          for (int ks = 0; ks < NK; ks++) s[m] = mma<HALF>(*(const s16x8*)(sQ + m * QT + Tile<D>::cols(qoff, 16 * ks) + qs * 32 * D), kf[m][ks], s[m]);
+        }
+#pragma unroll
+        for (int ks = 0; ks < NV; ks++) dp = mma<HALF>(*(const s16x8*)(sO + Tile<DV>::cols(ooff, 16 * ks) + qs * 32 * DV), vf[ks], dp);
+        // register r <-> query q0 + (r & 3) + 8 (r >> 2) + 4 g, lane <-> key
+        const int rb = k0 - q0 - a.off;                    // relative position of the block's first key and first query
+        const bool right = BIAS && rb - 31 >= a.R, left = BIAS && rb + 31 <= -a.R, near = BIAS && !right && !left;
+        float cc = a.c, cb = 0.f;
+        if constexpr (BIAS) {
+          if (right) cb = br;
+          else if (left) cb = bl;
+          else {
+            const float* bp = sB + (rb + l31 - 4 * g - 27 - rlo);
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[0][r] = fmaf(s[0][r], a.c, bp[27 - (r & 3) - 8 * (r >> 2)]);
+            cc = 1.f;
+          }
+        }
+        if (a.causal && q0 + a.off < k0 + 31) {            // key seen by queries at key - off and behind
+          const int lim = key - q0 - a.off - 4 * g;
+#pragma unroll
+          for (int m = 0; m < MAPS; m++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) if ((r & 3) + 8 * (r >> 2) < lim) s[m][r] = -INFINITY;
+        }
+        unsigned pp[8], pd[MAPS][8];
+        float ds0[16];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          f32x4 L[MAPS], r_[MAPS];
+#pragma unroll
+          for (int m = 0; m < MAPS; m++) {
+            L[m] = *(const f32x4*)(st + m * 128 + qs * 32 + 8 * j + 4 * g);
+            r_[m] = *(const f32x4*)(st + m * 128 + 64 + qs * 32 + 8 * j + 4 * g);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            float p[2], d0[2], d1[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+              const int r = 4 * j + e + u;
+              p[u] = ex2(fmaf(s[0][r], cc, cb - L[0][e + u]));
+              d0[u] = p[u] * (dp[r] - r_[0][e + u]);
+              if constexpr (BIAS) ds0[r] = d0[u];
+              if constexpr (MAPS == 2) {
+                const float p2 = -lam * ex2(fmaf(s[MAPS - 1][r], cc, -L[MAPS - 1][e + u]));
+                d1[u] = p2 * (dp[r] - r_[MAPS - 1][e + u]);
+                p[u] += p2;
+              }
+            }
+            pp[2 * j + e / 2] = pack2<HALF>(p[0], p[1]);
+            pd[0][2 * j + e / 2] = pack2<HALF>(d0[0], d0[1]);
+            if constexpr (MAPS == 2) pd[MAPS - 1][2 * j + e / 2] = pack2<HALF>(d1[0], d1[1]);
+          }
+        }
+        if constexpr (BIAS) {
+          if (part) {
+            if (near) {
+              if (kok) {                                   // one address per lane and instruction: the order of a wave's LDS additions is its program's
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                  const int at = g * 64 + l31 - 4 * g + 31 - (r & 3) - 8 * (r >> 2);
+                  __hip_atomic_fetch_add(diag + at, ds0[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                }
+              }
+              flush(rb);
+              open = true; base = rb - 32;
+            } else {
+              float t = 0.f;
+#pragma unroll
+              for (int r = 0; r < 16; r++) t += ds0[r];
+              t = kok ? t : 0.f;
+              if (right) fr += t; else fl += t;
+              if (left && open) { flush(rb); open = false; }
+            }
+          }
+        }
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++) {
+          const s16x8 p8 = frag(pp + 4 * hf);
+#pragma unroll
+          for (int i = 0; i < NDV; i++) {
+            const int ro = (qs * 32 + 16 * hf) * DV;
+            const s16x8 ot = cat4(lds_tr16(sO + Tile<DV>::cols(to0, 32 * i) + ro), lds_tr16(sO + Tile<DV>::cols(to1, 32 * i) + ro));
+            dv[i] = mma<HALF>(ot, p8, dv[i]);
+          }
+#pragma unroll
+          for (int m = 0; m < MAPS; m++) {
+            const s16x8 d8 = frag(pd[m] + 4 * hf);
+#pragma unroll
+            for (int i = 0; i < ND; i++) {
+              const int ro = m * QT + (qs * 32 + 16 * hf) * D;
+              const s16x8 qt_ = cat4(lds_tr16(sQ + Tile<D>::cols(tq0, 32 * i) + ro), lds_tr16(sQ + Tile<D>::cols(tq1, 32 * i) + ro));
+              dk[m][i] = mma<HALF>(qt_, d8, dk[m][i]);
+            }
+          }
+        }
+      }
+      if (n + 1 < nqt) stats(qt + 1, buf ^ 1);
+    }
+    if constexpr (BIAS) {
+      if (part && k0 < a.Sk) {
+        if (open) flush(base);
+        fl = wave_sum_dpp(fl); fr = wave_sum_dpp(fr);
+        if (lane == 0) {                                   // (position -R / +R outside the reachable window: its sum is 0)
+          if (-a.R >= a.glo && -a.R < a.glo + a.gw) part[-a.R - a.glo] = fl;
+          if (a.R >= a.glo && a.R < a.glo + a.gw) part[a.R - a.glo] = fr;
+        }
+      }
+    }
+  }
+  dma_wait();
+  __syncthreads();
+  if (k0 >= a.Sk) return;
+  bf16_t* slab = stage + wave * 32 * 72;
+  if (!kok) {                                              // lane = key: its rows are zeros, whatever the unmasked arithmetic left in them
+#pragma unroll
+    for (int m = 0; m < MAPS; m++)
+#pragma unroll
+      for (int i = 0; i < ND; i++) zero(dk[m][i]);
+#pragma unroll
+    for (int i = 0; i < NDV; i++) zero(dv[i]);
+  }
+#pragma unroll
+  for (int m = 0; m < MAPS; m++)
+    store_rows<HALF, D>(dk[m], a.scale, slab, lane, [=](int row) -> bf16_t* {
+      return k0 + row < a.Sk ? a.dk + ((((size_t)b * a.Sk + k0 + row) * a.Hkv + kh) * MAPS + m) * D : nullptr; });
+  store_rows<HALF, DV>(dv, 1.f, slab, lane, [=](int row) -> bf16_t* {
+    return k0 + row < a.Sk ? a.dv + (((size_t)b * a.Sk + k0 + row) * a.Hkv + kh) * DV : nullptr; });
+}
+
+// ------------------------------------------------------------------------------------------------
+// bias table's gradient: part [H][B x 32-key blocks][gw] -> sums over a chunk of rows -> sums over the positions of a bucket.  Fixed order.
+// ------------------------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void diag_sum_kernel(const float* part, long long rows, int gw, int chunk, float* out) {
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = blockIdx.x * 64 + lane, h = blockIdx.z;
+  const long long r0 = (long long)blockIdx.y * chunk, r1 = r0 + chunk < rows ? r0 + chunk : rows;
+  float x = 0.f;
+  if (col < gw) {
+#pragma unroll 4
+    for (long long r = r0 + w; r < r1; r += 4) x += part[(h * rows + r) * gw + col];
+  }
+  red[w][lane] = x;
+  __syncthreads();
+  if (w == 0 && col < gw) out[((size_t)h * gridDim.y + blockIdx.y) * gw + col] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+}
+__global__ __launch_bounds__(64) void bucket_sum_kernel(const float* sums, int chunks, int gw, int glo, const int* buckets, int R, int NB, int H, float* dtable) {
+  const int bk = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
+  double x = 0.;
+  for (int i = lane; i < gw; i += 64) {
+    const int rel = min(max(glo + i, -R), R);
+    if (min(max(buckets[rel + R], 0), NB - 1) != bk) continue;
+    for (int c = 0; c < chunks; c++) x += (double)sums[((size_t)h * chunks + c) * gw + i];
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+  if (lane == 0) dtable[(size_t)bk * H + h] = (float)x;
+}
+// lam's gradient: minus the sum of a head's n partial row sums
+__global__ __launch_bounds__(256) void lam_sum_kernel(const float* part, long long n, float* dlam) {
+  __shared__ double red[4];
+  const float* p = part + (size_t)blockIdx.x * n;
+  double x = 0.;
+#pragma unroll 8
+  for (long long i = threadIdx.x; i < n; i += 256) x += (double)p[i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+  __syncthreads();
+  if (threadIdx.x == 0) dlam[blockIdx.x] = -(float)((red[0] + red[1]) + (red[2] + red[3]));
+}
+
+// ------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------
+constexpr int MAX_REACH = 8191, MAX_BUCKETS = 1 << 16;
+constexpr int DIAG_BYTES = 4 * 2 * 64 * 4;
+
+int check_attn(const uvtg_attn_dims* d, int maps) {
+  if (!d) return -10;
+  if (d->struct_size != (int)sizeof(uvtg_attn_dims)) return -18;
+  if (d->B <= 0 || d->H <= 0 || d->Hkv <= 0 || d->Sq <= 0 || d->Sk <= 0) return -11;
+  if (d->dtype != 0 && d->dtype != 1) return -30;
+  if (d->H % d->Hkv) return -31;
+  if (d->D != 32 && d->D != 64 && !(d->D == 128 && maps == 1)) return maps == 1 ? -5 : -32;
+  if (!(d->scale > 0.f) || !isfinite(d->scale)) return -33;
+  if (d->Sq > (1 << 24) || d->Sk > (1 << 24) || d->q_offset > (1 << 28) || d->q_offset < -(1 << 28)) return -34;
+  if ((long long)d->B * d->H > 65535 * 64ll || (long long)d->B * d->Hkv > 65535) return -34;
+  if ((long long)((d->Sq + 31) / 32) * d->B * d->H > 0x7fffffffll || (long long)((d->Sk + 31) / 32) * d->B * d->Hkv > 0x7fffffffll) return -34;
+  const long long st[] = {d->q_sb, d->q_ss, d->q_sh, d->k_sb, d->k_ss, d->k_sh, d->v_sb, d->v_ss, d->v_sh, maps == 2 ? d->q_sm : 0, maps == 2 ? d->k_sm : 0};
+  for (long long s : st) if (s % 8 || s < 0) return -35;
+  if (maps == 1) {
+    if (d->reach < 1 || d->reach > MAX_REACH) return -36;
+    if (d->n_buckets < 1 || d->n_buckets > MAX_BUCKETS) return -37;
+  }
+  return 0;
+}
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// Few rows or few workgroups: the split kernel (a row block of 32 instead of 128, the keys cut into ranges).  heads packed per row block, row
+// blocks per key head, key ranges
+struct SplitPlan { int use, hb, blocks, nsplit; };
+SplitPlan plan_split(const uvtg_attn_dims* d, int maps) {
+  SplitPlan p = {0, 1, 0, 1};
+  const int G = d->H / d->Hkv;
+  const long long wg = (long long)((d->Sq + 127) / 128) * d->H * d->B;
+  p.use = d->Sq <= 32 || (wg < 128 && d->Sk >= 512);
+  if (!p.use) return p;
+  if (d->Sq < 32) {
+    p.hb = 32 / d->Sq < G ? 32 / d->Sq : G;
+    const int win = maps == 1 ? (2 * d->reach + 1 < d->Sk + d->Sq ? 2 * d->reach + 1 : d->Sk + d->Sq) : 0;
+    while (p.hb > 1 && (long long)p.hb * win * 4 > 32768) p.hb--;
+  }
+  p.blocks = ((G + p.hb - 1) / p.hb) * ((p.hb * d->Sq + 31) / 32);
+  const long long base = (long long)p.blocks * d->B * d->Hkv;
+  const long long want = (512 + base - 1) / base, most = (d->Sk + 127) / 128;
+  p.nsplit = (int)(want < most ? want : most);
+  if (p.nsplit > 128) p.nsplit = 128;
+  if (p.nsplit < 1) p.nsplit = 1;
+  return p;
+}
+// relative positions that any (query, key) pair has, clamped to +-R
+void reachable(const uvtg_attn_dims* d, int& glo, int& gw) {
+  const int R = d->reach;
+  auto cl = [R](long long x) { return (int)(x < -R ? -R : x > R ? R : x); };
+  glo = cl(-(long long)(d->Sq - 1) - d->q_offset);
+  gw = cl((long long)d->Sk - 1 - d->q_offset) - glo + 1;
+}
+size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+struct BwdWs { size_t rvec, part, sums, total; long long rows; int chunk, chunks; };
+BwdWs bwd_ws(const uvtg_attn_dims* d, int maps) {
+  BwdWs w;
+  w.rvec = 0;
+  size_t at = align256((size_t)d->B * d->H * maps * d->Sq * 4);
+  w.part = at;
+  if (maps == 1) {
+    int glo, gw;
+    reachable(d, glo, gw);
+    w.rows = (long long)d->B * ((d->Sk + 31) / 32);
+    w.chunk = w.rows > 256 * 1024 ? (int)((w.rows + 1023) / 1024) : 256;
+    w.chunks = (int)((w.rows + w.chunk - 1) / w.chunk);
+    at += align256((size_t)d->H * w.rows * gw * 4);
+    w.sums = at;
+    at += align256((size_t)d->H * w.chunks * gw * 4);
+  } else {
+    w.rows = (long long)d->B * ((d->Sq + 31) / 32);
+    w.chunk = w.chunks = 0;
+    at += align256((size_t)d->H * w.rows * 4);
+    w.sums = at;
+  }
+  w.total = at;
+  return w;
+}
+
+MapArgs map_args(const uvtg_attn_dims* d) {
+  MapArgs a;
+  memset(&a, 0, sizeof(a));
+  a.q_sb = d->q_sb; a.q_ss = d->q_ss; a.q_sh = d->q_sh; a.q_sm = d->q_sm;
+  a.k_sb = d->k_sb; a.k_ss = d->k_ss; a.k_sh = d->k_sh; a.k_sm = d->k_sm;
+  a.v_sb = d->v_sb; a.v_ss = d->v_ss; a.v_sh = d->v_sh; a.mask_sb = d->kvalid_sb;
+  a.B = d->B; a.H = d->H; a.Hkv = d->Hkv; a.G = d->H / d->Hkv; a.Sq = d->Sq; a.Sk = d->Sk; a.NB = d->n_buckets; a.R = d->reach;
+  a.off = d->q_offset; a.causal = d->causal != 0; a.scale = d->scale; a.c = d->scale * LOG2E;
+  return a;
+}
+
+// entries of the bias window of a workgroup of `rows` rows
+size_t window_bytes(const uvtg_attn_dims* d, int maps, int rows, long long other) {
+  if (maps == 2) return 0;
+  const long long w = 2ll * (d->reach + PAD) + 1, most = other + rows + 192;
+  return (size_t)(w < most ? w : most) * 4;
+}
+
+template <bool HALF, int D, int MAPS> int run_fwd(const uvtg_attn_dims* d, MapArgs a, hipStream_t s) {
+  constexpr int DV = MAPS * D;
+  const SplitPlan p = plan_split(d, MAPS);
+  if (!p.use) {
+    const size_t lds = 2 * 64 * (MAPS * D + DV) * 2 + WIN * 8 + window_bytes(d, MAPS, 128, d->Sk);
+    hipLaunchKernelGGL((maps_fwd_kernel<HALF, D, MAPS>), dim3((unsigned)((d->Sq + 127) / 128) * d->H * d->B), dim3(256), lds, s, a);
+    UVTG_CHECK_LAUNCH();
+    return 0;
+  }
+  a.hb = p.hb; a.nsplit = p.nsplit;
+  constexpr size_t tiles = 4 * 32 * (MAPS * D + DV) * 2, sums = 4 * DV * 32 * 4;
+  const long long win = MAPS == 1 ? (2ll * d->reach + 1 < d->Sk + d->Sq + 64ll ? 2ll * d->reach + 1 : d->Sk + d->Sq + 64ll) : 0;
+  const size_t lds = (tiles > sums ? tiles : sums) + 2 * WIN * 4 + MAPS * 2 * 128 * 4 + (size_t)p.hb * win * 4;
+  hipLaunchKernelGGL((maps_fwd_split_kernel<HALF, D, MAPS>), dim3(p.blocks, p.nsplit, d->B * d->Hkv), dim3(256), lds, s, a);
+  UVTG_CHECK_LAUNCH();
+  if (p.nsplit > 1) {
+    hipLaunchKernelGGL((maps_join_kernel<HALF, D, MAPS>), dim3((unsigned)(((long long)d->B * d->H * d->Sq + 3) / 4)), dim3(256), 0, s, a);
+    UVTG_CHECK_LAUNCH();
+  }
+  return 0;
+}
+template <bool HALF, int D, int MAPS> int run_bwd(const uvtg_attn_dims* d, MapArgs a, float* dsum, char* ws, hipStream_t s) {
+  constexpr int DV = MAPS * D;
+  const BwdWs w = bwd_ws(d, MAPS);
+  a.rvec = (float*)(ws + w.rvec);
+  a.part = (MAPS == 2 || dsum) ? (float*)(ws + w.part) : nullptr;
+  if (MAPS == 1) reachable(d, a.glo, a.gw);
+  const size_t lds_q = 2 * 64 * (MAPS * D + DV) * 2 + WIN * 8 + window_bytes(d, MAPS, 128, d->Sk);
+  hipLaunchKernelGGL((maps_bwd_q_kernel<HALF, D, MAPS>), dim3((unsigned)((d->Sq + 127) / 128) * d->H * d->B), dim3(256), lds_q, s, a);
+  UVTG_CHECK_LAUNCH();
+  const size_t lds_k = 2 * 64 * (MAPS * D + DV) * 2 + 2 * MAPS * 2 * 64 * 4 + DIAG_BYTES + window_bytes(d, MAPS, 128, d->Sq);
+  hipLaunchKernelGGL((maps_bwd_k_kernel<HALF, D, MAPS>), dim3((unsigned)((d->Sk + 127) / 128) * d->Hkv * d->B), dim3(256), lds_k, s, a);
+  UVTG_CHECK_LAUNCH();
+  if (!dsum) return 0;
+  if (MAPS == 1) {
+    float* sums = (float*)(ws + w.sums);
+    hipLaunchKernelGGL(diag_sum_kernel, dim3((a.gw + 63) / 64, w.chunks, d->H), dim3(256), 0, s, a.part, w.rows, a.gw, w.chunk, sums);
+    UVTG_CHECK_LAUNCH();
+    hipLaunchKernelGGL(bucket_sum_kernel, dim3(d->n_buckets, d->H), dim3(64), 0, s, sums, w.chunks, a.gw, a.glo, a.buckets, a.R, a.NB, a.H, dsum);
+  } else hipLaunchKernelGGL(lam_sum_kernel, dim3(d->H), dim3(256), 0, s, a.part, w.rows, dsum);
+  UVTG_CHECK_LAUNCH();
+  return 0;
+}
+
+template <int MAPS> int dispatch_fwd(const uvtg_attn_dims* d, const MapArgs& a, hipStream_t s) {
+#define GO(D_) if (d->D == D_) return d->dtype ? run_fwd<true, D_, MAPS>(d, a, s) : run_fwd<false, D_, MAPS>(d, a, s);
+  GO(32) GO(64)
+  if constexpr (MAPS == 1) { GO(128) }
+#undef GO
+  return -5;
+}
+template <int MAPS> int dispatch_bwd(const uvtg_attn_dims* d, const MapArgs& a, float* dsum, char* ws, hipStream_t s) {
+#define GO(D_) if (d->D == D_) return d->dtype ? run_bwd<true, D_, MAPS>(d, a, dsum, ws, s) : run_bwd<false, D_, MAPS>(d, a, dsum, ws, s);
+  GO(32) GO(64)
+  if constexpr (MAPS == 1) { GO(128) }
+#undef GO
+  return -5;
+}
+
+}  // namespace
+
+extern "C" size_t uvtg_attn_ws_bytes(const uvtg_attn_dims* d, int maps, int backward) {
+  if ((maps != 1 && maps != 2) || check_attn(d, maps)) return 0;
+  if (backward) return bwd_ws(d, maps).total;
+  const SplitPlan p = plan_split(d, maps);
+  return p.use && p.nsplit > 1 ? (size_t)d->B * d->H * d->Sq * p.nsplit * maps * (maps * d->D + 2) * 4 : 0;
+}
+extern "C" int uvtg_relpos_attention_fwd(const uvtg_attn_dims* d, const void* q, const void* k, const void* v, const float* table, const int* buckets,
+                                         const unsigned char* kvalid, void* o, float* lse, void* ws, uvtg_stream_t st) {
+  if (int e = check_attn(d, 1)) return e;
+  if (!q || !k || !v || !table || !buckets || !o || (!ws && uvtg_attn_ws_bytes(d, 1, 0))) return -20;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o)) return -35;
+  MapArgs a = map_args(d);
+  a.q = (const bf16_t*)q; a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.table = table; a.buckets = buckets; a.kvalid = kvalid;
+  a.out = (bf16_t*)o; a.lse = lse; a.acc = (float*)ws;
+  return dispatch_fwd<1>(d, a, (hipStream_t)st);
+}
+extern "C" int uvtg_relpos_attention_bwd(const uvtg_attn_dims* d, const void* q, const void* k, const void* v, const float* table, const int* buckets,
+                                         const unsigned char* kvalid, const void* o, const float* lse, const void* dO, void* dq, void* dk, void* dv,
+                                         float* dtable, void* ws, uvtg_stream_t st) {
+  if (int e = check_attn(d, 1)) return e;
+  if (!q || !k || !v || !table || !buckets || !o || !lse || !dO || !dq || !dk || !dv || !ws) return -20;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(dO) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv)) return -35;
+  MapArgs a = map_args(d);
+  a.q = (const bf16_t*)q; a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.table = table; a.buckets = buckets; a.kvalid = kvalid;
+  a.o = (const bf16_t*)o; a.lse_in = lse; a.dO = (const bf16_t*)dO; a.dq = (bf16_t*)dq; a.dk = (bf16_t*)dk; a.dv = (bf16_t*)dv;
+  return dispatch_bwd<1>(d, a, dtable, (char*)ws, (hipStream_t)st);
+}
+extern "C" int uvtg_diff_attention_fwd(const uvtg_attn_dims* d, const void* q, const void* k, const void* v, const float* lam, const unsigned char* kvalid,
+                                       void* o, void* o2, float* lse, void* ws, uvtg_stream_t st) {
+  if (int e = check_attn(d, 2)) return e;
+  if (!q || !k || !v || !lam || !o || (!ws && uvtg_attn_ws_bytes(d, 2, 0))) return -20;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(o2)) return -35;
+  MapArgs a = map_args(d);
+  a.q = (const bf16_t*)q; a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.lam = lam; a.kvalid = kvalid;
+  a.out = (bf16_t*)o; a.out2 = (bf16_t*)o2; a.lse = lse; a.acc = (float*)ws;
+  return dispatch_fwd<2>(d, a, (hipStream_t)st);
+}
+extern "C" int uvtg_diff_attention_bwd(const uvtg_attn_dims* d, const void* q, const void* k, const void* v, const float* lam, const unsigned char* kvalid,
+                                       const void* o, const void* o2, const float* lse, const void* dO, void* dq, void* dk, void* dv, float* dlam, void* ws,
+                                       uvtg_stream_t st) {
+  if (int e = check_attn(d, 2)) return e;
+  if (!q || !k || !v || !lam || !o || !o2 || !lse || !dO || !dq || !dk || !dv || !ws) return -20;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(o2) || !aligned16(dO) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv))
+    return -35;
+  MapArgs a = map_args(d);
+  a.q = (const bf16_t*)q; a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.lam = lam; a.kvalid = kvalid;
+  a.o = (const bf16_t*)o; a.o2 = (const bf16_t*)o2; a.lse_in = lse; a.dO = (const bf16_t*)dO; a.dq = (bf16_t*)dq; a.dk = (bf16_t*)dk; a.dv = (bf16_t*)dv;
+  return dispatch_bwd<2>(d, a, dlam, (char*)ws, (hipStream_t)st);
+}

@@ -534,6 +534,14 @@ extern "C" const char* uvtg_strerror(int code) {
     case -23: return "lens_host: every sample needs 1 <= len_v <= Lv clips and 1 <= len_t <= Lt text tokens";
     case -25: return "dims: precise must be 0 (bf16 operands) or 1 (fp16 hi + lo operand images)";
     case -24: return "forward: the memory output cannot be requested in a bf16 training call (neither the packed stream nor the last layer's clip-row tail computes its text rows)";
+    case -30: return "attention: dtype must be 0 (bf16) or 1 (fp16)";
+    case -31: return "attention: H must be a multiple of Hkv";
+    case -32: return "differential attention: head_dim of a map must be 32 or 64";
+    case -33: return "attention: scale must be positive and finite";
+    case -34: return "attention: length, offset or batch x heads beyond what the kernels address";
+    case -35: return "attention: strides and addresses must be non-negative multiples of 16 bytes";
+    case -36: return "attention: reach must be 1 .. 8191";
+    case -37: return "attention: n_buckets must be 1 .. 65536";
     default: return "invalid argument";
   }
 }

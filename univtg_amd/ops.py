@@ -210,3 +210,166 @@ def postprocess_mr(pred_logits, pred_spans, saliency, timestamp, timestamp_mask,
                                                float(clip_length), int(eval_mode == "add"), float(nms_thd), int(max_before), int(max_after),
                                                _ptr(win), _ptr(order), _ptr(keep), _ptr(nk), _ptr(sal_out), _stream()), "uvtg_postprocess_mr")
     return win, order, keep, nk, sal_out
+
+
+# ---- attention over score maps: learned relative position bias by buckets, differential heads -------------------------------------------
+_ATTN_TYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+
+def relpos_buckets(num_buckets, max_distance, bidirectional=True, device="cuda"):
+    """Bucket of every relative position (key minus query) -max_distance .. max_distance, int32 [2 * max_distance + 1]: the lower half of the
+    buckets holds one distance each, the upper half is spaced evenly in the logarithm up to max_distance, from where on the last one holds all.
+    bidirectional: half of the buckets for keys behind the query (and at it), half for keys ahead; else keys ahead share bucket 0.
+    Borders are found in whole numbers, so that none depends on how a logarithm is rounded."""
+    n = num_buckets // 2 if bidirectional else num_buckets
+    exact = n // 2
+    if n < 2 or (bidirectional and num_buckets % 2) or max_distance <= exact:
+        raise ValueError(f"relpos_buckets: {num_buckets} buckets cannot be spaced up to a distance of {max_distance}")
+    steps, b, behind = n - exact, 0, []
+    for d in range(max_distance + 1):
+        if d < exact:
+            behind.append(d)
+            continue
+        # bucket exact + b from (d / exact) ** steps >= (max_distance / exact) ** b on
+        while b < steps - 1 and d ** steps * exact ** (b + 1) >= max_distance ** (b + 1) * exact ** steps:
+            b += 1
+        behind.append(exact + b)
+    ahead = [n + b for b in behind[1:]] if bidirectional else [behind[0]] * max_distance
+    return torch.tensor(behind[::-1] + ahead, dtype=torch.int32, device=device)
+
+
+def _attn_operand(t):
+    """t as the kernels address it: channels contiguous, every other stride and the address a multiple of 16 bytes (else a contiguous copy)."""
+    st = t.stride()
+    if st[-1] == 1 and t.data_ptr() % 16 == 0:
+        for n, s in zip(t.shape[:-1], st[:-1]):
+            if n > 1 and s % 8:
+                break
+        else:
+            return t
+    return t.contiguous() if t.data_ptr() % 16 == 0 or not t.is_contiguous() else t.clone(memory_format=torch.contiguous_format)
+
+
+def _attn_call(name, maps, q, k, v, kvalid, q_offset, causal, scale):
+    """Checks and lays out the operands both attentions share: (dims, q, k, v, kvalid)."""
+    _need_cuda(q)
+    nd = 3 + maps
+    if q.dim() != nd or k.dim() != nd or v.dim() != 4:
+        raise ValueError(f"{name}: q and k must be [B, S, heads, {'2, ' if maps == 2 else ''}D] and v [B, Sk, Hkv, {'2 D' if maps == 2 else 'D'}]")
+    B, Sq, H = q.shape[:3]
+    Sk, Hkv, D = k.shape[1], k.shape[2], q.shape[-1]
+    m = (2,) if maps == 2 else ()
+    if tuple(q.shape[3:-1]) != m or tuple(k.shape) != (B, Sk, Hkv, *m, D) or tuple(v.shape) != (B, Sk, Hkv, maps * D):
+        raise ValueError(f"{name}: shapes do not agree: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if q.dtype not in _ATTN_TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"{name}: q, k and v must all be bfloat16 or all float16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if k.device != q.device or v.device != q.device or (kvalid is not None and kvalid.device != q.device):
+        raise ValueError(f"{name}: every operand must be on {q.device}")
+    q, k, v = _attn_operand(q), _attn_operand(k), _attn_operand(v)
+    if kvalid is not None:
+        if kvalid.dtype not in (torch.uint8, torch.bool) or tuple(kvalid.shape) != (B, Sk):
+            raise ValueError(f"{name}: kvalid must be uint8 or bool [B, Sk] = [{B}, {Sk}], got {kvalid.dtype} {tuple(kvalid.shape)}")
+        if kvalid.stride(1) != 1 or kvalid.stride(0) < 0:
+            kvalid = kvalid.contiguous()
+    qs, ks, vs = ([s if n > 1 else 0 for n, s in zip(t.shape, t.stride())] for t in (q, k, v))
+    d = _lib.AttnDims(dtype=_ATTN_TYPES[q.dtype], B=B, H=H, Hkv=Hkv, D=D, Sq=Sq, Sk=Sk, causal=int(bool(causal)), q_offset=int(q_offset),
+                      scale=D ** -0.5 if scale is None else float(scale), q_sb=qs[0], q_ss=qs[1], q_sh=qs[2], q_sm=qs[3] if maps == 2 else 0,
+                      k_sb=ks[0], k_ss=ks[1], k_sh=ks[2], k_sm=ks[3] if maps == 2 else 0, v_sb=vs[0], v_ss=vs[1], v_sh=vs[2],
+                      kvalid_sb=0 if kvalid is None else kvalid.stride(0))
+    return d, q, k, v, kvalid
+
+
+def _attn_ws(d, maps, backward, device):
+    n = _lib.load().uvtg_attn_ws_bytes(C.byref(d), maps, backward)
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def _relpos_operands(d, q, table, buckets):
+    if table.dim() != 2 or table.shape[1] != d.H or table.device != q.device:
+        raise ValueError(f"relpos_attention: table must be [n_buckets, H = {d.H}] on {q.device}, got {tuple(table.shape)} on {table.device}")
+    if buckets.dim() != 1 or buckets.dtype != torch.int32 or buckets.numel() % 2 == 0 or buckets.device != q.device:
+        raise ValueError(f"relpos_attention: buckets must be int32 [2 * reach + 1] on {q.device}, got {buckets.dtype} {tuple(buckets.shape)} on {buckets.device}")
+    d.n_buckets, d.reach = table.shape[0], buckets.numel() // 2
+    return _f32c(table), buckets.contiguous()
+
+
+def _attn_saved(name, t, like, what):
+    if t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name}: {what} must be {like.dtype} on {like.device}")
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def relpos_attention_fwd(q, k, v, table, buckets, kvalid=None, q_offset=0, causal=False, scale=None):
+    """softmax(scale q k^T + table[buckets[clamp(j - i - q_offset)], h]) v: q [B, Sq, H, D], k and v [B, Sk, Hkv, D] (bf16 or fp16, D 32 / 64 / 128,
+    any strides), table [n_buckets, H] fp32, buckets int32 [2 reach + 1] (relpos_buckets), kvalid [B, Sk] uint8 / bool (0 = masked key).  causal:
+    query i sees keys up to i + q_offset.  scale defaults to D ** -0.5.  Returns o [B, Sq, H, D] and lse [B, H, Sq] (fp32); a row that sees no key
+    is 0 with lse -inf."""
+    with torch.cuda.device_of(q):
+        d, q, k, v, kvalid = _attn_call("relpos_attention", 1, q, k, v, kvalid, q_offset, causal, scale)
+        table, buckets = _relpos_operands(d, q, table, buckets)
+        o = torch.empty(d.B, d.Sq, d.H, d.D, dtype=q.dtype, device=q.device)
+        lse = torch.empty(d.B, d.H, d.Sq, dtype=torch.float32, device=q.device)
+        ws = _attn_ws(d, 1, 0, q.device)
+        _lib.check(_lib.load().uvtg_relpos_attention_fwd(C.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(table), _ptr(buckets), _ptr(kvalid), _ptr(o), _ptr(lse),
+                                                         _ptr(ws), _stream()), "uvtg_relpos_attention_fwd")
+    return o, lse
+
+
+def relpos_attention_bwd(do, q, k, v, table, buckets, o, lse, kvalid=None, q_offset=0, causal=False, scale=None, need_dtable=True):
+    """Gradients of relpos_attention_fwd from its outputs and do: dq, dk, dv (the operands' type, contiguous) and dtable (fp32, or None)."""
+    with torch.cuda.device_of(q):
+        d, q, k, v, kvalid = _attn_call("relpos_attention", 1, q, k, v, kvalid, q_offset, causal, scale)
+        table, buckets = _relpos_operands(d, q, table, buckets)
+        if tuple(do.shape) != (d.B, d.Sq, d.H, d.D) or o.shape != do.shape or tuple(lse.shape) != (d.B, d.H, d.Sq):
+            raise ValueError("relpos_attention_bwd: do and o must be [B, Sq, H, D], lse [B, H, Sq]")
+        do, o = _attn_saved("relpos_attention_bwd", do, q, "do"), _attn_saved("relpos_attention_bwd", o, q, "o")
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+        dv = torch.empty(v.shape, dtype=q.dtype, device=q.device)
+        dtable = torch.empty(table.shape, dtype=torch.float32, device=q.device) if need_dtable else None
+        ws = _attn_ws(d, 1, 1, q.device)
+        _lib.check(_lib.load().uvtg_relpos_attention_bwd(C.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(table), _ptr(buckets), _ptr(kvalid), _ptr(o),
+                                                         _ptr(_f32c(lse)), _ptr(do), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable), _ptr(ws), _stream()),
+                   "uvtg_relpos_attention_bwd")
+    return dq, dk, dv, dtable
+
+
+def _lam_operand(d, q, lam):
+    if tuple(lam.shape) != (d.H,) or lam.device != q.device:
+        raise ValueError(f"diff_attention: lam must be [H = {d.H}] on {q.device}, got {tuple(lam.shape)} on {lam.device}")
+    return _f32c(lam)
+
+
+def diff_attention_fwd(q, k, v, lam, kvalid=None, q_offset=0, causal=False, scale=None, need_o2=False):
+    """Differential attention (softmax(scale q1 k1^T) - lam[h] softmax(scale q2 k2^T)) v: q [B, Sq, H, 2, D], k [B, Sk, Hkv, 2, D], v [B, Sk, Hkv, 2 D]
+    (bf16 or fp16, D 32 / 64, any strides), lam [H] fp32; kvalid, q_offset, causal and scale as in relpos_attention_fwd.  Returns o [B, Sq, H, 2 D]
+    and lse [B, H, 2, Sq] (fp32), and with need_o2 also o2, the second map's own output, which the backward pass reads."""
+    with torch.cuda.device_of(q):
+        d, q, k, v, kvalid = _attn_call("diff_attention", 2, q, k, v, kvalid, q_offset, causal, scale)
+        lam = _lam_operand(d, q, lam)
+        o = torch.empty(d.B, d.Sq, d.H, 2 * d.D, dtype=q.dtype, device=q.device)
+        o2 = torch.empty_like(o) if need_o2 else None
+        lse = torch.empty(d.B, d.H, 2, d.Sq, dtype=torch.float32, device=q.device)
+        ws = _attn_ws(d, 2, 0, q.device)
+        _lib.check(_lib.load().uvtg_diff_attention_fwd(C.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(lam), _ptr(kvalid), _ptr(o), _ptr(o2), _ptr(lse),
+                                                       _ptr(ws), _stream()), "uvtg_diff_attention_fwd")
+    return (o, lse, o2) if need_o2 else (o, lse)
+
+
+def diff_attention_bwd(do, q, k, v, lam, o, o2, lse, kvalid=None, q_offset=0, causal=False, scale=None, need_dlam=True):
+    """Gradients of diff_attention_fwd(need_o2=True) from its outputs and do: dq, dk, dv (the operands' type, contiguous) and dlam (fp32, or None)."""
+    with torch.cuda.device_of(q):
+        d, q, k, v, kvalid = _attn_call("diff_attention", 2, q, k, v, kvalid, q_offset, causal, scale)
+        lam = _lam_operand(d, q, lam)
+        if tuple(do.shape) != (d.B, d.Sq, d.H, 2 * d.D) or o.shape != do.shape or o2.shape != do.shape or tuple(lse.shape) != (d.B, d.H, 2, d.Sq):
+            raise ValueError("diff_attention_bwd: do, o and o2 must be [B, Sq, H, 2 D], lse [B, H, 2, Sq]")
+        do, o, o2 = (_attn_saved("diff_attention_bwd", t, q, w) for t, w in ((do, "do"), (o, "o"), (o2, "o2")))
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+        dv = torch.empty(v.shape, dtype=q.dtype, device=q.device)
+        dlam = torch.empty(d.H, dtype=torch.float32, device=q.device) if need_dlam else None
+        ws = _attn_ws(d, 2, 1, q.device)
+        _lib.check(_lib.load().uvtg_diff_attention_bwd(C.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(lam), _ptr(kvalid), _ptr(o), _ptr(o2), _ptr(_f32c(lse)),
+                                                       _ptr(do), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dlam), _ptr(ws), _stream()), "uvtg_diff_attention_bwd")
+    return dq, dk, dv, dlam
