@@ -244,18 +244,31 @@ def test_no_cpu_fallback():
 
 def test_capture_is_refused_while_a_foreign_graph_of_a_leaf_lives():
     from univtg_amd import attention
+
+    class Twice(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, y):
+            return x * 2 + y
+
+        @staticmethod
+        def backward(ctx, g):
+            return g * 2, g
+
     x, y = torch.zeros(3, requires_grad=True), torch.zeros(3)
-    attention._leaves_stream((x, y), 1, False)
-    attention._leaves_stream((x, y), 2, True)                # no graph of x is alive: its accumulator is new each time
-    alive = x * 2
-    attention._leaves_stream((x, y), 1, False)
-    attention._leaves_stream((x, y), 1, True)
-    attention._leaves_stream((x, y), 2, False)
+    alive = attention._apply(Twice, (x, y), x, y)            # noted on x for stream 0
+    attention._refuse_foreign([x], 0)
     with pytest.raises(RuntimeError, match="still holds a leaf"):
-        attention._leaves_stream((x, y), 2, True)
+        attention._refuse_foreign([x], 2)
+    kept = alive * 3                                         # the graph lives on behind a result
+    for _ in range(3):
+        attention._apply(Twice, (x, y), x, y)
+    assert len(x._attention_graphs) == 2                     # the graphs that died are forgotten
     del alive
-    attention._leaves_stream((x, y), 2, True)
-    attention._leaves_stream((x * 2,), 7, True)              # not a leaf
+    with pytest.raises(RuntimeError, match="still holds a leaf"):
+        attention._refuse_foreign([x], 2)
+    del kept
+    attention._refuse_foreign([x], 2)
+    assert not hasattr(y, "_attention_graphs")
 
 
 def test_reference_against_differences():
@@ -572,8 +585,8 @@ def test_captured_training_step():
     refused = 0
     for x in (own, leaves):
         if x is leaves:
-            with pytest.raises(RuntimeError, match="still holds a leaf"), torch.cuda.stream(torch.cuda.Stream()):
-                attention._leaves_stream(leaves, torch.cuda.current_stream().cuda_stream, True)
+            with pytest.raises(RuntimeError, match="still holds a leaf"):
+                attention._refuse_foreign(leaves, torch.cuda.Stream().cuda_stream)
             refused += 1
             assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(alive, leaves, do), want))
             del alive                                        # the last eager graph of these leaves: now they may be captured

@@ -10,6 +10,8 @@ Under `torch.no_grad()`, or when nothing requires a gradient, they are the forwa
 values (`q_offset` = how many came before) run the kernel that splits the keys."""
 from __future__ import annotations
 
+import weakref
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -48,28 +50,31 @@ class _DiffAttention(torch.autograd.Function):
         return dq, dk, dv, dlam, None, None
 
 
-_STREAM = "univtg_amd.attention.stream"
+def _apply(function, leaves, *args):
+    """function.apply(*args), which differentiates `leaves`.  A gradient accumulator lives as long as some autograd graph of its leaf does, and autograd's
+    engine makes the stream it was made on wait for a backward pass: during a capture that joins a stream outside it, which ends the process in
+    capture_end, not in an error.  So every graph made here is noted on its leaves, and a capture is refused while one of another stream is alive."""
+    on_gpu = leaves[0].is_cuda
+    stream = torch.cuda.current_stream(leaves[0].device).cuda_stream if on_gpu else 0
+    leaves = [t for t in leaves if t.requires_grad and t.is_leaf]
+    if on_gpu and leaves and torch.cuda.is_current_stream_capturing():
+        _refuse_foreign(leaves, stream)
+    o = function.apply(*args)
+    if leaves:
+        note = (weakref.ref(o.grad_fn), stream)
+        for t in leaves:
+            t._attention_graphs = [n for n in getattr(t, "_attention_graphs", ()) if n[0]() is not None] + [note]
+    return o
 
 
-def _leaves_stream(tensors, stream, capturing):
-    """Notes on the gradient accumulator of every leaf the stream it was made for, and refuses a capture while one of another stream is alive.  An
-    accumulator lives as long as some autograd graph of its leaf does, and autograd's engine makes its stream wait for the backward pass: during a
-    capture that joins a stream outside it, which ends the process in capture_end, not in an error."""
-    for t in tensors:
-        if t.requires_grad and t.is_leaf:
-            note = torch.autograd.graph.get_gradient_edge(t).node.metadata
-            if note.setdefault(_STREAM, stream) != stream and capturing:
-                raise RuntimeError("attention: an autograd graph made outside this capture still holds a leaf of the captured call; release its outputs "
-                                   "before the capture, or pass the captured call leaves of its own")
+def _refuse_foreign(leaves, stream):
+    if any(ref() is not None and s != stream for t in leaves for ref, s in getattr(t, "_attention_graphs", ())):
+        raise RuntimeError("attention: an autograd graph made outside this capture still holds a leaf of the captured call; release its outputs "
+                           "before the capture, or pass the captured call leaves of its own")
 
 
 def _needs_grad(*tensors):
-    if not torch.is_grad_enabled() or not any(t.requires_grad for t in tensors):
-        return False
-    if tensors[0].is_cuda:
-        with torch.cuda.device_of(tensors[0]):
-            _leaves_stream(tensors, torch.cuda.current_stream().cuda_stream, torch.cuda.is_current_stream_capturing())
-    return True
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
 def relpos_attention(q, k, v, table, buckets, kvalid=None, q_offset=0, causal=False, scale=None):
@@ -78,7 +83,8 @@ def relpos_attention(q, k, v, table, buckets, kvalid=None, q_offset=0, causal=Fa
     opts = (q_offset, causal, scale)
     if not _needs_grad(q, k, v, table):
         return ops.relpos_attention_fwd(q, k, v, table, buckets, kvalid, *opts)[0]
-    return _RelposAttention.apply(q, k, v, table.float(), buckets, kvalid, opts)
+    table = table.float()
+    return _apply(_RelposAttention, (q, k, v, table), q, k, v, table, buckets, kvalid, opts)
 
 
 def diff_attention(q, k, v, lam, kvalid=None, q_offset=0, causal=False, scale=None):
@@ -86,4 +92,5 @@ def diff_attention(q, k, v, lam, kvalid=None, q_offset=0, causal=False, scale=No
     opts = (q_offset, causal, scale)
     if not _needs_grad(q, k, v, lam):
         return ops.diff_attention_fwd(q, k, v, lam, kvalid, *opts)[0]
-    return _DiffAttention.apply(q, k, v, lam.float(), kvalid, opts)
+    lam = lam.float()
+    return _apply(_DiffAttention, (q, k, v, lam), q, k, v, lam, kvalid, opts)

@@ -239,49 +239,57 @@ def relpos_buckets(num_buckets, max_distance, bidirectional=True, device="cuda")
 
 
 def _attn_operand(t):
-    """t as the kernels address it: channels contiguous, every other stride and the address a multiple of 16 bytes (else a contiguous copy)."""
+    """t as the kernels address it and its strides: channels contiguous, every other stride and the address a multiple of 16 bytes (else a contiguous
+    copy); the stride of an axis of one entry is never used."""
     st = t.stride()
     if st[-1] == 1 and t.data_ptr() % 16 == 0:
-        for n, s in zip(t.shape[:-1], st[:-1]):
-            if n > 1 and s % 8:
+        if 1 in t.shape:
+            st = [s if n > 1 else 0 for n, s in zip(t.shape, st)]
+        for s in st[:-1]:
+            if s % 8:
                 break
         else:
-            return t
-    return t.contiguous() if t.data_ptr() % 16 == 0 or not t.is_contiguous() else t.clone(memory_format=torch.contiguous_format)
+            return t, st
+    t = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+    return t, t.stride()
 
 
 def _attn_call(name, maps, q, k, v, kvalid, q_offset, causal, scale):
     """Checks and lays out the operands both attentions share: (dims, q, k, v, kvalid)."""
-    _need_cuda(q)
-    nd = 3 + maps
-    if q.dim() != nd or k.dim() != nd or v.dim() != 4:
+    qs, ks, vs, dtype, dev = q.shape, k.shape, v.shape, q.dtype, q.device
+    if len(qs) != 3 + maps or len(ks) != 3 + maps or len(vs) != 4:
         raise ValueError(f"{name}: q and k must be [B, S, heads, {'2, ' if maps == 2 else ''}D] and v [B, Sk, Hkv, {'2 D' if maps == 2 else 'D'}]")
-    B, Sq, H = q.shape[:3]
-    Sk, Hkv, D = k.shape[1], k.shape[2], q.shape[-1]
-    m = (2,) if maps == 2 else ()
-    if tuple(q.shape[3:-1]) != m or tuple(k.shape) != (B, Sk, Hkv, *m, D) or tuple(v.shape) != (B, Sk, Hkv, maps * D):
-        raise ValueError(f"{name}: shapes do not agree: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    if q.dtype not in _ATTN_TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+    B, Sq, H, D, Sk, Hkv = qs[0], qs[1], qs[2], qs[-1], ks[1], ks[2]
+    if (maps == 2 and (qs[3] != 2 or ks[3] != 2)) or ks[0] != B or ks[-1] != D or vs != (B, Sk, Hkv, maps * D):
+        raise ValueError(f"{name}: shapes do not agree: q {tuple(qs)}, k {tuple(ks)}, v {tuple(vs)}")
+    if dtype not in _ATTN_TYPES or k.dtype != dtype or v.dtype != dtype:
         raise ValueError(f"{name}: q, k and v must all be bfloat16 or all float16, got {q.dtype}, {k.dtype}, {v.dtype}")
-    if k.device != q.device or v.device != q.device or (kvalid is not None and kvalid.device != q.device):
-        raise ValueError(f"{name}: every operand must be on {q.device}")
-    q, k, v = _attn_operand(q), _attn_operand(k), _attn_operand(v)
+    if k.device != dev or v.device != dev or (kvalid is not None and kvalid.device != dev):
+        raise ValueError(f"{name}: every operand must be on {dev}")
+    q, qs = _attn_operand(q)
+    k, ks = _attn_operand(k)
+    v, vs = _attn_operand(v)
+    mask_sb = 0
     if kvalid is not None:
-        if kvalid.dtype not in (torch.uint8, torch.bool) or tuple(kvalid.shape) != (B, Sk):
+        if kvalid.dtype not in (torch.uint8, torch.bool) or kvalid.shape != (B, Sk):
             raise ValueError(f"{name}: kvalid must be uint8 or bool [B, Sk] = [{B}, {Sk}], got {kvalid.dtype} {tuple(kvalid.shape)}")
-        if kvalid.stride(1) != 1 or kvalid.stride(0) < 0:
+        if kvalid.stride(1) != 1:
             kvalid = kvalid.contiguous()
-    qs, ks, vs = ([s if n > 1 else 0 for n, s in zip(t.shape, t.stride())] for t in (q, k, v))
-    d = _lib.AttnDims(dtype=_ATTN_TYPES[q.dtype], B=B, H=H, Hkv=Hkv, D=D, Sq=Sq, Sk=Sk, causal=int(bool(causal)), q_offset=int(q_offset),
-                      scale=D ** -0.5 if scale is None else float(scale), q_sb=qs[0], q_ss=qs[1], q_sh=qs[2], q_sm=qs[3] if maps == 2 else 0,
-                      k_sb=ks[0], k_ss=ks[1], k_sh=ks[2], k_sm=ks[3] if maps == 2 else 0, v_sb=vs[0], v_ss=vs[1], v_sh=vs[2],
-                      kvalid_sb=0 if kvalid is None else kvalid.stride(0))
+        mask_sb = kvalid.stride(0)
+    d = _lib.AttnDims(0, _ATTN_TYPES[dtype], B, H, Hkv, D, Sq, Sk, 1 if causal else 0, int(q_offset), D ** -0.5 if scale is None else float(scale), 0, 0,
+                      qs[0], qs[1], qs[2], qs[3] if maps == 2 else 0, ks[0], ks[1], ks[2], ks[3] if maps == 2 else 0, vs[0], vs[1], vs[2], mask_sb)
     return d, q, k, v, kvalid
 
 
-def _attn_ws(d, maps, backward, device):
-    n = _lib.load().uvtg_attn_ws_bytes(C.byref(d), maps, backward)
+def _attn_ws(lib, d, maps, backward, device):
+    n = lib.uvtg_attn_ws_bytes(d, maps, backward)
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def _elsewhere(t):
+    """Whether t is on another GPU than the current one, whose streams the call would then use."""
+    _need_cuda(t)
+    return t.device.index != torch.cuda.current_device()
 
 
 def _relpos_operands(d, q, table, buckets):
@@ -300,43 +308,51 @@ def _attn_saved(name, t, like, what):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
 def relpos_attention_fwd(q, k, v, table, buckets, kvalid=None, q_offset=0, causal=False, scale=None):
     """softmax(scale q k^T + table[buckets[clamp(j - i - q_offset)], h]) v: q [B, Sq, H, D], k and v [B, Sk, Hkv, D] (bf16 or fp16, D 32 / 64 / 128,
     any strides), table [n_buckets, H] fp32, buckets int32 [2 reach + 1] (relpos_buckets), kvalid [B, Sk] uint8 / bool (0 = masked key).  causal:
     query i sees keys up to i + q_offset.  scale defaults to D ** -0.5.  Returns o [B, Sq, H, D] and lse [B, H, Sq] (fp32); a row that sees no key
     is 0 with lse -inf."""
-    with torch.cuda.device_of(q):
-        d, q, k, v, kvalid = _attn_call("relpos_attention", 1, q, k, v, kvalid, q_offset, causal, scale)
-        table, buckets = _relpos_operands(d, q, table, buckets)
-        o = torch.empty(d.B, d.Sq, d.H, d.D, dtype=q.dtype, device=q.device)
-        lse = torch.empty(d.B, d.H, d.Sq, dtype=torch.float32, device=q.device)
-        ws = _attn_ws(d, 1, 0, q.device)
-        _lib.check(_lib.load().uvtg_relpos_attention_fwd(C.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(table), _ptr(buckets), _ptr(kvalid), _ptr(o), _ptr(lse),
-                                                         _ptr(ws), _stream()), "uvtg_relpos_attention_fwd")
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return relpos_attention_fwd(q, k, v, table, buckets, kvalid, q_offset, causal, scale)
+    lib = _lib.load()
+    d, q, k, v, kvalid = _attn_call("relpos_attention", 1, q, k, v, kvalid, q_offset, causal, scale)
+    table, buckets = _relpos_operands(d, q, table, buckets)
+    o = torch.empty((d.B, d.Sq, d.H, d.D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((d.B, d.H, d.Sq), dtype=torch.float32, device=q.device)
+    ws = _attn_ws(lib, d, 1, 0, q.device)
+    _lib.check(lib.uvtg_relpos_attention_fwd(d, _at(q), _at(k), _at(v), _at(table), _at(buckets), _at(kvalid), _at(o), _at(lse), _at(ws), _stream()),
+               "uvtg_relpos_attention_fwd")
     return o, lse
 
 
 def relpos_attention_bwd(do, q, k, v, table, buckets, o, lse, kvalid=None, q_offset=0, causal=False, scale=None, need_dtable=True):
     """Gradients of relpos_attention_fwd from its outputs and do: dq, dk, dv (the operands' type, contiguous) and dtable (fp32, or None)."""
-    with torch.cuda.device_of(q):
-        d, q, k, v, kvalid = _attn_call("relpos_attention", 1, q, k, v, kvalid, q_offset, causal, scale)
-        table, buckets = _relpos_operands(d, q, table, buckets)
-        if tuple(do.shape) != (d.B, d.Sq, d.H, d.D) or o.shape != do.shape or tuple(lse.shape) != (d.B, d.H, d.Sq):
-            raise ValueError("relpos_attention_bwd: do and o must be [B, Sq, H, D], lse [B, H, Sq]")
-        do, o = _attn_saved("relpos_attention_bwd", do, q, "do"), _attn_saved("relpos_attention_bwd", o, q, "o")
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-        dv = torch.empty(v.shape, dtype=q.dtype, device=q.device)
-        dtable = torch.empty(table.shape, dtype=torch.float32, device=q.device) if need_dtable else None
-        ws = _attn_ws(d, 1, 1, q.device)
-        _lib.check(_lib.load().uvtg_relpos_attention_bwd(C.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(table), _ptr(buckets), _ptr(kvalid), _ptr(o),
-                                                         _ptr(_f32c(lse)), _ptr(do), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable), _ptr(ws), _stream()),
-                   "uvtg_relpos_attention_bwd")
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return relpos_attention_bwd(do, q, k, v, table, buckets, o, lse, kvalid, q_offset, causal, scale, need_dtable)
+    lib = _lib.load()
+    d, q, k, v, kvalid = _attn_call("relpos_attention", 1, q, k, v, kvalid, q_offset, causal, scale)
+    table, buckets = _relpos_operands(d, q, table, buckets)
+    if do.shape != (d.B, d.Sq, d.H, d.D) or o.shape != do.shape or lse.shape != (d.B, d.H, d.Sq):
+        raise ValueError("relpos_attention_bwd: do and o must be [B, Sq, H, D], lse [B, H, Sq]")
+    do, o = _attn_saved("relpos_attention_bwd", do, q, "do"), _attn_saved("relpos_attention_bwd", o, q, "o")
+    lse = _f32c(lse)
+    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
+    dtable = torch.empty(table.shape, dtype=torch.float32, device=q.device) if need_dtable else None
+    ws = _attn_ws(lib, d, 1, 1, q.device)
+    _lib.check(lib.uvtg_relpos_attention_bwd(d, _at(q), _at(k), _at(v), _at(table), _at(buckets), _at(kvalid), _at(o), _at(lse), _at(do), _at(dq), _at(dk),
+                                             _at(dv), _at(dtable), _at(ws), _stream()), "uvtg_relpos_attention_bwd")
     return dq, dk, dv, dtable
 
 
 def _lam_operand(d, q, lam):
-    if tuple(lam.shape) != (d.H,) or lam.device != q.device:
+    if lam.shape != (d.H,) or lam.device != q.device:
         raise ValueError(f"diff_attention: lam must be [H = {d.H}] on {q.device}, got {tuple(lam.shape)} on {lam.device}")
     return _f32c(lam)
 
@@ -345,31 +361,36 @@ def diff_attention_fwd(q, k, v, lam, kvalid=None, q_offset=0, causal=False, scal
     """Differential attention (softmax(scale q1 k1^T) - lam[h] softmax(scale q2 k2^T)) v: q [B, Sq, H, 2, D], k [B, Sk, Hkv, 2, D], v [B, Sk, Hkv, 2 D]
     (bf16 or fp16, D 32 / 64, any strides), lam [H] fp32; kvalid, q_offset, causal and scale as in relpos_attention_fwd.  Returns o [B, Sq, H, 2 D]
     and lse [B, H, 2, Sq] (fp32), and with need_o2 also o2, the second map's own output, which the backward pass reads."""
-    with torch.cuda.device_of(q):
-        d, q, k, v, kvalid = _attn_call("diff_attention", 2, q, k, v, kvalid, q_offset, causal, scale)
-        lam = _lam_operand(d, q, lam)
-        o = torch.empty(d.B, d.Sq, d.H, 2 * d.D, dtype=q.dtype, device=q.device)
-        o2 = torch.empty_like(o) if need_o2 else None
-        lse = torch.empty(d.B, d.H, 2, d.Sq, dtype=torch.float32, device=q.device)
-        ws = _attn_ws(d, 2, 0, q.device)
-        _lib.check(_lib.load().uvtg_diff_attention_fwd(C.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(lam), _ptr(kvalid), _ptr(o), _ptr(o2), _ptr(lse),
-                                                       _ptr(ws), _stream()), "uvtg_diff_attention_fwd")
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return diff_attention_fwd(q, k, v, lam, kvalid, q_offset, causal, scale, need_o2)
+    lib = _lib.load()
+    d, q, k, v, kvalid = _attn_call("diff_attention", 2, q, k, v, kvalid, q_offset, causal, scale)
+    lam = _lam_operand(d, q, lam)
+    o = torch.empty((d.B, d.Sq, d.H, 2 * d.D), dtype=q.dtype, device=q.device)
+    o2 = torch.empty_like(o) if need_o2 else None
+    lse = torch.empty((d.B, d.H, 2, d.Sq), dtype=torch.float32, device=q.device)
+    ws = _attn_ws(lib, d, 2, 0, q.device)
+    _lib.check(lib.uvtg_diff_attention_fwd(d, _at(q), _at(k), _at(v), _at(lam), _at(kvalid), _at(o), _at(o2), _at(lse), _at(ws), _stream()),
+               "uvtg_diff_attention_fwd")
     return (o, lse, o2) if need_o2 else (o, lse)
 
 
 def diff_attention_bwd(do, q, k, v, lam, o, o2, lse, kvalid=None, q_offset=0, causal=False, scale=None, need_dlam=True):
     """Gradients of diff_attention_fwd(need_o2=True) from its outputs and do: dq, dk, dv (the operands' type, contiguous) and dlam (fp32, or None)."""
-    with torch.cuda.device_of(q):
-        d, q, k, v, kvalid = _attn_call("diff_attention", 2, q, k, v, kvalid, q_offset, causal, scale)
-        lam = _lam_operand(d, q, lam)
-        if tuple(do.shape) != (d.B, d.Sq, d.H, 2 * d.D) or o.shape != do.shape or o2.shape != do.shape or tuple(lse.shape) != (d.B, d.H, 2, d.Sq):
-            raise ValueError("diff_attention_bwd: do, o and o2 must be [B, Sq, H, 2 D], lse [B, H, 2, Sq]")
-        do, o, o2 = (_attn_saved("diff_attention_bwd", t, q, w) for t, w in ((do, "do"), (o, "o"), (o2, "o2")))
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-        dv = torch.empty(v.shape, dtype=q.dtype, device=q.device)
-        dlam = torch.empty(d.H, dtype=torch.float32, device=q.device) if need_dlam else None
-        ws = _attn_ws(d, 2, 1, q.device)
-        _lib.check(_lib.load().uvtg_diff_attention_bwd(C.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(lam), _ptr(kvalid), _ptr(o), _ptr(o2), _ptr(_f32c(lse)),
-                                                       _ptr(do), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dlam), _ptr(ws), _stream()), "uvtg_diff_attention_bwd")
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return diff_attention_bwd(do, q, k, v, lam, o, o2, lse, kvalid, q_offset, causal, scale, need_dlam)
+    lib = _lib.load()
+    d, q, k, v, kvalid = _attn_call("diff_attention", 2, q, k, v, kvalid, q_offset, causal, scale)
+    lam = _lam_operand(d, q, lam)
+    if do.shape != (d.B, d.Sq, d.H, 2 * d.D) or o.shape != do.shape or o2.shape != do.shape or lse.shape != (d.B, d.H, 2, d.Sq):
+        raise ValueError("diff_attention_bwd: do, o and o2 must be [B, Sq, H, 2 D], lse [B, H, 2, Sq]")
+    do, o, o2 = (_attn_saved("diff_attention_bwd", t, q, w) for t, w in ((do, "do"), (o, "o"), (o2, "o2")))
+    lse = _f32c(lse)
+    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
+    dlam = torch.empty(d.H, dtype=torch.float32, device=q.device) if need_dlam else None
+    ws = _attn_ws(lib, d, 2, 1, q.device)
+    _lib.check(lib.uvtg_diff_attention_bwd(d, _at(q), _at(k), _at(v), _at(lam), _at(kvalid), _at(o), _at(o2), _at(lse), _at(do), _at(dq), _at(dk), _at(dv),
+                                           _at(dlam), _at(ws), _stream()), "uvtg_diff_attention_bwd")
     return dq, dk, dv, dlam
