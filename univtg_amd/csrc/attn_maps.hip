@@ -199,7 +199,7 @@ __device__ __forceinline__ void mask_scores(f32x16& s, unsigned mask32, int lim,
 // ------------------------------------------------------------------------------------------------
 template <bool HALF, int D, int MAPS>
 __global__ __launch_bounds__(256, 2) void maps_fwd_kernel(const MapArgs a) {
-  constexpr int DV = MAPS * D, KT = 64 * D, STAGE = MAPS * KT + 64 * DV, NK = D / 16, ND = DV / 32;
+  constexpr int DV = MAPS * D, KT = 64 * D, STAGE = MAPS * KT + 64 * DV, NK = D / 16, ND = DV / 32, NB = MAPS == 2 ? 1 : 2;
   constexpr bool BIAS = MAPS == 1;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   bf16_t* stage = (bf16_t*)smem;
@@ -269,79 +269,82 @@ __global__ __launch_bounds__(256, 2) void maps_fwd_kernel(const MapArgs a) {
       const int seen = a.causal ? q0 + min(31, a.Sq - 1 - q0) + a.off - key0 : 64;      // last key (relative) that any query of the wave sees
       if (live && seen >= 0) {
         const bool part = mask != ~0ull || (a.causal && q0 + a.off < key0 + 63);
-        unsigned pk[MAPS][2][8];
+        // NB blocks of 32 keys per softmax step: two for one map; one for two, whose accumulators leave no registers for more
+#pragma unroll 1
+        for (int kp = 0; kp < 2; kp += NB) {
+          unsigned pk[MAPS][NB][8];
 #pragma unroll
-        for (int m = 0; m < MAPS; m++) {
-          f32x16 s[2];
+          for (int m = 0; m < MAPS; m++) {
+            f32x16 s[NB];
 #pragma unroll
-          for (int kb = 0; kb < 2; kb++) {
-            zero(s[kb]);
+            for (int kb = 0; kb < NB; kb++) {
+              zero(s[kb]);
 #pragma unroll
-            for (int ks = 0; ks < NK; ks++)
-              s[kb] = mma<HALF>(*(const s16x8*)(sK + m * KT + Tile<D>::cols(koff, 16 * ks) + kb * 32 * D), qf[m][ks], s[kb]);
-          }
-          // log2-domain scores are cc s + cb: the scale and a bias that is the same over the tile cost nothing, they ride in the exponent's FMA
-          float cc = a.c, cb = 0.f;
-          if constexpr (BIAS) {
-            const int rmin = key0 - q0 - 31 - a.off, rmax = key0 + 63 - q0 - a.off;
-            if (rmin >= a.R) cb = br;
-            else if (rmax <= -a.R) cb = bl;
-            else {
-              const float* bp = sB + (key0 - min(q_raw, last_q) - a.off + 4 * g - rlo);
-#pragma unroll
-              for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[kb][r] = fmaf(s[kb][r], a.c, bp[kb * 32 + (r & 3) + 8 * (r >> 2)]);
-              cc = 1.f;
+              for (int ks = 0; ks < NK; ks++)
+                s[kb] = mma<HALF>(*(const s16x8*)(sK + m * KT + Tile<D>::cols(koff, 16 * ks) + (kp + kb) * 32 * D), qf[m][ks], s[kb]);
             }
-          }
-          if (part) {
-            const int lim = a.causal ? q_raw + a.off - key0 : 64;
-            mask_scores(s[0], (unsigned)mask, lim, g, -INFINITY);
-            mask_scores(s[1], (unsigned)(mask >> 32), lim - 32, g, -INFINITY);
-          }
-          float mx = s[0][0];
+            // log2-domain scores are cc s + cb: the scale and a bias that is the same over the tile cost nothing, they ride in the exponent's FMA
+            float cc = a.c, cb = 0.f;
+            if constexpr (BIAS) {
+              const int rmin = key0 - q0 - 31 - a.off, rmax = key0 + 63 - q0 - a.off;
+              if (rmin >= a.R) cb = br;
+              else if (rmax <= -a.R) cb = bl;
+              else {
+                const float* bp = sB + (key0 - min(q_raw, last_q) - a.off + 4 * g - rlo);
 #pragma unroll
-          for (int r = 1; r < 16; r++) mx = fmaxf(mx, s[0][r]);
+                for (int kb = 0; kb < NB; kb++)
 #pragma unroll
-          for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[1][r]);
-          mx = fmaf(half_max(mx), cc, cb);
-          // the reference point of the exponentials follows the running maximum only when it has fallen 8 (a factor of 256) behind: the sums are
-          // fp32 and the probabilities at most 2^8, and the accumulators are rescaled a few times per row instead of at every new maximum
-          if (__builtin_amdgcn_ballot_w64(mx > m_run[m] + 8.f)) {
-            const float mn = fmaxf(m_run[m], mx);
-            const float al = ex2(m_run[m] - (mn == -INFINITY ? 0.f : mn));
-            m_run[m] = mn; l_run[m] *= al;
-#pragma unroll
-            for (int i = 0; i < ND; i++)
-#pragma unroll
-              for (int r = 0; r < 16; r++) oacc[m][i][r] *= al;
-          }
-          const float e0 = cb - (m_run[m] == -INFINITY ? 0.f : m_run[m]);
-          float rs = 0.f;
-#pragma unroll
-          for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-              const float p0 = ex2(fmaf(s[kb][r], cc, e0)), p1 = ex2(fmaf(s[kb][r + 1], cc, e0));
-              rs += p0 + p1;
-              pk[m][kb][r / 2] = pack2<HALF>(p0, p1);
+                  for (int r = 0; r < 16; r++) s[kb][r] = fmaf(s[kb][r], a.c, bp[(kp + kb) * 32 + (r & 3) + 8 * (r >> 2)]);
+                cc = 1.f;
+              }
             }
-          l_run[m] += rs;                                  // (this half-wave's keys; the halves meet at the end)
+            if (part) {
+              const int lim = a.causal ? q_raw + a.off - key0 : 64;
+#pragma unroll
+              for (int kb = 0; kb < NB; kb++) mask_scores(s[kb], (unsigned)(mask >> (32 * (kp + kb))), lim - 32 * (kp + kb), g, -INFINITY);
+            }
+            float mx = s[0][0];
+#pragma unroll
+            for (int kb = 0; kb < NB; kb++)
+#pragma unroll
+              for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[kb][r]);
+            mx = fmaf(half_max(mx), cc, cb);
+            // the reference point of the exponentials follows the running maximum only when it has fallen 8 (a factor of 256) behind: the sums are
+            // fp32 and the probabilities at most 2^8, and the accumulators are rescaled a few times per row instead of at every new maximum
+            if (__builtin_amdgcn_ballot_w64(mx > m_run[m] + 8.f)) {
+              const float mn = fmaxf(m_run[m], mx);
+              const float al = ex2(m_run[m] - (mn == -INFINITY ? 0.f : mn));
+              m_run[m] = mn; l_run[m] *= al;
+#pragma unroll
+              for (int i = 0; i < ND; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) oacc[m][i][r] *= al;
+            }
+            const float e0 = cb - (m_run[m] == -INFINITY ? 0.f : m_run[m]);
+            float rs = 0.f;
+#pragma unroll
+            for (int kb = 0; kb < NB; kb++)
+#pragma unroll
+              for (int r = 0; r < 16; r += 2) {
+                const float p0 = ex2(fmaf(s[kb][r], cc, e0)), p1 = ex2(fmaf(s[kb][r + 1], cc, e0));
+                rs += p0 + p1;
+                pk[m][kb][r / 2] = pack2<HALF>(p0, p1);
+              }
+            l_run[m] += rs;                                  // (this half-wave's keys; the halves meet at the end)
+          }
+#pragma unroll
+          for (int kb = 0; kb < NB; kb++)
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+              const int ro = ((kp + kb) * 32 + 16 * hf) * DV;
+#pragma unroll
+              for (int i = 0; i < ND; i++) {
+                const s16x8 vt = cat4(lds_tr16(sV + Tile<DV>::cols(toff0, 32 * i) + ro), lds_tr16(sV + Tile<DV>::cols(toff1, 32 * i) + ro));
+#pragma unroll
+                for (int m = 0; m < MAPS; m++) oacc[m][i] = mma<HALF>(vt, frag(pk[m][kb] + 4 * hf), oacc[m][i]);
+              }
+            }
         }
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-          for (int hf = 0; hf < 2; hf++) {
-            const int ro = (kb * 32 + 16 * hf) * DV;
-#pragma unroll
-            for (int i = 0; i < ND; i++) {
-              const s16x8 vt = cat4(lds_tr16(sV + Tile<DV>::cols(toff0, 32 * i) + ro), lds_tr16(sV + Tile<DV>::cols(toff1, 32 * i) + ro));
-#pragma unroll
-              for (int m = 0; m < MAPS; m++)
-                oacc[m][i] = mma<HALF>(vt, frag(pk[m][kb] + 4 * hf), oacc[m][i]);
-            }
-          }
       }
       t = tn; buf ^= 1;
     }
@@ -726,7 +729,7 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
       const int seen = a.causal ? q0 + min(31, a.Sq - 1 - q0) + a.off - key0 : 64;
       if (live && seen >= 0) {
         const bool part = mask != ~0ull || (a.causal && q0 + a.off < key0 + 63);
-#pragma unroll
+#pragma unroll 1
         for (int kb = 0; kb < 2; kb++) {
           f32x16 dp, s[MAPS];
           zero(dp);
@@ -806,8 +809,8 @@ __global__ __launch_bounds__(256, 1) void maps_bwd_k_kernel(const MapArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   bf16_t* stage = (bf16_t*)smem;
   float* sStat = (float*)(smem + 2 * STAGE * 2);           // [2][MAPS][2][64]: log2 of the row sums, r
-  float* sDiag = sStat + 2 * MAPS * 2 * 64;                // [4 waves][2 halves][64] sums along diagonals
-  float* sB = sDiag + 4 * 2 * 64;
+  float* sDiag = sStat + 2 * MAPS * 2 * 64;                // [4 waves][32 queries][64]: score gradients, row q shifted by q
+  float* sB = sDiag + (BIAS ? 4 * 32 * 64 : 0);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;
   const int nkb = (a.Sk + 127) / 128;
   int blk, b, kh;
@@ -848,7 +851,11 @@ __global__ __launch_bounds__(256, 1) void maps_bwd_k_kernel(const MapArgs a) {
   int rlo, rhi;
   bias_window(a, blk * 128 - (a.Sq + 63) - a.off, blk * 128 + 127 - first * 64 - a.off, rlo, rhi);
   const int nk32 = (a.Sk + 31) / 32;
-  float* diag = sDiag + wave * 128;
+  float* diag = sDiag + wave * 2048;
+  if constexpr (BIAS) {                                    // entries no (query, key) of a 32 x 32 block falls on stay zero for good
+#pragma unroll
+    for (int i = 0; i < 32; i++) diag[i * 64 + lane] = 0.f;
+  }
   for (int hg = 0; hg < a.G; hg++) {
     const int h = kh * a.G + hg;
     const bf16_t* qb_ = a.q + (long long)b * a.q_sb + (long long)h * a.q_sh;
@@ -857,8 +864,9 @@ __global__ __launch_bounds__(256, 1) void maps_bwd_k_kernel(const MapArgs a) {
     const float* rv = a.rvec + ((size_t)b * a.H + h) * MAPS * a.Sq;
     const float lam = MAPS == 2 ? a.lam[h] : 0.f;
     float fl = 0.f, fr = 0.f, bl = 0.f, br = 0.f;          // sums and bias of the positions at and behind -R / +R
-    bool open = false;                                     // diagonals of the last block are still being summed
+    float carry = 0.f;                                     // sums of the last block's lower diagonals, at the lanes they have in the next block
     int base = 0;
+    bool open = false;
     float* part = nullptr;
     __syncthreads();                                       // the previous head's tiles, bias and statistics are read
     if constexpr (BIAS) {
@@ -866,7 +874,6 @@ __global__ __launch_bounds__(256, 1) void maps_bwd_k_kernel(const MapArgs a) {
       if (a.part) {
         part = a.part + (((size_t)h * a.B + b) * nk32 + k0 / 32) * a.gw;
         if (k0 < a.Sk) for (int i = lane; i < a.gw; i += 64) part[i] = 0.f;     // (done before the first tile's wait)
-        diag[lane] = 0.f; diag[64 + lane] = 0.f;
       }
     }
     float pl = 0.f;
@@ -883,23 +890,17 @@ __global__ __launch_bounds__(256, 1) void maps_bwd_k_kernel(const MapArgs a) {
     auto stats = [&](int qt, int buf) {
       if (tid < MAPS * 128) sStat[buf * MAPS * 128 + tid] = tid & 64 ? pl : (qt * 64 + (tid & 63) >= a.Sq || pl == -INFINITY) ? ROW_OFF : pl * LOG2E;
     };
-    // a finished 64-entry window of diagonal sums: relative positions base - 31 .. base + 31 at entries 0 .. 62; the upper 32 are complete and
-    // leave, the lower 31 move up for the next query block
-    auto flush = [&](int base_) {
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      const float v = diag[lane] + diag[64 + lane];
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      if (lane < 63) diag[lane < 31 ? lane + 32 : lane - 31] = lane < 31 ? v : 0.f;
-      diag[64 + lane] = 0.f;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
+    // lane l <-> relative position base + l - 31 (l < 63) of a block whose first key is `base` ahead of its first query.  The next block starts 32
+    // queries later: the upper 32 positions are complete and leave, the lower 31 move up 32 lanes and wait for it.
+    auto leave = [&](float v, int base_) {
       const int rel = base_ + lane - 31;
       if (lane >= 31 && lane < 63) {
         if (rel >= a.R) fr += v;
         else if (rel <= -a.R) fl += v;
         else if (rel >= a.glo && rel < a.glo + a.gw) part[rel - a.glo] = v;
       }
+      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+      carry = lane >= 32 && lane < 63 ? __int_as_float(sw[0]) : 0.f;
     };
     if (nqt > 0) { request(first, 0); stats(first, 0); }
     for (int n = 0; n < nqt; n++) {
@@ -979,14 +980,20 @@ __global__ __launch_bounds__(256, 1) void maps_bwd_k_kernel(const MapArgs a) {
         if constexpr (BIAS) {
           if (part) {
             if (near) {
-              if (kok) {                                   // one address per lane and instruction: the order of a wave's LDS additions is its program's
+              // sums along the block's 63 diagonals: row q of the block is written q entries to the left, lane l adds up column l
 #pragma unroll
-                for (int r = 0; r < 16; r++) {
-                  const int at = g * 64 + l31 - 4 * g + 31 - (r & 3) - 8 * (r >> 2);
-                  __hip_atomic_fetch_add(diag + at, ds0[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                }
+              for (int r = 0; r < 16; r++) {
+                const int q = (r & 3) + 8 * (r >> 2);
+                diag[(q + 4 * g) * 64 + 31 - q - 4 * g + l31] = kok ? ds0[r] : 0.f;
               }
-              flush(rb);
+              __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+              __builtin_amdgcn_wave_barrier();
+              float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int i = 0; i < 32; i++) t[i & 3] += diag[i * 64 + lane];
+              __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+              __builtin_amdgcn_wave_barrier();
+              leave(((t[0] + t[1]) + (t[2] + t[3])) + carry, rb);
               open = true; base = rb - 32;
             } else {
               float t = 0.f;
@@ -994,7 +1001,7 @@ __global__ __launch_bounds__(256, 1) void maps_bwd_k_kernel(const MapArgs a) {
               for (int r = 0; r < 16; r++) t += ds0[r];
               t = kok ? t : 0.f;
               if (right) fr += t; else fl += t;
-              if (left && open) { flush(rb); open = false; }
+              if (left && open) { leave(carry, rb); open = false; }
             }
           }
         }
@@ -1023,7 +1030,7 @@ __global__ __launch_bounds__(256, 1) void maps_bwd_k_kernel(const MapArgs a) {
     }
     if constexpr (BIAS) {
       if (part && k0 < a.Sk) {
-        if (open) flush(base);
+        if (open) leave(carry, base);
         fl = wave_sum_dpp(fl); fr = wave_sum_dpp(fr);
         if (lane == 0) {                                   // (position -R / +R outside the reachable window: its sum is 0)
           if (-a.R >= a.glo && -a.R < a.glo + a.gw) part[-a.R - a.glo] = fl;
@@ -1098,7 +1105,7 @@ __global__ __launch_bounds__(256) void lam_sum_kernel(const float* part, long lo
 // host side
 // ------------------------------------------------------------------------------------------------
 constexpr int MAX_REACH = 8191, MAX_BUCKETS = 1 << 16;
-constexpr int DIAG_BYTES = 4 * 2 * 64 * 4;
+constexpr int DIAG_BYTES = 4 * 32 * 64 * 4;                // skewed score gradients of the key kernel's waves
 
 int check_attn(const uvtg_attn_dims* d, int maps) {
   if (!d) return -10;
@@ -1224,7 +1231,7 @@ template <bool HALF, int D, int MAPS> int run_bwd(const uvtg_attn_dims* d, MapAr
   const size_t lds_q = 2 * 64 * (MAPS * D + DV) * 2 + WIN * 8 + window_bytes(d, MAPS, 128, d->Sk);
   hipLaunchKernelGGL((maps_bwd_q_kernel<HALF, D, MAPS>), dim3((unsigned)((d->Sq + 127) / 128) * d->H * d->B), dim3(256), lds_q, s, a);
   UVTG_CHECK_LAUNCH();
-  const size_t lds_k = 2 * 64 * (MAPS * D + DV) * 2 + 2 * MAPS * 2 * 64 * 4 + DIAG_BYTES + window_bytes(d, MAPS, 128, d->Sq);
+  const size_t lds_k = 2 * 64 * (MAPS * D + DV) * 2 + 2 * MAPS * 2 * 64 * 4 + (MAPS == 1 ? DIAG_BYTES : 0) + window_bytes(d, MAPS, 128, d->Sq);
   hipLaunchKernelGGL((maps_bwd_k_kernel<HALF, D, MAPS>), dim3((unsigned)((d->Sk + 127) / 128) * d->Hkv * d->B), dim3(256), lds_k, s, a);
   UVTG_CHECK_LAUNCH();
   if (!dsum) return 0;
