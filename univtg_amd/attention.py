@@ -21,33 +21,27 @@ from . import ops
 class _RelposAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, buckets, kvalid, opts):
-        o, lse = ops.relpos_attention_fwd(q, k, v, table, buckets, kvalid, *opts)
-        ctx.save_for_backward(q, k, v, table, buckets, kvalid, o, lse)
-        ctx.opts = opts
+        o, lse, (ctx.dims, *operands) = ops._relpos_fwd(q, k, v, table, buckets, kvalid, *opts)
+        ctx.save_for_backward(*operands, o, lse)
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, table, buckets, kvalid, o, lse = ctx.saved_tensors
-        dq, dk, dv, dtable = ops.relpos_attention_bwd(do, q, k, v, table, buckets, o, lse, kvalid, *ctx.opts, need_dtable=ctx.needs_input_grad[3])
-        return dq, dk, dv, dtable, None, None, None
+        return *ops._relpos_bwd(do, ctx.dims, *ctx.saved_tensors, ctx.needs_input_grad[3]), None, None, None
 
 
 class _DiffAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lam, kvalid, opts):
-        o, lse, o2 = ops.diff_attention_fwd(q, k, v, lam, kvalid, *opts, need_o2=True)
-        ctx.save_for_backward(q, k, v, lam, kvalid, o, o2, lse)
-        ctx.opts = opts
+        o, lse, o2, (ctx.dims, *operands) = ops._diff_fwd(q, k, v, lam, kvalid, *opts, True)
+        ctx.save_for_backward(*operands, o, o2, lse)
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, lam, kvalid, o, o2, lse = ctx.saved_tensors
-        dq, dk, dv, dlam = ops.diff_attention_bwd(do, q, k, v, lam, o, o2, lse, kvalid, *ctx.opts, need_dlam=ctx.needs_input_grad[3])
-        return dq, dk, dv, dlam, None, None
+        return *ops._diff_bwd(do, ctx.dims, *ctx.saved_tensors, ctx.needs_input_grad[3]), None, None
 
 
 def _apply(function, leaves, *args):
@@ -55,7 +49,7 @@ def _apply(function, leaves, *args):
     engine makes the stream it was made on wait for a backward pass: during a capture that joins a stream outside it, which ends the process in
     capture_end, not in an error.  So every graph made here is noted on its leaves, and a capture is refused while one of another stream is alive."""
     on_gpu = leaves[0].is_cuda
-    stream = torch.cuda.current_stream(leaves[0].device).cuda_stream if on_gpu else 0
+    stream = ops._stream_of(leaves[0]) if on_gpu else 0
     leaves = [t for t in leaves if t.requires_grad and t.is_leaf]
     if on_gpu and leaves and torch.cuda.is_current_stream_capturing():
         _refuse_foreign(leaves, stream)
@@ -83,6 +77,9 @@ def relpos_attention(q, k, v, table, buckets, kvalid=None, q_offset=0, causal=Fa
     opts = (q_offset, causal, scale)
     if not _needs_grad(q, k, v, table):
         return ops.relpos_attention_fwd(q, k, v, table, buckets, kvalid, *opts)[0]
+    if ops._elsewhere(q):
+        with torch.cuda.device(q.device):
+            return relpos_attention(q, k, v, table, buckets, kvalid, *opts)
     table = table.float()
     return _apply(_RelposAttention, (q, k, v, table), q, k, v, table, buckets, kvalid, opts)
 
@@ -92,5 +89,8 @@ def diff_attention(q, k, v, lam, kvalid=None, q_offset=0, causal=False, scale=No
     opts = (q_offset, causal, scale)
     if not _needs_grad(q, k, v, lam):
         return ops.diff_attention_fwd(q, k, v, lam, kvalid, *opts)[0]
+    if ops._elsewhere(q):
+        with torch.cuda.device(q.device):
+            return diff_attention(q, k, v, lam, kvalid, *opts)
     lam = lam.float()
     return _apply(_DiffAttention, (q, k, v, lam), q, k, v, lam, kvalid, opts)

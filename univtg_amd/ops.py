@@ -292,6 +292,10 @@ def _elsewhere(t):
     return t.device.index != torch.cuda.current_device()
 
 
+def _stream_of(t):
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
 def _relpos_operands(d, q, table, buckets):
     if table.dim() != 2 or table.shape[1] != d.H or table.device != q.device:
         raise ValueError(f"relpos_attention: table must be [n_buckets, H = {d.H}] on {q.device}, got {tuple(table.shape)} on {table.device}")
@@ -312,6 +316,32 @@ def _at(t):
     return None if t is None else t.data_ptr()
 
 
+def _relpos_fwd(q, k, v, table, buckets, kvalid, q_offset, causal, scale):
+    """(o, lse) and what the backward call reads again: the descriptor and the operands as laid out."""
+    lib = _lib.load()
+    d, q, k, v, kvalid = _attn_call("relpos_attention", 1, q, k, v, kvalid, q_offset, causal, scale)
+    table, buckets = _relpos_operands(d, q, table, buckets)
+    dev = q.device
+    o = torch.empty((d.B, d.Sq, d.H, d.D), dtype=q.dtype, device=dev)
+    lse = torch.empty((d.B, d.H, d.Sq), dtype=torch.float32, device=dev)
+    ws = _attn_ws(lib, d, 1, 0, dev)
+    _lib.check(lib.uvtg_relpos_attention_fwd(d, _at(q), _at(k), _at(v), _at(table), _at(buckets), _at(kvalid), _at(o), _at(lse), _at(ws), _stream_of(q)),
+               "uvtg_relpos_attention_fwd")
+    return o, lse, (d, q, k, v, table, buckets, kvalid)
+
+
+def _relpos_bwd(do, d, q, k, v, table, buckets, kvalid, o, lse, need_dtable):
+    lib = _lib.load()
+    do = _attn_saved("relpos_attention_bwd", do, q, "do")
+    dev, t = q.device, q.dtype
+    dq, dk, dv = torch.empty(q.shape, dtype=t, device=dev), torch.empty(k.shape, dtype=t, device=dev), torch.empty(v.shape, dtype=t, device=dev)
+    dtable = torch.empty(table.shape, dtype=torch.float32, device=dev) if need_dtable else None
+    ws = _attn_ws(lib, d, 1, 1, dev)
+    _lib.check(lib.uvtg_relpos_attention_bwd(d, _at(q), _at(k), _at(v), _at(table), _at(buckets), _at(kvalid), _at(o), _at(lse), _at(do), _at(dq), _at(dk),
+                                             _at(dv), _at(dtable), _at(ws), _stream_of(q)), "uvtg_relpos_attention_bwd")
+    return dq, dk, dv, dtable
+
+
 def relpos_attention_fwd(q, k, v, table, buckets, kvalid=None, q_offset=0, causal=False, scale=None):
     """softmax(scale q k^T + table[buckets[clamp(j - i - q_offset)], h]) v: q [B, Sq, H, D], k and v [B, Sk, Hkv, D] (bf16 or fp16, D 32 / 64 / 128,
     any strides), table [n_buckets, H] fp32, buckets int32 [2 reach + 1] (relpos_buckets), kvalid [B, Sk] uint8 / bool (0 = masked key).  causal:
@@ -320,15 +350,7 @@ def relpos_attention_fwd(q, k, v, table, buckets, kvalid=None, q_offset=0, causa
     if _elsewhere(q):
         with torch.cuda.device(q.device):
             return relpos_attention_fwd(q, k, v, table, buckets, kvalid, q_offset, causal, scale)
-    lib = _lib.load()
-    d, q, k, v, kvalid = _attn_call("relpos_attention", 1, q, k, v, kvalid, q_offset, causal, scale)
-    table, buckets = _relpos_operands(d, q, table, buckets)
-    o = torch.empty((d.B, d.Sq, d.H, d.D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((d.B, d.H, d.Sq), dtype=torch.float32, device=q.device)
-    ws = _attn_ws(lib, d, 1, 0, q.device)
-    _lib.check(lib.uvtg_relpos_attention_fwd(d, _at(q), _at(k), _at(v), _at(table), _at(buckets), _at(kvalid), _at(o), _at(lse), _at(ws), _stream()),
-               "uvtg_relpos_attention_fwd")
-    return o, lse
+    return _relpos_fwd(q, k, v, table, buckets, kvalid, q_offset, causal, scale)[:2]
 
 
 def relpos_attention_bwd(do, q, k, v, table, buckets, o, lse, kvalid=None, q_offset=0, causal=False, scale=None, need_dtable=True):
@@ -336,25 +358,43 @@ def relpos_attention_bwd(do, q, k, v, table, buckets, o, lse, kvalid=None, q_off
     if _elsewhere(q):
         with torch.cuda.device(q.device):
             return relpos_attention_bwd(do, q, k, v, table, buckets, o, lse, kvalid, q_offset, causal, scale, need_dtable)
-    lib = _lib.load()
     d, q, k, v, kvalid = _attn_call("relpos_attention", 1, q, k, v, kvalid, q_offset, causal, scale)
     table, buckets = _relpos_operands(d, q, table, buckets)
     if do.shape != (d.B, d.Sq, d.H, d.D) or o.shape != do.shape or lse.shape != (d.B, d.H, d.Sq):
         raise ValueError("relpos_attention_bwd: do and o must be [B, Sq, H, D], lse [B, H, Sq]")
-    do, o = _attn_saved("relpos_attention_bwd", do, q, "do"), _attn_saved("relpos_attention_bwd", o, q, "o")
-    lse = _f32c(lse)
-    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
-    dtable = torch.empty(table.shape, dtype=torch.float32, device=q.device) if need_dtable else None
-    ws = _attn_ws(lib, d, 1, 1, q.device)
-    _lib.check(lib.uvtg_relpos_attention_bwd(d, _at(q), _at(k), _at(v), _at(table), _at(buckets), _at(kvalid), _at(o), _at(lse), _at(do), _at(dq), _at(dk),
-                                             _at(dv), _at(dtable), _at(ws), _stream()), "uvtg_relpos_attention_bwd")
-    return dq, dk, dv, dtable
+    return _relpos_bwd(do, d, q, k, v, table, buckets, kvalid, _attn_saved("relpos_attention_bwd", o, q, "o"), _f32c(lse), need_dtable)
 
 
 def _lam_operand(d, q, lam):
     if lam.shape != (d.H,) or lam.device != q.device:
         raise ValueError(f"diff_attention: lam must be [H = {d.H}] on {q.device}, got {tuple(lam.shape)} on {lam.device}")
     return _f32c(lam)
+
+
+def _diff_fwd(q, k, v, lam, kvalid, q_offset, causal, scale, need_o2):
+    lib = _lib.load()
+    d, q, k, v, kvalid = _attn_call("diff_attention", 2, q, k, v, kvalid, q_offset, causal, scale)
+    lam = _lam_operand(d, q, lam)
+    dev = q.device
+    o = torch.empty((d.B, d.Sq, d.H, 2 * d.D), dtype=q.dtype, device=dev)
+    o2 = torch.empty_like(o) if need_o2 else None
+    lse = torch.empty((d.B, d.H, 2, d.Sq), dtype=torch.float32, device=dev)
+    ws = _attn_ws(lib, d, 2, 0, dev)
+    _lib.check(lib.uvtg_diff_attention_fwd(d, _at(q), _at(k), _at(v), _at(lam), _at(kvalid), _at(o), _at(o2), _at(lse), _at(ws), _stream_of(q)),
+               "uvtg_diff_attention_fwd")
+    return o, lse, o2, (d, q, k, v, lam, kvalid)
+
+
+def _diff_bwd(do, d, q, k, v, lam, kvalid, o, o2, lse, need_dlam):
+    lib = _lib.load()
+    do = _attn_saved("diff_attention_bwd", do, q, "do")
+    dev, t = q.device, q.dtype
+    dq, dk, dv = torch.empty(q.shape, dtype=t, device=dev), torch.empty(k.shape, dtype=t, device=dev), torch.empty(v.shape, dtype=t, device=dev)
+    dlam = torch.empty(d.H, dtype=torch.float32, device=dev) if need_dlam else None
+    ws = _attn_ws(lib, d, 2, 1, dev)
+    _lib.check(lib.uvtg_diff_attention_bwd(d, _at(q), _at(k), _at(v), _at(lam), _at(kvalid), _at(o), _at(o2), _at(lse), _at(do), _at(dq), _at(dk), _at(dv),
+                                           _at(dlam), _at(ws), _stream_of(q)), "uvtg_diff_attention_bwd")
+    return dq, dk, dv, dlam
 
 
 def diff_attention_fwd(q, k, v, lam, kvalid=None, q_offset=0, causal=False, scale=None, need_o2=False):
@@ -364,15 +404,7 @@ def diff_attention_fwd(q, k, v, lam, kvalid=None, q_offset=0, causal=False, scal
     if _elsewhere(q):
         with torch.cuda.device(q.device):
             return diff_attention_fwd(q, k, v, lam, kvalid, q_offset, causal, scale, need_o2)
-    lib = _lib.load()
-    d, q, k, v, kvalid = _attn_call("diff_attention", 2, q, k, v, kvalid, q_offset, causal, scale)
-    lam = _lam_operand(d, q, lam)
-    o = torch.empty((d.B, d.Sq, d.H, 2 * d.D), dtype=q.dtype, device=q.device)
-    o2 = torch.empty_like(o) if need_o2 else None
-    lse = torch.empty((d.B, d.H, 2, d.Sq), dtype=torch.float32, device=q.device)
-    ws = _attn_ws(lib, d, 2, 0, q.device)
-    _lib.check(lib.uvtg_diff_attention_fwd(d, _at(q), _at(k), _at(v), _at(lam), _at(kvalid), _at(o), _at(o2), _at(lse), _at(ws), _stream()),
-               "uvtg_diff_attention_fwd")
+    o, lse, o2, _ = _diff_fwd(q, k, v, lam, kvalid, q_offset, causal, scale, need_o2)
     return (o, lse, o2) if need_o2 else (o, lse)
 
 
@@ -381,16 +413,9 @@ def diff_attention_bwd(do, q, k, v, lam, o, o2, lse, kvalid=None, q_offset=0, ca
     if _elsewhere(q):
         with torch.cuda.device(q.device):
             return diff_attention_bwd(do, q, k, v, lam, o, o2, lse, kvalid, q_offset, causal, scale, need_dlam)
-    lib = _lib.load()
     d, q, k, v, kvalid = _attn_call("diff_attention", 2, q, k, v, kvalid, q_offset, causal, scale)
     lam = _lam_operand(d, q, lam)
     if do.shape != (d.B, d.Sq, d.H, 2 * d.D) or o.shape != do.shape or o2.shape != do.shape or lse.shape != (d.B, d.H, 2, d.Sq):
         raise ValueError("diff_attention_bwd: do, o and o2 must be [B, Sq, H, 2 D], lse [B, H, 2, Sq]")
-    do, o, o2 = (_attn_saved("diff_attention_bwd", t, q, w) for t, w in ((do, "do"), (o, "o"), (o2, "o2")))
-    lse = _f32c(lse)
-    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
-    dlam = torch.empty(d.H, dtype=torch.float32, device=q.device) if need_dlam else None
-    ws = _attn_ws(lib, d, 2, 1, q.device)
-    _lib.check(lib.uvtg_diff_attention_bwd(d, _at(q), _at(k), _at(v), _at(lam), _at(kvalid), _at(o), _at(o2), _at(lse), _at(do), _at(dq), _at(dk), _at(dv),
-                                           _at(dlam), _at(ws), _stream()), "uvtg_diff_attention_bwd")
-    return dq, dk, dv, dlam
+    o, o2 = (_attn_saved("diff_attention_bwd", t, q, w) for t, w in ((o, "o"), (o2, "o2")))
+    return _diff_bwd(do, d, q, k, v, lam, kvalid, o, o2, _f32c(lse), need_dlam)
