@@ -268,7 +268,7 @@ typedef struct uvtg_attn_dims {
   int B, H, Hkv, D, Sq, Sk;    /* H a multiple of Hkv                                         */
   int causal, q_offset;        /* position of query 0 on the keys' axis                       */
   float scale;                 /* > 0                                                         */
-  int n_buckets, reach;        /* relpos: rows of table; 1 <= reach <= 8191                   */
+  int n_buckets, reach;        /* relpos: rows of table; 1 <= reach <= 4095                   */
   long long q_sb, q_ss, q_sh, q_sm, k_sb, k_ss, k_sh, k_sm, v_sb, v_ss, v_sh;   /* batch, position, head, map (diff) */
   long long kvalid_sb;
 } uvtg_attn_dims;

@@ -204,7 +204,7 @@ def _dims(**kw):
 @pytest.mark.parametrize("maps, bad, code", [
     (1, dict(B=0), -11), (1, dict(Sk=0), -11), (2, dict(Sq=-1), -11), (1, dict(dtype=2), -30), (2, dict(Hkv=3), -31), (1, dict(D=48), -5), (2, dict(D=128), -32),
     (1, dict(scale=0.0), -33), (2, dict(scale=float("inf")), -33), (1, dict(scale=float("nan")), -33), (1, dict(q_offset=1 << 30), -34), (1, dict(Sk=1 << 25), -34),
-    (1, dict(q_ss=257), -35), (2, dict(k_sm=4), -35), (1, dict(v_sh=-64), -35), (1, dict(reach=0), -36), (1, dict(reach=8192), -36), (1, dict(n_buckets=0), -37),
+    (1, dict(q_ss=257), -35), (2, dict(k_sm=4), -35), (1, dict(v_sh=-64), -35), (1, dict(reach=0), -36), (1, dict(reach=4096), -36), (1, dict(n_buckets=0), -37),
     (1, dict(B=1 << 16, H=1 << 10, Hkv=1 << 10), -34), (1, {}, -20), (2, {}, -20)])
 def test_c_abi_refuses(maps, bad, code):
     """Every refusal comes back before anything is enqueued (no GPU here, null pointers)."""

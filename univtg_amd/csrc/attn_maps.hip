@@ -19,6 +19,7 @@ typedef __attribute__((ext_vector_type(2))) _Float16 half2_t;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float ROW_OFF = 1e30f;       // "log2 of the sum" of a query row that has no probabilities: exp2(x - ROW_OFF) is an exact 0
 constexpr int PAD = 96;                // entries on either side of the bias window: the positions of a wave's 32 queries x 64 keys span 95
+constexpr int SLAB = 32 * 72;          // elements of a wave's store slab
 constexpr int WIN = 256;               // key tiles whose masks a workgroup holds in LDS at a time
 
 struct MapArgs {
@@ -86,19 +87,93 @@ template <int W> struct Tile {
   __device__ static __forceinline__ int rows8(int base) { return (base ^ 16) + 8 * W; }
 };
 
-// `rows` rows (a multiple of 64 / (W / 8)) of a strided matrix -> LDS tile; rows behind `last` repeat it.  `nw` waves share the work.
+// A chain of N fragment reads and the MFMAs that use them, R reads ahead of their use: left alone the scheduler sinks each read to its MFMA, and
+// every MFMA then waits out an LDS round trip.  fill() may run well before run(), under other arithmetic.
+__device__ __forceinline__ void fence();
+template <int N, int R, typename Load> __device__ __forceinline__ void fill(s16x8 (&f)[R], Load&& load) {
+#pragma unroll
+  for (int i = 0; i < (N < R ? N : R); i++) f[i] = load(i);
+}
+template <int N, int R, typename Load, typename Use> __device__ __forceinline__ void run(s16x8 (&f)[R], Load&& load, Use&& use) {
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    use(i, f[i % R]);
+    if (i + R < N) f[i % R] = load(i + R);
+    fence();
+  }
+}
+// Fragments by LDS byte address: `at` is the lane's place in a tile whose start is a multiple of its row size, so that a column step is an XOR of the
+// address (one VALU operation) and a step of 16 rows, another tile of the stage, an immediate.  opaque() keeps the compiler from hoisting the XORs
+// out of the loop: it would spend a register on each of them, and spill.
+__device__ __forceinline__ unsigned lds_at(const bf16_t* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const bf16_t*)p; }
+__device__ __forceinline__ unsigned opaque(unsigned x) { asm volatile("" : "+v"(x)); return x; }
+__device__ __forceinline__ s16x8 row_frag(unsigned at, int i, int bytes) {
+  return *(const __attribute__((address_space(3))) s16x8*)(uintptr_t)((at ^ (32 * i)) + bytes);
+}
+__device__ __forceinline__ s16x8 col_frag(unsigned at0, unsigned at1, int i, int bytes) {
+  typedef __attribute__((address_space(3))) s16x4* lptr;
+  return cat4(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(uintptr_t)((at0 ^ (64 * i)) + bytes)), __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(uintptr_t)((at1 ^ (64 * i)) + bytes)));
+}
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// ROWS rows of a strided matrix -> LDS tile, `nw` waves sharing the work; rows behind `last` repeat it.  A whole tile of ordinary rows is addressed by
+// a scalar base and a 32-bit lane offset that does not depend on the tile (an instruction covers 512 / W rows, and NW waves step by a multiple of the
+// permutation's period); the last tile, and rows more than 64 MB apart, by 64-bit lane addresses.
+// The request itself is inline assembly: behind the builtin the compiler makes every LDS read that might touch the destination wait for ALL requests
+// in flight, so that a tile requested ahead stalls the reads of the tile at hand (measured: two thirds of these kernels' time).  What orders requests
+// and reads here is dma_wait() and the barrier behind it.
+__device__ __forceinline__ void dma16(const void* base, unsigned offset, unsigned lds) {
+  unsigned m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0) : "v"(offset), "s"(base), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void dma16(const void* lane_ptr, unsigned lds) {
+  unsigned m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0) : "v"(lane_ptr), "s"(lds) : "memory");
+}
 template <int W, int ROWS, int NW> __device__ __forceinline__ void load_tile(const bf16_t* base, long long stride, int row0, int last, bf16_t* tile, int wave, int lane) {
-  constexpr int RPI = 512 / W, NI = ROWS / RPI;
+  constexpr int RPI = 512 / W, NI = ROWS / RPI, PERIOD = W == 128 ? 4 : W == 64 ? 2 : 1;
+  const int lr = lane / (W / 8), lc = lane % (W / 8);
+  const unsigned lds = lds_at(tile);
+  if (row0 + ROWS - 1 <= last && stride < (1 << 25)) {
+#pragma unroll
+    for (int i = 0; i < (NI + NW - 1) / NW; i++) {
+      const int n = i * NW + wave;
+      if (NI % NW == 0 || n < NI)
+        dma16(base + ((long long)row0 + n * RPI) * stride, 2u * (unsigned)(lr * (int)stride + ((lc ^ Tile<W>::f((NW % PERIOD ? n : wave) * RPI + lr)) * 8)), lds + n * 1024);
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < (NI + NW - 1) / NW; i++) {
     const int n = i * NW + wave;
     if (NI % NW == 0 || n < NI) {
-      const int r = n * RPI + lane / (W / 8), ch = (lane % (W / 8)) ^ Tile<W>::f(r);
-      const bf16_t* g = base + (long long)min(row0 + r, last) * stride + ch * 8;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)(tile + n * 512), 16, 0, 0);
+      const int r = n * RPI + lr;
+      dma16(base + (long long)min(row0 + r, last) * stride + (lc ^ Tile<W>::f(r)) * 8, lds + n * 1024);
     }
   }
 }
+// The same for the loops over tiles, which keep a lane's row and chunk of a request ready.  Rows behind the last are clamped to it.
+template <int W, int ROWS, int NW> struct Loader {
+  static constexpr int RPI = 512 / W, NI = ROWS / RPI, PIECES = (NI + NW - 1) / NW, PERIOD = W == 128 ? 4 : W == 64 ? 2 : 1;
+  static_assert(NW % PERIOD == 0, "a wave's requests of a tile share one lane offset");
+  const char* base;
+  unsigned stride;                              // bytes (the host refuses rows further than 128 MB apart)
+  int last, wave, row, chunk;
+  __device__ __forceinline__ Loader(const bf16_t* b, long long stride_, int last_, int wave_, int lane)
+      : base((const char*)b), stride(2u * (unsigned)stride_), last(last_), wave(wave_), row(lane / (W / 8)) {
+    chunk = ((lane % (W / 8)) ^ Tile<W>::f(wave * RPI + row)) * 16;
+  }
+  __device__ __forceinline__ void tile(int row0, unsigned lds, long long disp) const {
+#pragma unroll
+    for (int i = 0; i < PIECES; i++) {
+      const int n = i * NW + wave, r0 = min(row0 + n * RPI, last);
+      if (NI % NW == 0 || n < NI)
+        dma16(base + disp + (unsigned long long)(unsigned)r0 * stride, (unsigned)min((int)opaque(row), last - r0) * stride + chunk, lds + n * 1024);   // (opaque: not kept ready)
+    }
+  }
+};
 // zero the rows of a landed tile whose mask bit is clear: a masked key's k / v row may hold anything, infinities and NaN included
 template <int W> __device__ __forceinline__ void clear_rows(bf16_t* tile, unsigned long long mask, int rows, int tid, int nt) {
   for (int i = tid; i < rows * (W / 8); i += nt)
@@ -106,22 +181,42 @@ template <int W> __device__ __forceinline__ void clear_rows(bf16_t* tile, unsign
 }
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// Key masks of tiles w0 .. of 64 keys, one 64-bit word each (keys behind the last: 0)
-__device__ __forceinline__ void load_masks(const MapArgs& a, int b, int w0, int n, unsigned long long* sMask, int wave, int lane) {
-  const unsigned char* kv = a.kvalid ? a.kvalid + (size_t)b * a.mask_sb : nullptr;
+// Key masks of the tiles of 64 keys, one 64-bit word each: of up to WIN tiles from w0 on in LDS, or plain arithmetic where there is no mask
+template <int NW> struct Masks {
+  const unsigned char* kv;
+  unsigned long long* words;
+  int w0, Sk, ntiles, wave, lane;
+  __device__ __forceinline__ Masks(const MapArgs& a, int b, int ntiles_, unsigned long long* words_, int wave_, int lane_)
+      : kv(a.kvalid ? a.kvalid + (size_t)b * a.mask_sb : nullptr), words(words_), w0(0), Sk(a.Sk), ntiles(ntiles_), wave(wave_), lane(lane_) {}
+  __device__ __forceinline__ void load() {       // (a barrier before and behind)
+    if (!kv) return;
+    const int n = min(WIN, ntiles - w0);
 #pragma unroll 4
-  for (int t = wave; t < n; t += 4) {
-    const int key = (w0 + t) * 64 + lane;
-    const bool on = key < a.Sk && (!kv || kv[key] != 0);
-    const unsigned long long m = __builtin_amdgcn_ballot_w64(on);
-    if (lane == 0) sMask[t] = m;
+    for (int t = wave; t < n; t += NW) {
+      const int key = (w0 + t) * 64 + lane;
+      const unsigned long long m = __builtin_amdgcn_ballot_w64(key < Sk && kv[min(key, Sk - 1)] != 0);
+      if (lane == 0) words[t] = m;
+    }
   }
-}
-// next tile of the window with a key that is not masked
-__device__ __forceinline__ int next_tile(const unsigned long long* sMask, int t, int n) {
-  while (t < n && uniform64(sMask[t]) == 0) t++;
-  return t;
-}
+  __device__ __forceinline__ unsigned long long at(int t) const {
+    if (kv) return uniform64(words[t - w0]);
+    return t * 64 + 64 <= Sk ? ~0ull : (1ull << (Sk - t * 64)) - 1;
+  }
+  // first tile from t on with a key that is not masked (ntiles: none), and its mask; every wave of the workgroup calls it with the same t
+  __device__ __forceinline__ int find(int t, unsigned long long& m) {
+    for (; t < ntiles; t++) {
+      if (kv && t >= w0 + WIN) {
+        __syncthreads();
+        w0 += WIN;
+        load();
+        __syncthreads();
+      }
+      m = at(t);
+      if (m) return t;
+    }
+    return ntiles;
+  }
+};
 
 // Bias of relative positions rlo .. rhi for one head, times log2(e): entry (rel - rlo).  Positions behind +-R take the bias of +-R.
 __device__ __forceinline__ void load_bias(const MapArgs& a, int h, int rlo, int rhi, float* sB, int tid, int nt) {
@@ -195,25 +290,39 @@ __device__ __forceinline__ void mask_scores(f32x16& s, unsigned mask32, int lim,
 }
 
 // ------------------------------------------------------------------------------------------------
-// forward: one workgroup = 128 queries of one head, 4 waves of 32, 64-key tiles in two LDS stages
+// forward: one workgroup = 32 NW queries of one head, a wave of 32 each, 64-key tiles in two LDS stages.  The first two tiles are requested before
+// anything else is known; from then on the requests of the next tile go out between the MFMAs of the current one.
 // ------------------------------------------------------------------------------------------------
-template <bool HALF, int D, int MAPS>
-__global__ __launch_bounds__(256, 2) void maps_fwd_kernel(const MapArgs a) {
-  constexpr int DV = MAPS * D, KT = 64 * D, STAGE = MAPS * KT + 64 * DV, NK = D / 16, ND = DV / 32, NB = MAPS == 2 ? 1 : 2;
+template <bool HALF, int D, int MAPS, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void maps_fwd_kernel(const MapArgs a) {
+  constexpr int DV = MAPS * D, KT = 64 * D, STAGE = MAPS * KT + 64 * DV, NK = D / 16, ND = DV / 32, NB = MAPS == 2 ? 1 : 2, RA = 4;
   constexpr bool BIAS = MAPS == 1;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   bf16_t* stage = (bf16_t*)smem;
   unsigned long long* sMask = (unsigned long long*)(smem + 2 * STAGE * 2);
   float* sB = (float*)(sMask + WIN);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;
-  const int nqb = (a.Sq + 127) / 128;
+  const int nqb = (a.Sq + 32 * NW - 1) / (32 * NW);
   int blk, b, h;
   block_id(nqb, a, a.H, blk, b, h);
   if (a.causal) blk = nqb - 1 - blk;                     // the longest rows first
-  const int kh = h / a.G, q0 = blk * 128 + wave * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1);
+  const int kh = h / a.G, qb = blk * 32 * NW, q0 = qb + wave * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1);
   const bool live = q0 < a.Sq;
-  const bf16_t* kb_ = a.k + (long long)b * a.k_sb + (long long)kh * a.k_sh;
-  const bf16_t* vb_ = a.v + (long long)b * a.v_sb + (long long)kh * a.v_sh;
+  const int last_q = min(qb + 32 * NW - 1, a.Sq - 1);
+  int ntiles = (a.Sk + 63) / 64;
+  if (a.causal) ntiles = last_q + a.off < 0 ? 0 : min(ntiles, (last_q + a.off) / 64 + 1);
+  typedef Loader<D, 64, NW> KL;
+  typedef Loader<DV, 64, NW> VL;
+  const KL kl(a.k + (long long)b * a.k_sb + (long long)kh * a.k_sh, a.k_ss, a.Sk - 1, wave, lane);
+  const VL vl(a.v + (long long)b * a.v_sb + (long long)kh * a.v_sh, a.v_ss, a.Sk - 1, wave, lane);
+  auto request = [&](int kt, int buf) {
+    const unsigned s = lds_at(stage) + buf * STAGE * 2;
+#pragma unroll
+    for (int m = 0; m < MAPS; m++) kl.tile(kt * 64, s + m * KT * 2, 2 * m * a.k_sm);
+    vl.tile(kt * 64, s + MAPS * KT * 2, 0);
+  };
+  if (ntiles > 0) request(0, 0);
+  if (ntiles > 1) request(1, 1);
 
   s16x8 qf[MAPS][NK];
 #pragma unroll
@@ -221,6 +330,11 @@ __global__ __launch_bounds__(256, 2) void maps_fwd_kernel(const MapArgs a) {
 #pragma unroll
     for (int ks = 0; ks < NK; ks++)
       qf[m][ks] = *(const s16x8*)(a.q + (long long)b * a.q_sb + (long long)qrow * a.q_ss + (long long)h * a.q_sh + m * a.q_sm + 16 * ks + 8 * g);
+  Masks<NW> masks(a, b, ntiles, sMask, wave, lane);
+  masks.load();
+  int rlo, rhi;
+  bias_window(a, -(last_q + a.off), ntiles * 64 - 1 - qb - a.off, rlo, rhi);
+  if constexpr (BIAS) load_bias(a, h, rlo, rhi, sB, tid, 64 * NW);
   f32x16 oacc[MAPS][ND];
   float m_run[MAPS], l_run[MAPS];
 #pragma unroll
@@ -229,125 +343,113 @@ __global__ __launch_bounds__(256, 2) void maps_fwd_kernel(const MapArgs a) {
 #pragma unroll
     for (int i = 0; i < ND; i++) zero(oacc[m][i]);
   }
-  const int last_q = min(blk * 128 + 127, a.Sq - 1);
-  int ntiles = (a.Sk + 63) / 64;
-  if (a.causal) ntiles = last_q + a.off < 0 ? 0 : min(ntiles, (last_q + a.off) / 64 + 1);
-  int rlo, rhi;
-  bias_window(a, -(last_q + a.off), ntiles * 64 - 1 - blk * 128 - a.off, rlo, rhi);
+  const int koff = 2 * Tile<D>::off(l31, 8 * g);                                                      // bytes
+  const int toff0 = 2 * Tile<DV>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), toff1 = 2 * Tile<DV>::rows8(toff0 / 2);
+  __syncthreads();
   float bl = 0.f, br = 0.f;
-  if constexpr (BIAS) load_bias(a, h, rlo, rhi, sB, tid, 256);
-
-  const int koff = Tile<D>::off(l31, 8 * g);
-  const int toff0 = Tile<DV>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), toff1 = Tile<DV>::rows8(toff0);
-  auto request = [&](int kt, int buf) {
-    bf16_t* s = stage + buf * STAGE;
-#pragma unroll
-    for (int m = 0; m < MAPS; m++) load_tile<D, 64, 4>(kb_ + m * a.k_sm, a.k_ss, kt * 64, a.Sk - 1, s + m * KT, wave, lane);
-    load_tile<DV, 64, 4>(vb_, a.v_ss, kt * 64, a.Sk - 1, s + MAPS * KT, wave, lane);
-  };
-  for (int w0 = 0; w0 < ntiles; w0 += WIN) {
-    const int wn = min(WIN, ntiles - w0);
+  if constexpr (BIAS) { bl = rlo <= -a.R ? sB[0] : 0.f; br = rhi >= a.R ? sB[rhi - rlo] : 0.f; }
+  unsigned long long mask = ntiles > 0 ? masks.at(0) : 0, mask_n = ntiles > 1 ? masks.at(1) : 0;
+#pragma nounroll
+  for (int t = 0, tn = min(1, ntiles), buf = 0; t < ntiles;) {
+    dma_wait();
     __syncthreads();
-    load_masks(a, b, w0, wn, sMask, wave, lane);
-    __syncthreads();
-    if constexpr (BIAS) if (w0 == 0) { bl = rlo <= -a.R ? sB[0] : 0.f; br = rhi >= a.R ? sB[rhi - rlo] : 0.f; }
-    int t = next_tile(sMask, 0, wn), buf = 0;
-    if (t < wn) request(w0 + t, 0);
-    while (t < wn) {
-      dma_wait();
+    const bool req = tn > 1 && tn < ntiles;                // (the second tile has been requested before the loop)
+    bf16_t* sK = stage + buf * STAGE;
+    bf16_t* sV = sK + MAPS * KT;
+    if (mask != ~0ull) {
+      clear_rows<DV>(sV, mask, 64, tid, 64 * NW);
       __syncthreads();
-      const int tn = next_tile(sMask, t + 1, wn);
-      const unsigned long long mask = uniform64(sMask[t]);
-      bf16_t* sK = stage + buf * STAGE;
-      bf16_t* sV = sK + MAPS * KT;
-      if (mask != ~0ull) {
-        clear_rows<DV>(sV, mask, 64, tid, 256);
-        __syncthreads();
-      }
-      if (tn < wn) request(w0 + tn, buf ^ 1);
-      const int key0 = (w0 + t) * 64;
-      const int seen = a.causal ? q0 + min(31, a.Sq - 1 - q0) + a.off - key0 : 64;      // last key (relative) that any query of the wave sees
-      if (live && seen >= 0) {
-        const bool part = mask != ~0ull || (a.causal && q0 + a.off < key0 + 63);
-        // NB blocks of 32 keys per softmax step: two for one map; one for two, whose accumulators leave no registers for more
+    }
+    const int key0 = t * 64;
+    const int seen = a.causal ? q0 + min(31, a.Sq - 1 - q0) + a.off - key0 : 64;      // last key (relative) that any query of the wave sees
+    const bool work = live && seen >= 0;
+    if (req && !work) request(tn, buf ^ 1);
+    if (work) {
+      const bool part = mask != ~0ull || (a.causal && q0 + a.off < key0 + 63);
+      // NB blocks of 32 keys per softmax step: two for one map; one for two, whose accumulators leave no registers for more
+      constexpr int NS = MAPS * NK * NB, NP = 2 * NB * ND;
 #pragma unroll 1
-        for (int kp = 0; kp < 2; kp += NB) {
-          unsigned pk[MAPS][NB][8];
+      for (int kp = 0; kp < 2; kp += NB) {
+        unsigned pk[MAPS][NB][8];
+        f32x16 sc[MAPS][NB];
+        s16x8 fa[RA];
+        const unsigned ka = opaque(lds_at(sK) + koff + kp * 64 * D), va0 = opaque(lds_at(sV) + toff0 + kp * 64 * DV), va1 = opaque(lds_at(sV) + toff1 + kp * 64 * DV);
+        auto krow = [&](int i) { return row_frag(ka, i / NB % NK, (i / NB / NK * KT + i % NB * 32 * D) * 2); };
+        auto vcol = [&](int i) { return col_frag(va0, va1, i % ND, (i / ND) * 16 * DV * 2); };
 #pragma unroll
-          for (int m = 0; m < MAPS; m++) {
-            f32x16 s[NB];
+        for (int m = 0; m < MAPS; m++)
 #pragma unroll
-            for (int kb = 0; kb < NB; kb++) {
-              zero(s[kb]);
+          for (int kb = 0; kb < NB; kb++) zero(sc[m][kb]);
+        fill<NS>(fa, krow);
+        fence();
+        run<NS>(fa, krow, [&](int i, s16x8 x) {
+          sc[i / NB / NK][i % NB] = mma<HALF>(x, qf[i / NB / NK][i / NB % NK], sc[i / NB / NK][i % NB]);
+        });
+        if (req && kp == 0) request(tn, buf ^ 1);          // (while the score MFMAs run)
+        fill<NP>(fa, vcol);                                // (arrive under the softmax arithmetic)
+        fence();
 #pragma unroll
-              for (int ks = 0; ks < NK; ks++)
-                s[kb] = mma<HALF>(*(const s16x8*)(sK + m * KT + Tile<D>::cols(koff, 16 * ks) + (kp + kb) * 32 * D), qf[m][ks], s[kb]);
+        for (int m = 0; m < MAPS; m++) {
+          f32x16 (&s)[NB] = sc[m];
+          // log2-domain scores are cc s + cb: the scale and a bias that is the same over the tile cost nothing, they ride in the exponent's FMA
+          float cc = a.c, cb = 0.f;
+          if constexpr (BIAS) {
+            const int rmin = key0 - q0 - 31 - a.off, rmax = key0 + 63 - q0 - a.off;
+            if (rmin >= a.R) cb = br;
+            else if (rmax <= -a.R) cb = bl;
+            else {
+              const float* bp = sB + (key0 - min(q_raw, last_q) - a.off + 4 * g - rlo);
+#pragma unroll
+              for (int kb = 0; kb < NB; kb++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[kb][r] = fmaf(s[kb][r], a.c, bp[(kp + kb) * 32 + (r & 3) + 8 * (r >> 2)]);
+              cc = 1.f;
             }
-            // log2-domain scores are cc s + cb: the scale and a bias that is the same over the tile cost nothing, they ride in the exponent's FMA
-            float cc = a.c, cb = 0.f;
-            if constexpr (BIAS) {
-              const int rmin = key0 - q0 - 31 - a.off, rmax = key0 + 63 - q0 - a.off;
-              if (rmin >= a.R) cb = br;
-              else if (rmax <= -a.R) cb = bl;
-              else {
-                const float* bp = sB + (key0 - min(q_raw, last_q) - a.off + 4 * g - rlo);
-#pragma unroll
-                for (int kb = 0; kb < NB; kb++)
-#pragma unroll
-                  for (int r = 0; r < 16; r++) s[kb][r] = fmaf(s[kb][r], a.c, bp[(kp + kb) * 32 + (r & 3) + 8 * (r >> 2)]);
-                cc = 1.f;
-              }
-            }
-            if (part) {
-              const int lim = a.causal ? q_raw + a.off - key0 : 64;
-#pragma unroll
-              for (int kb = 0; kb < NB; kb++) mask_scores(s[kb], (unsigned)(mask >> (32 * (kp + kb))), lim - 32 * (kp + kb), g, -INFINITY);
-            }
-            float mx = s[0][0];
-#pragma unroll
-            for (int kb = 0; kb < NB; kb++)
-#pragma unroll
-              for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[kb][r]);
-            mx = fmaf(half_max(mx), cc, cb);
-            // the reference point of the exponentials follows the running maximum only when it has fallen 8 (a factor of 256) behind: the sums are
-            // fp32 and the probabilities at most 2^8, and the accumulators are rescaled a few times per row instead of at every new maximum
-            if (__builtin_amdgcn_ballot_w64(mx > m_run[m] + 8.f)) {
-              const float mn = fmaxf(m_run[m], mx);
-              const float al = ex2(m_run[m] - (mn == -INFINITY ? 0.f : mn));
-              m_run[m] = mn; l_run[m] *= al;
-#pragma unroll
-              for (int i = 0; i < ND; i++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) oacc[m][i][r] *= al;
-            }
-            const float e0 = cb - (m_run[m] == -INFINITY ? 0.f : m_run[m]);
-            float rs = 0.f;
-#pragma unroll
-            for (int kb = 0; kb < NB; kb++)
-#pragma unroll
-              for (int r = 0; r < 16; r += 2) {
-                const float p0 = ex2(fmaf(s[kb][r], cc, e0)), p1 = ex2(fmaf(s[kb][r + 1], cc, e0));
-                rs += p0 + p1;
-                pk[m][kb][r / 2] = pack2<HALF>(p0, p1);
-              }
-            l_run[m] += rs;                                  // (this half-wave's keys; the halves meet at the end)
           }
+          if (part) {
+            const int lim = a.causal ? q_raw + a.off - key0 : 64;
+#pragma unroll
+            for (int kb = 0; kb < NB; kb++) mask_scores(s[kb], (unsigned)(mask >> (32 * (kp + kb))), lim - 32 * (kp + kb), g, -INFINITY);
+          }
+          float mx = s[0][0];
 #pragma unroll
           for (int kb = 0; kb < NB; kb++)
 #pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-              const int ro = ((kp + kb) * 32 + 16 * hf) * DV;
+            for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[kb][r]);
+          mx = fmaf(half_max(mx), cc, cb);
+          // the reference point of the exponentials follows the running maximum only when it has fallen 8 (a factor of 256) behind: the sums are
+          // fp32 and the probabilities at most 2^8, and the accumulators are rescaled a few times per row instead of at every new maximum
+          if (__builtin_amdgcn_ballot_w64(mx > m_run[m] + 8.f)) {
+            const float mn = fmaxf(m_run[m], mx);
+            const float al = ex2(m_run[m] - (mn == -INFINITY ? 0.f : mn));
+            m_run[m] = mn; l_run[m] *= al;
 #pragma unroll
-              for (int i = 0; i < ND; i++) {
-                const s16x8 vt = cat4(lds_tr16(sV + Tile<DV>::cols(toff0, 32 * i) + ro), lds_tr16(sV + Tile<DV>::cols(toff1, 32 * i) + ro));
+            for (int i = 0; i < ND; i++)
 #pragma unroll
-                for (int m = 0; m < MAPS; m++) oacc[m][i] = mma<HALF>(vt, frag(pk[m][kb] + 4 * hf), oacc[m][i]);
-              }
+              for (int r = 0; r < 16; r++) oacc[m][i][r] *= al;
+          }
+          const float e0 = cb - (m_run[m] == -INFINITY ? 0.f : m_run[m]);
+          float rs = 0.f;
+#pragma unroll
+          for (int kb = 0; kb < NB; kb++)
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+              const float p0 = ex2(fmaf(s[kb][r], cc, e0)), p1 = ex2(fmaf(s[kb][r + 1], cc, e0));
+              rs += p0 + p1;
+              pk[m][kb][r / 2] = pack2<HALF>(p0, p1);
             }
+          l_run[m] += rs;                                  // (this half-wave's keys; the halves meet at the end)
         }
+        fence();
+        run<NP>(fa, vcol, [&](int i, s16x8 x) {
+          const int grp = i / ND;                          // 16 keys
+#pragma unroll
+          for (int m = 0; m < MAPS; m++) oacc[m][i % ND] = mma<HALF>(x, frag(pk[m][grp / 2] + 4 * (grp % 2)), oacc[m][i % ND]);
+        });
       }
-      t = tn; buf ^= 1;
     }
+    t = tn; mask = mask_n; buf ^= 1;
+    tn = masks.find(tn + 1, mask_n);
   }
   dma_wait();                                              // no LDS-DMA may outlive the workgroup
   __syncthreads();
@@ -359,7 +461,7 @@ __global__ __launch_bounds__(256, 2) void maps_fwd_kernel(const MapArgs a) {
     inv[m] = l == 0.f ? 0.f : 1.f / l;
     if (a.lse && g == 0 && q_raw < a.Sq) a.lse[(((size_t)b * a.H + h) * MAPS + m) * a.Sq + q_raw] = l == 0.f ? -INFINITY : m_run[m] * LN2 + __logf(l);
   }
-  bf16_t* slab = stage + wave * 32 * 72;
+  bf16_t* slab = stage + wave * SLAB;
   auto rows = [&](bf16_t* base) {
     return [=](int row) -> bf16_t* { return q0 + row < a.Sq ? base + (((size_t)b * a.Sq + q0 + row) * a.H + h) * DV : nullptr; };
   };
@@ -384,7 +486,7 @@ __global__ __launch_bounds__(256, 2) void maps_fwd_split_kernel(const MapArgs a)
   constexpr int DV = MAPS * D, KT = 32 * D, STAGE = MAPS * KT + 32 * DV, NK = D / 16, ND = DV / 32;
   constexpr int NLK = MAPS * 32 * D / 512, NLV = 32 * DV / 512;                 // LDS-DMA instructions of a tile's k and v
   constexpr bool BIAS = MAPS == 1;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   bf16_t* stage = (bf16_t*)smem;                                               // [4 waves][STAGE], then fp32 [4][DV][32] in the same place
   constexpr int SB = 4 * STAGE * 2 > 4 * DV * 32 * 4 ? 4 * STAGE * 2 : 4 * DV * 32 * 4;
   unsigned* sMask = (unsigned*)(smem + SB);                                    // [2 WIN] 32-key masks
@@ -629,44 +731,59 @@ __global__ __launch_bounds__(256) void maps_join_kernel(const MapArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// backward, queries: dq and the row sums r_i = sum_j p_ij dp_ij.  One workgroup = 128 queries of one head, as the forward.
+// backward, queries: dq and the row sums r_i = sum_j p_ij dp_ij.  One workgroup = 32 NW queries of one head, tiles as in the forward.
 // ds = p (dp - r) needs r before the first key: rowsum(dO o) gives it up to the rounding of o, which is enough for dq (16 bits), and the exact
 // fp32 sum falls out of the same registers (one FMA per element): the key kernel forms ds, the bias table's and lam's gradients from that.
+// Row statistics leave as [B][H][64-query tile][MAPS][2][64] floats: log2 of the row sum (ROW_OFF for a row without one), r.
 // ------------------------------------------------------------------------------------------------
-template <bool HALF, int D, int MAPS>
-__global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
-  constexpr int DV = MAPS * D, KT = 64 * D, STAGE = MAPS * KT + 64 * DV, NK = D / 16, NV = DV / 16, ND = D / 32;
+template <bool HALF, int D, int MAPS, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void maps_bwd_q_kernel(const MapArgs a) {
+  constexpr int DV = MAPS * D, KT = 64 * D, STAGE = MAPS * KT + 64 * DV, NK = D / 16, NV = DV / 16, ND = D / 32, RA = 4;
   constexpr bool BIAS = MAPS == 1;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   bf16_t* stage = (bf16_t*)smem;
   unsigned long long* sMask = (unsigned long long*)(smem + 2 * STAGE * 2);
   float* sB = (float*)(sMask + WIN);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;
-  const int nqb = (a.Sq + 127) / 128;
+  const int nqb = (a.Sq + 32 * NW - 1) / (32 * NW);
   int blk, b, h;
   block_id(nqb, a, a.H, blk, b, h);
   if (a.causal) blk = nqb - 1 - blk;
-  const int kh = h / a.G, q0 = blk * 128 + wave * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1);
+  const int kh = h / a.G, qb = blk * 32 * NW, q0 = qb + wave * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1);
   const bool live = q0 < a.Sq;
-  const bf16_t* kb_ = a.k + (long long)b * a.k_sb + (long long)kh * a.k_sh;
-  const bf16_t* vb_ = a.v + (long long)b * a.v_sb + (long long)kh * a.v_sh;
+  const int last_q = min(qb + 32 * NW - 1, a.Sq - 1);
+  int ntiles = (a.Sk + 63) / 64;
+  if (a.causal) ntiles = last_q + a.off < 0 ? 0 : min(ntiles, (last_q + a.off) / 64 + 1);
+  typedef Loader<D, 64, NW> KL;
+  typedef Loader<DV, 64, NW> VL;
+  const KL kl(a.k + (long long)b * a.k_sb + (long long)kh * a.k_sh, a.k_ss, a.Sk - 1, wave, lane);
+  const VL vl(a.v + (long long)b * a.v_sb + (long long)kh * a.v_sh, a.v_ss, a.Sk - 1, wave, lane);
+  auto request = [&](int kt, int buf) {
+    const unsigned s = lds_at(stage) + buf * STAGE * 2;
+#pragma unroll
+    for (int m = 0; m < MAPS; m++) kl.tile(kt * 64, s + m * KT * 2, 2 * m * a.k_sm);
+    vl.tile(kt * 64, s + MAPS * KT * 2, 0);
+  };
+  if (ntiles > 0) request(0, 0);
+  if (ntiles > 1) request(1, 1);
   s16x8 qf[MAPS][NK], of[NV];
   float L[MAPS], del[MAPS], racc[MAPS];
-#pragma unroll
-  for (int m = 0; m < MAPS; m++) {
-#pragma unroll
-    for (int ks = 0; ks < NK; ks++)
-      qf[m][ks] = *(const s16x8*)(a.q + (long long)b * a.q_sb + (long long)qrow * a.q_ss + (long long)h * a.q_sh + m * a.q_sm + 16 * ks + 8 * g);
-    const float l = a.lse_in[(((size_t)b * a.H + h) * MAPS + m) * a.Sq + qrow];
-    L[m] = l == -INFINITY ? ROW_OFF : l * LOG2E;
-    del[m] = 0.f; racc[m] = 0.f;
-  }
   const float lam = MAPS == 2 ? a.lam[h] : 0.f;
   {
     const size_t ro = (((size_t)b * a.Sq + qrow) * a.H + h) * DV + 8 * g;
 #pragma unroll
+    for (int m = 0; m < MAPS; m++) {
+#pragma unroll
+      for (int ks = 0; ks < NK; ks++)
+        qf[m][ks] = *(const s16x8*)(a.q + (long long)b * a.q_sb + (long long)qrow * a.q_ss + (long long)h * a.q_sh + m * a.q_sm + 16 * ks + 8 * g);
+      const float l = a.lse_in[(((size_t)b * a.H + h) * MAPS + m) * a.Sq + qrow];
+      L[m] = l == -INFINITY ? ROW_OFF : l * LOG2E;
+      del[m] = 0.f; racc[m] = 0.f;
+    }
+#pragma unroll
+    for (int ks = 0; ks < NV; ks++) of[ks] = *(const s16x8*)(a.dO + ro + 16 * ks);
+#pragma unroll
     for (int ks = 0; ks < NV; ks++) {
-      of[ks] = *(const s16x8*)(a.dO + ro + 16 * ks);
       const s16x8 x = *(const s16x8*)(a.o + ro + 16 * ks);
       s16x8 y;
       if constexpr (MAPS == 2) y = *(const s16x8*)(a.o2 + ro + 16 * ks);
@@ -683,100 +800,95 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
 #pragma unroll
     for (int m = 0; m < MAPS; m++) del[m] = half_sum(del[m]);
   }
+  Masks<NW> masks(a, b, ntiles, sMask, wave, lane);
+  masks.load();
+  int rlo, rhi;
+  bias_window(a, -(last_q + a.off), ntiles * 64 - 1 - qb - a.off, rlo, rhi);
+  if constexpr (BIAS) load_bias(a, h, rlo, rhi, sB, tid, 64 * NW);
   f32x16 acc[MAPS][ND];
 #pragma unroll
   for (int m = 0; m < MAPS; m++)
 #pragma unroll
     for (int i = 0; i < ND; i++) zero(acc[m][i]);
-  const int last_q = min(blk * 128 + 127, a.Sq - 1);
-  int ntiles = (a.Sk + 63) / 64;
-  if (a.causal) ntiles = last_q + a.off < 0 ? 0 : min(ntiles, (last_q + a.off) / 64 + 1);
-  int rlo, rhi;
-  bias_window(a, -(last_q + a.off), ntiles * 64 - 1 - blk * 128 - a.off, rlo, rhi);
+  const int koff = 2 * Tile<D>::off(l31, 8 * g), voff = 2 * Tile<DV>::off(l31, 8 * g);                // bytes
+  const int toff0 = 2 * Tile<D>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), toff1 = 2 * Tile<D>::rows8(toff0 / 2);
+  __syncthreads();
   float bl = 0.f, br = 0.f;
-  if constexpr (BIAS) load_bias(a, h, rlo, rhi, sB, tid, 256);
-  const int koff = Tile<D>::off(l31, 8 * g), voff = Tile<DV>::off(l31, 8 * g);
-  const int toff0 = Tile<D>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), toff1 = Tile<D>::rows8(toff0);
-  auto request = [&](int kt, int buf) {
-    bf16_t* s = stage + buf * STAGE;
+  if constexpr (BIAS) { bl = rlo <= -a.R ? sB[0] : 0.f; br = rhi >= a.R ? sB[rhi - rlo] : 0.f; }
+  unsigned long long mask = ntiles > 0 ? masks.at(0) : 0, mask_n = ntiles > 1 ? masks.at(1) : 0;
+#pragma nounroll
+  for (int t = 0, tn = min(1, ntiles), buf = 0; t < ntiles;) {
+    dma_wait();
+    __syncthreads();
+    const bool req = tn > 1 && tn < ntiles;
+    bf16_t* sK = stage + buf * STAGE;
+    bf16_t* sV = sK + MAPS * KT;
+    if (mask != ~0ull) {
 #pragma unroll
-    for (int m = 0; m < MAPS; m++) load_tile<D, 64, 4>(kb_ + m * a.k_sm, a.k_ss, kt * 64, a.Sk - 1, s + m * KT, wave, lane);
-    load_tile<DV, 64, 4>(vb_, a.v_ss, kt * 64, a.Sk - 1, s + MAPS * KT, wave, lane);
-  };
-  for (int w0 = 0; w0 < ntiles; w0 += WIN) {
-    const int wn = min(WIN, ntiles - w0);
-    __syncthreads();
-    load_masks(a, b, w0, wn, sMask, wave, lane);
-    __syncthreads();
-    if constexpr (BIAS) if (w0 == 0) { bl = rlo <= -a.R ? sB[0] : 0.f; br = rhi >= a.R ? sB[rhi - rlo] : 0.f; }
-    int t = next_tile(sMask, 0, wn), buf = 0;
-    if (t < wn) request(w0 + t, 0);
-    while (t < wn) {
-      dma_wait();
+      for (int m = 0; m < MAPS; m++) clear_rows<D>(sK + m * KT, mask, 64, tid, 64 * NW);
+      clear_rows<DV>(sV, mask, 64, tid, 64 * NW);
       __syncthreads();
-      const int tn = next_tile(sMask, t + 1, wn);
-      const unsigned long long mask = uniform64(sMask[t]);
-      bf16_t* sK = stage + buf * STAGE;
-      bf16_t* sV = sK + MAPS * KT;
-      if (mask != ~0ull) {
-#pragma unroll
-        for (int m = 0; m < MAPS; m++) clear_rows<D>(sK + m * KT, mask, 64, tid, 256);
-        clear_rows<DV>(sV, mask, 64, tid, 256);
-        __syncthreads();
-      }
-      if (tn < wn) request(w0 + tn, buf ^ 1);
-      const int key0 = (w0 + t) * 64;
-      const int seen = a.causal ? q0 + min(31, a.Sq - 1 - q0) + a.off - key0 : 64;
-      if (live && seen >= 0) {
-        const bool part = mask != ~0ull || (a.causal && q0 + a.off < key0 + 63);
+    }
+    const int key0 = t * 64;
+    const int seen = a.causal ? q0 + min(31, a.Sq - 1 - q0) + a.off - key0 : 64;
+    const bool work = live && seen >= 0;
+    if (req && !work) request(tn, buf ^ 1);
+    if (work) {
+      const bool part = mask != ~0ull || (a.causal && q0 + a.off < key0 + 63);
+      constexpr int NS = NV + MAPS * NK, NP = 2 * MAPS * ND;
 #pragma unroll 1
-        for (int kb = 0; kb < 2; kb++) {
-          f32x16 dp, s[MAPS];
-          zero(dp);
+      for (int kb = 0; kb < 2; kb++) {
+        f32x16 dp, s[MAPS];
+        s16x8 fa[RA];
+        const unsigned ka = opaque(lds_at(sK) + koff + kb * 64 * D), va = DV == D ? ka : opaque(lds_at(sV) + voff + kb * 64 * DV);
+        const unsigned ta0 = opaque(lds_at(sK) + toff0 + kb * 64 * D), ta1 = opaque(lds_at(sK) + toff1 + kb * 64 * D);
+        auto kvrow = [&](int i) { return i < NV ? row_frag(va, i, DV == D ? MAPS * KT * 2 : 0) : row_frag(ka, (i - NV) % NK, (i - NV) / NK * KT * 2); };
+        auto kcol = [&](int i) { return col_frag(ta0, ta1, i % ND, (i / (2 * ND) * KT + i / ND % 2 * 16 * D) * 2); };
+        zero(dp);
 #pragma unroll
-          for (int ks = 0; ks < NV; ks++) dp = mma<HALF>(*(const s16x8*)(sV + Tile<DV>::cols(voff, 16 * ks) + kb * 32 * DV), of[ks], dp);
-          unsigned pk[MAPS][8];
+        for (int m = 0; m < MAPS; m++) zero(s[m]);
+        fill<NS>(fa, kvrow);
+        fence();
+        run<NS>(fa, kvrow, [&](int i, s16x8 x) {
+          const int j = i < NV ? 0 : i - NV;
+          if (i < NV) dp = mma<HALF>(x, of[i < NV ? i : 0], dp); else s[j / NK] = mma<HALF>(x, qf[j / NK][j % NK], s[j / NK]);
+        });
+        if (req && kb == 0) request(tn, buf ^ 1);
+        fill<NP>(fa, kcol);
+        fence();
+        unsigned pk[MAPS][8];
 #pragma unroll
-          for (int m = 0; m < MAPS; m++) {
-            zero(s[m]);
+        for (int m = 0; m < MAPS; m++) {
+          float cc = a.c, cb = 0.f;
+          if constexpr (BIAS) {
+            const int rmin = key0 - q0 - 31 - a.off, rmax = key0 + 63 - q0 - a.off;
+            if (rmin >= a.R) cb = br;
+            else if (rmax <= -a.R) cb = bl;
+            else {
+              const float* bp = sB + (key0 - min(q_raw, last_q) - a.off + 4 * g - rlo);
 #pragma unroll
-            for (int ks = 0; ks < NK; ks++) s[m] = mma<HALF>(*(const s16x8*)(sK + m * KT + Tile<D>::cols(koff, 16 * ks) + kb * 32 * D), qf[m][ks], s[m]);
-            float cc = a.c, cb = 0.f;
-            if constexpr (BIAS) {
-              const int rmin = key0 - q0 - 31 - a.off, rmax = key0 + 63 - q0 - a.off;
-              if (rmin >= a.R) cb = br;
-              else if (rmax <= -a.R) cb = bl;
-              else {
-                const float* bp = sB + (key0 - min(q_raw, last_q) - a.off + 4 * g - rlo);
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[m][r] = fmaf(s[m][r], a.c, bp[kb * 32 + (r & 3) + 8 * (r >> 2)]);
-                cc = 1.f;
-              }
-            }
-            if (part) mask_scores(s[m], (unsigned)(mask >> (32 * kb)), (a.causal ? q_raw + a.off - key0 : 64) - 32 * kb, g, -INFINITY);
-            const float e0 = cb - L[m];
-            const float f = m == 0 ? 1.f : -lam;
-#pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-              const float p0 = ex2(fmaf(s[m][r], cc, e0)), p1 = ex2(fmaf(s[m][r + 1], cc, e0));
-              racc[m] = fmaf(p0, dp[r], racc[m]); racc[m] = fmaf(p1, dp[r + 1], racc[m]);
-              pk[m][r / 2] = pack2<HALF>((m ? f * p0 : p0) * (dp[r] - del[m]), (m ? f * p1 : p1) * (dp[r + 1] - del[m]));
+              for (int r = 0; r < 16; r++) s[m][r] = fmaf(s[m][r], a.c, bp[kb * 32 + (r & 3) + 8 * (r >> 2)]);
+              cc = 1.f;
             }
           }
+          if (part) mask_scores(s[m], (unsigned)(mask >> (32 * kb)), (a.causal ? q_raw + a.off - key0 : 64) - 32 * kb, g, -INFINITY);
+          const float e0 = cb - L[m];
+          const float f = m == 0 ? 1.f : -lam;
 #pragma unroll
-          for (int m = 0; m < MAPS; m++)
-#pragma unroll
-            for (int hf = 0; hf < 2; hf++)
-#pragma unroll
-              for (int i = 0; i < ND; i++) {
-                const int ro = m * KT + (kb * 32 + 16 * hf) * D;
-                const s16x8 kt = cat4(lds_tr16(sK + Tile<D>::cols(toff0, 32 * i) + ro), lds_tr16(sK + Tile<D>::cols(toff1, 32 * i) + ro));
-                acc[m][i] = mma<HALF>(kt, frag(pk[m] + 4 * hf), acc[m][i]);
-              }
+          for (int r = 0; r < 16; r += 2) {
+            const float p0 = ex2(fmaf(s[m][r], cc, e0)), p1 = ex2(fmaf(s[m][r + 1], cc, e0));
+            racc[m] = fmaf(p0, dp[r], racc[m]); racc[m] = fmaf(p1, dp[r + 1], racc[m]);
+            pk[m][r / 2] = pack2<HALF>((m ? f * p0 : p0) * (dp[r] - del[m]), (m ? f * p1 : p1) * (dp[r + 1] - del[m]));
+          }
         }
+        fence();
+        run<NP>(fa, kcol, [&](int i, s16x8 x) {
+          acc[i / (2 * ND)][i % ND] = mma<HALF>(x, frag(pk[i / (2 * ND)] + 4 * (i / ND % 2)), acc[i / (2 * ND)][i % ND]);
+        });
       }
-      t = tn; buf ^= 1;
     }
+    t = tn; mask = mask_n; buf ^= 1;
+    tn = masks.find(tn + 1, mask_n);
   }
   dma_wait();
   __syncthreads();
@@ -784,14 +896,15 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
 #pragma unroll
   for (int m = 0; m < MAPS; m++) {
     const float r = half_sum(racc[m]);
-    if (g == 0 && q_raw < a.Sq) a.rvec[(((size_t)b * a.H + h) * MAPS + m) * a.Sq + q_raw] = r;
+    float* st = a.rvec + ((((size_t)b * a.H + h) * ((a.Sq + 63) / 64) + q0 / 64) * MAPS + m) * 128 + (q0 & 32) + l31;
+    st[g * 64] = g ? r : q_raw < a.Sq ? L[m] : ROW_OFF;
     if (MAPS == 2 && m == MAPS - 1) {                      // lam's gradient: the wave's 32 rows, [H][B][32-row block]
       const float w = wave_sum_dpp(g == 0 && q_raw < a.Sq ? r : 0.f);
       const int n32 = (a.Sq + 31) / 32;
       if (lane == 0) a.part[((size_t)h * a.B + b) * n32 + q0 / 32] = w;
     }
   }
-  bf16_t* slab = stage + wave * 32 * 72;
+  bf16_t* slab = stage + wave * SLAB;
 #pragma unroll
   for (int m = 0; m < MAPS; m++)
     store_rows<HALF, D>(acc[m], a.scale, slab, lane, [=](int row) -> bf16_t* {
@@ -799,42 +912,60 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// backward, keys: dk, dv and (relpos) the bias gradient by relative position.  One workgroup = 128 keys of one key head, 4 waves of 32; it walks
-// the queries of every head of the group in tiles of 64, so that the shared heads' gradients are summed in registers, in a fixed order.
+// backward, keys: dk, dv and (relpos) the bias gradient by relative position.  One workgroup = 128 keys of one key head; it walks the queries of
+// every head of the group in tiles of 64, so that the shared heads' gradients are summed in registers, in a fixed order.  8 waves: wave w has keys
+// 32 (w & 3) .. and of each tile the queries 32 (w >> 2) .., and the two waves of a key block add up at the end: two waves per SIMD, whose LDS round
+// trips, exponentials and MFMAs overlap (one wave of 4 per SIMD, with everything in 420 registers, spent two thirds of its time waiting).
 // ------------------------------------------------------------------------------------------------
 template <bool HALF, int D, int MAPS>
-__global__ __launch_bounds__(256, 1) void maps_bwd_k_kernel(const MapArgs a) {
+__global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
   constexpr int DV = MAPS * D, QT = 64 * D, STAGE = MAPS * QT + 64 * DV, NK = D / 16, NV = DV / 16, ND = D / 32, NDV = DV / 32;
-  constexpr bool BIAS = MAPS == 1;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  constexpr bool BIAS = MAPS == 1, VLDS = DV == 128;       // 128 channels: v's fragments stay in LDS, beside the accumulators they would not fit
+  constexpr int RA = VLDS ? 3 : 4, RV = 2;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   bf16_t* stage = (bf16_t*)smem;
-  float* sStat = (float*)(smem + 2 * STAGE * 2);           // [2][MAPS][2][64]: log2 of the row sums, r
-  float* sDiag = sStat + 2 * MAPS * 2 * 64;                // [4 waves][32 queries][64]: score gradients, row q shifted by q
-  float* sB = sDiag + (BIAS ? 4 * 32 * 64 : 0);
+  bf16_t* sV = stage + 2 * STAGE;
+  float* sStat = (float*)(sV + (VLDS ? 128 * DV : 0));     // [2][2][2][64]: log2 of the row sums, r of a tile's maps
+  float* sDiag = sStat + 2 * 256;                          // [8 waves][16 queries][48]: score gradients, row q shifted by q
+  float* sAny = sDiag + (BIAS ? 8 * 768 : 0);              // [8]
+  float* sB = sAny + 8;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;
+  const int kw = wave & 3, qh = wave >> 2;
   const int nkb = (a.Sk + 127) / 128;
   int blk, b, kh;
   block_id(nkb, a, a.Hkv, blk, b, kh);
-  const int k0 = blk * 128 + wave * 32, key = k0 + l31, krow = min(key, a.Sk - 1);
+  const int k0 = blk * 128 + kw * 32, key = k0 + l31, krow = min(key, a.Sk - 1);
+  const int first = a.causal ? max(0, (blk * 128 - a.off)) / 64 : 0, nq64 = (a.Sq + 63) / 64;          // tiles of queries that see a key
+  typedef Loader<D, 64, 8> QL;
+  typedef Loader<DV, 64, 8> OL;
+  QL ql(a.q + (long long)b * a.q_sb + (long long)kh * a.G * a.q_sh, a.q_ss, a.Sq - 1, wave, lane);
+  OL ol(a.dO + ((size_t)b * a.Sq * a.H + kh * a.G) * DV, (long long)a.H * DV, a.Sq - 1, wave, lane);
+  const float* stat = a.rvec + ((size_t)b * a.H + kh * a.G) * nq64 * MAPS * 128;
+  auto request = [&](int qt, int buf) {
+    const unsigned s = lds_at(stage) + buf * STAGE * 2;
+#pragma unroll
+    for (int m = 0; m < MAPS; m++) ql.tile(qt * 64, s + m * QT * 2, 2 * m * a.q_sm);
+    ol.tile(qt * 64, s + MAPS * QT * 2, 0);
+    if (wave == 7) dma16(stat + (size_t)qt * MAPS * 128, opaque(lane * 16), lds_at((bf16_t*)sStat) + buf * 1024);     // the tile's row statistics
+  };
+  auto request_two = [&]() {
+    if (first < nq64) request(first, 0);
+    if (first + 1 < nq64) request(first + 1, 1);
+  };
+  request_two();
+  // lane = key in every product: whatever a masked key's row holds reaches only its own gradient rows, which are zeroed before the store
   const bool kok = key < a.Sk && (!a.kvalid || a.kvalid[(size_t)b * a.mask_sb + krow] != 0);
-  const bool live = __builtin_amdgcn_ballot_w64(kok) != 0;                    // some key of the wave is not masked
-  // a masked key's row may hold anything: its fragments are zeros, its gradient rows are zeros, and it adds to no bias sum
-  s16x8 kf[MAPS][NK], vf[NV];
-  {
-    const s16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+  const bf16_t* vb_ = a.v + (long long)b * a.v_sb + (long long)kh * a.v_sh;
+  s16x8 kf[MAPS][NK], vf[VLDS ? 1 : NV];
 #pragma unroll
-    for (int m = 0; m < MAPS; m++)
+  for (int m = 0; m < MAPS; m++)
 #pragma unroll
-      for (int ks = 0; ks < NK; ks++) {
-        const s16x8 x = *(const s16x8*)(a.k + (long long)b * a.k_sb + (long long)krow * a.k_ss + (long long)kh * a.k_sh + m * a.k_sm + 16 * ks + 8 * g);
-        kf[m][ks] = kok ? x : z;
-      }
+    for (int ks = 0; ks < NK; ks++)
+      kf[m][ks] = *(const s16x8*)(a.k + (long long)b * a.k_sb + (long long)krow * a.k_ss + (long long)kh * a.k_sh + m * a.k_sm + 16 * ks + 8 * g);
+  if constexpr (VLDS) load_tile<DV, 128, 8>(vb_, a.v_ss, blk * 128, a.Sk - 1, sV, wave, lane);
+  else
 #pragma unroll
-    for (int ks = 0; ks < NV; ks++) {
-      const s16x8 x = *(const s16x8*)(a.v + (long long)b * a.v_sb + (long long)krow * a.v_ss + (long long)kh * a.v_sh + 16 * ks + 8 * g);
-      vf[ks] = kok ? x : z;
-    }
-  }
+    for (int ks = 0; ks < NV; ks++) vf[ks] = *(const s16x8*)(vb_ + (long long)krow * a.v_ss + 16 * ks + 8 * g);
   f32x16 dk[MAPS][ND], dv[NDV];
 #pragma unroll
   for (int m = 0; m < MAPS; m++)
@@ -842,93 +973,87 @@ __global__ __launch_bounds__(256, 1) void maps_bwd_k_kernel(const MapArgs a) {
     for (int i = 0; i < ND; i++) zero(dk[m][i]);
 #pragma unroll
   for (int i = 0; i < NDV; i++) zero(dv[i]);
-  const int qoff = Tile<D>::off(l31, 8 * g), ooff = Tile<DV>::off(l31, 8 * g);
-  const int tq0 = Tile<D>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), tq1 = Tile<D>::rows8(tq0);
-  const int to0 = Tile<DV>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), to1 = Tile<DV>::rows8(to0);
-  // queries that see a key of the workgroup; no tile at all when none does, or when no key of the workgroup is valid
-  const int any = __syncthreads_or(kok ? 1 : 0);
-  const int first = a.causal ? max(0, (blk * 128 - a.off)) / 64 : 0, nqt = any ? max(0, (a.Sq + 63) / 64 - first) : 0;
+  const int qoff = 2 * Tile<D>::off(l31, 8 * g), ooff = 2 * Tile<DV>::off(l31, 8 * g);               // bytes
+  const int tq0 = 2 * Tile<D>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), tq1 = 2 * Tile<D>::rows8(tq0 / 2);
+  const int to0 = 2 * Tile<DV>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), to1 = 2 * Tile<DV>::rows8(to0 / 2);
   int rlo, rhi;
   bias_window(a, blk * 128 - (a.Sq + 63) - a.off, blk * 128 + 127 - first * 64 - a.off, rlo, rhi);
   const int nk32 = (a.Sk + 31) / 32;
-  float* diag = sDiag + wave * 2048;
-  if constexpr (BIAS) {                                    // entries no (query, key) of a 32 x 32 block falls on stay zero for good
+  // sums along the 63 diagonals of a 32 x 32 block in two passes of 16 queries: row q of a pass is written q entries to the left into 47 columns of
+  // 48 (the last, and what no key falls on, stays zero for good); lane l collects relative position l - 31 of the block, column l - 16 of the first
+  // pass and column l of the second
+  float* diag = sDiag + wave * 768;
+  if constexpr (BIAS) {
 #pragma unroll
-    for (int i = 0; i < 32; i++) diag[i * 64 + lane] = 0.f;
+    for (int i = 0; i < 12; i++) diag[i * 64 + lane] = 0.f;
   }
+  const bool live = __builtin_amdgcn_ballot_w64(kok) != 0;
+  if (lane == 0) sAny[wave] = live ? 1.f : 0.f;
+  int nqt = max(0, nq64 - first);
   for (int hg = 0; hg < a.G; hg++) {
     const int h = kh * a.G + hg;
-    const bf16_t* qb_ = a.q + (long long)b * a.q_sb + (long long)h * a.q_sh;
-    const bf16_t* ob_ = a.dO + ((size_t)b * a.Sq * a.H + h) * DV;
-    const float* lse = a.lse_in + ((size_t)b * a.H + h) * MAPS * a.Sq;
-    const float* rv = a.rvec + ((size_t)b * a.H + h) * MAPS * a.Sq;
     const float lam = MAPS == 2 ? a.lam[h] : 0.f;
     float fl = 0.f, fr = 0.f, bl = 0.f, br = 0.f;          // sums and bias of the positions at and behind -R / +R
-    float carry = 0.f;                                     // sums of the last block's lower diagonals, at the lanes they have in the next block
-    int base = 0;
-    bool open = false;
     float* part = nullptr;
-    __syncthreads();                                       // the previous head's tiles, bias and statistics are read
+    if (hg > 0) {
+      __syncthreads();                                     // the previous head's tiles, bias and statistics are read
+      ql.base += 2 * a.q_sh; ol.base += 2 * DV; stat += (size_t)nq64 * MAPS * 128;
+      if (nqt > 0) request_two();
+    }
     if constexpr (BIAS) {
-      load_bias(a, h, rlo, rhi, sB, tid, 256);
-      if (a.part) {
-        part = a.part + (((size_t)h * a.B + b) * nk32 + k0 / 32) * a.gw;
-        if (k0 < a.Sk) for (int i = lane; i < a.gw; i += 64) part[i] = 0.f;     // (done before the first tile's wait)
+      load_bias(a, h, rlo, rhi, sB, tid, 512);
+      if (k0 < a.Sk) {
+        part = a.part + ((((size_t)h * a.B + b) * nk32 + k0 / 32) * 2 + qh) * a.gw;
+        for (int i = lane; i < a.gw; i += 64) part[i] = 0.f;                    // (done before the first tile's wait)
       }
     }
-    float pl = 0.f;
-    auto request = [&](int qt, int buf) {
-      bf16_t* s = stage + buf * STAGE;
-#pragma unroll
-      for (int m = 0; m < MAPS; m++) load_tile<D, 64, 4>(qb_ + m * a.q_sm, a.q_ss, qt * 64, a.Sq - 1, s + m * QT, wave, lane);
-      load_tile<DV, 64, 4>(ob_, (long long)a.H * DV, qt * 64, a.Sq - 1, s + MAPS * QT, wave, lane);
-      if (tid < MAPS * 128) {                              // thread = (map, statistic, row)
-        const int m = tid >> 7, row = min(qt * 64 + (tid & 63), a.Sq - 1);
-        pl = (tid & 64 ? rv : lse)[m * a.Sq + row];
-      }
-    };
-    auto stats = [&](int qt, int buf) {
-      if (tid < MAPS * 128) sStat[buf * MAPS * 128 + tid] = tid & 64 ? pl : (qt * 64 + (tid & 63) >= a.Sq || pl == -INFINITY) ? ROW_OFF : pl * LOG2E;
-    };
-    // lane l <-> relative position base + l - 31 (l < 63) of a block whose first key is `base` ahead of its first query.  The next block starts 32
-    // queries later: the upper 32 positions are complete and leave, the lower 31 move up 32 lanes and wait for it.
-    auto leave = [&](float v, int base_) {
-      const int rel = base_ + lane - 31;
-      if (lane >= 31 && lane < 63) {
-        if (rel >= a.R) fr += v;
-        else if (rel <= -a.R) fl += v;
-        else if (rel >= a.glo && rel < a.glo + a.gw) part[rel - a.glo] = v;
-      }
-      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
-      carry = lane >= 32 && lane < 63 ? __int_as_float(sw[0]) : 0.f;
-    };
-    if (nqt > 0) { request(first, 0); stats(first, 0); }
+    __syncthreads();
+    if (hg == 0 && __builtin_amdgcn_readfirstlane(__float_as_int(sAny[0] + sAny[1] + sAny[2] + sAny[3])) == 0) nqt = 0;     // no key of the workgroup is valid
+    if constexpr (BIAS) { bl = rlo <= -a.R ? sB[0] : 0.f; br = rhi >= a.R ? sB[rhi - rlo] : 0.f; }
+#pragma nounroll
     for (int n = 0; n < nqt; n++) {
-      const int qt = first + n, buf = n & 1;
+      const int qt = first + n, buf = n & 1, q0 = qt * 64 + qh * 32;
       dma_wait();
       __syncthreads();
-      if (n == 0) if constexpr (BIAS) { bl = rlo <= -a.R ? sB[0] : 0.f; br = rhi >= a.R ? sB[rhi - rlo] : 0.f; }
-      if (n + 1 < nqt) request(qt + 1, buf ^ 1);
-      bf16_t* sQ = stage + buf * STAGE;
-      bf16_t* sO = sQ + MAPS * QT;
-      const float* st = sStat + buf * MAPS * 128;
-#pragma unroll 1
-      for (int qs = 0; qs < 2; qs++) {
-        const int q0 = qt * 64 + qs * 32;
-        if (q0 >= a.Sq || !live || (a.causal && q0 + 31 + a.off < k0)) continue;
+      const bool req = n > 0 && n + 1 < nqt;
+      const bool work = live && q0 < a.Sq && !(a.causal && q0 + 31 + a.off < k0);
+      if (req && !work) request(qt + 1, buf ^ 1);
+      if (work) {
+        const bf16_t* sQ = stage + buf * STAGE + qh * 32 * D;
+        const bf16_t* sO = stage + buf * STAGE + MAPS * QT + qh * 32 * DV;
+        const float* st = sStat + buf * 256 + qh * 32;
+        constexpr int NS = MAPS * NK, NP = NDV + MAPS * ND;
         f32x16 s[MAPS], dp;
         zero(dp);
 #pragma unroll
-        for (int m = 0; m < MAPS; m++) {
-          zero(s[m]);
+        for (int m = 0; m < MAPS; m++) zero(s[m]);
+        s16x8 fa[RA], fv[VLDS ? RV : 1];
+        const unsigned qa = opaque(lds_at(sQ) + qoff), oa = DV == D ? qa : opaque(lds_at(sO) + ooff);
+        const unsigned qt0 = opaque(lds_at(sQ) + tq0), qt1 = opaque(lds_at(sQ) + tq1), ot0 = DV == D ? qt0 : opaque(lds_at(sO) + to0), ot1 = DV == D ? qt1 : opaque(lds_at(sO) + to1);
+        constexpr int OB = DV == D ? MAPS * QT * 2 : 0;    // (one map: dO's tile is q's, one tile further)
+        auto qorow = [&](int i) { return i < NS ? row_frag(qa, i % NK, i / NK * QT * 2) : row_frag(oa, i - NS, OB); };
+        const unsigned va = VLDS ? opaque(lds_at(sV) + kw * 64 * DV + ooff) : 0;
+        fill<NS + NV>(fa, qorow);
+        fence();
 #pragma unroll
-          for (int ks = 0; ks < NK; ks++) s[m] = mma<HALF>(*(const s16x8*)(sQ + m * QT + Tile<D>::cols(qoff, 16 * ks) + qs * 32 * D), kf[m][ks], s[m]);
+        for (int i = 0; i < NS + NV; i++) {
+          if (i < NS) s[i < NS ? i / NK : 0] = mma<HALF>(fa[i % RA], kf[i < NS ? i / NK : 0][i % NK], s[i < NS ? i / NK : 0]);
+          else dp = mma<HALF>(fa[i % RA], VLDS ? fv[(i + RV - NS) % RV] : vf[VLDS || i < NS ? 0 : i - NS], dp);
+          if (i + RA < NS + NV) fa[i % RA] = qorow(i + RA);
+          if (VLDS && i + RV >= NS && i + RV < NS + NV) fv[(i + RV - NS) % RV] = row_frag(va, i + RV - NS, 0);
+          fence();
         }
-#pragma unroll
-        for (int ks = 0; ks < NV; ks++) dp = mma<HALF>(*(const s16x8*)(sO + Tile<DV>::cols(ooff, 16 * ks) + qs * 32 * DV), vf[ks], dp);
+        if (req) request(qt + 1, buf ^ 1);                 // (while the score MFMAs run)
+        // transposed fragments, 16 queries (hf) x 32 channels: dO's NDV blocks, then q's ND blocks of each map
+        auto tcol = [&](int i) {
+          const int hf = i / NP, c = i % NP;
+          if (c < NDV) return col_frag(ot0, ot1, c, OB + 32 * hf * DV);
+          return col_frag(qt0, qt1, (c - NDV) % ND, (c - NDV) / ND * QT * 2 + 32 * hf * D);
+        };
+        if constexpr (!VLDS) { fill<2 * NP>(fa, tcol); fence(); }                // (arrive under the softmax arithmetic)
         // register r <-> query q0 + (r & 3) + 8 (r >> 2) + 4 g, lane <-> key
         const int rb = k0 - q0 - a.off;                    // relative position of the block's first key and first query
-        const bool right = BIAS && rb - 31 >= a.R, left = BIAS && rb + 31 <= -a.R, near = BIAS && !right && !left;
+        const bool right = BIAS && rb - 31 >= a.R, left = BIAS && rb + 31 <= -a.R, close = BIAS && !right && !left;
         float cc = a.c, cb = 0.f;
         if constexpr (BIAS) {
           if (right) cb = br;
@@ -936,7 +1061,10 @@ __global__ __launch_bounds__(256, 1) void maps_bwd_k_kernel(const MapArgs a) {
           else {
             const float* bp = sB + (rb + l31 - 4 * g - 27 - rlo);
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[0][r] = fmaf(s[0][r], a.c, bp[27 - (r & 3) - 8 * (r >> 2)]);
+            for (int j = 0; j < 4; j++) {
+#pragma unroll
+              for (int e = 0; e < 4; e++) s[0][4 * j + e] = fmaf(s[0][4 * j + e], a.c, bp[27 - e - 8 * j]);
+            }
             cc = 1.f;
           }
         }
@@ -948,89 +1076,80 @@ __global__ __launch_bounds__(256, 1) void maps_bwd_k_kernel(const MapArgs a) {
             for (int r = 0; r < 16; r++) if ((r & 3) + 8 * (r >> 2) < lim) s[m][r] = -INFINITY;
         }
         unsigned pp[8], pd[MAPS][8];
-        float ds0[16];
+        float far = 0.f, dsum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          f32x4 L[MAPS], r_[MAPS];
+        for (int ps = 0; ps < 2; ps++) {                   // 16 queries
+          float ds0[8];
 #pragma unroll
-          for (int m = 0; m < MAPS; m++) {
-            L[m] = *(const f32x4*)(st + m * 128 + qs * 32 + 8 * j + 4 * g);
-            r_[m] = *(const f32x4*)(st + m * 128 + 64 + qs * 32 + 8 * j + 4 * g);
-          }
+          for (int j = 2 * ps; j < 2 * ps + 2; j++) {
+            f32x4 L[MAPS], r_[MAPS];
 #pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            float p[2], d0[2], d1[2];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-              const int r = 4 * j + e + u;
-              p[u] = ex2(fmaf(s[0][r], cc, cb - L[0][e + u]));
-              d0[u] = p[u] * (dp[r] - r_[0][e + u]);
-              if constexpr (BIAS) ds0[r] = d0[u];
-              if constexpr (MAPS == 2) {
-                const float p2 = -lam * ex2(fmaf(s[MAPS - 1][r], cc, -L[MAPS - 1][e + u]));
-                d1[u] = p2 * (dp[r] - r_[MAPS - 1][e + u]);
-                p[u] += p2;
-              }
+            for (int m = 0; m < MAPS; m++) {
+              L[m] = *(const f32x4*)(st + m * 128 + 8 * j + 4 * g);
+              r_[m] = *(const f32x4*)(st + m * 128 + 64 + 8 * j + 4 * g);
             }
-            pp[2 * j + e / 2] = pack2<HALF>(p[0], p[1]);
-            pd[0][2 * j + e / 2] = pack2<HALF>(d0[0], d0[1]);
-            if constexpr (MAPS == 2) pd[MAPS - 1][2 * j + e / 2] = pack2<HALF>(d1[0], d1[1]);
-          }
-        }
-        if constexpr (BIAS) {
-          if (part) {
-            if (near) {
-              // sums along the block's 63 diagonals: row q of the block is written q entries to the left, lane l adds up column l
 #pragma unroll
-              for (int r = 0; r < 16; r++) {
-                const int q = (r & 3) + 8 * (r >> 2);
-                diag[(q + 4 * g) * 64 + 31 - q - 4 * g + l31] = kok ? ds0[r] : 0.f;
+            for (int e = 0; e < 4; e += 2) {
+              float p[2], d0[2], d1[2];
+#pragma unroll
+              for (int u = 0; u < 2; u++) {
+                const int r = 4 * j + e + u;
+                p[u] = ex2(fmaf(s[0][r], cc, cb - L[0][e + u]));
+                d0[u] = p[u] * (dp[r] - r_[0][e + u]);
+                if constexpr (BIAS) { far += d0[u]; ds0[r - 8 * ps] = d0[u]; }
+                if constexpr (MAPS == 2) {
+                  const float p2 = -lam * ex2(fmaf(s[MAPS - 1][r], cc, -L[MAPS - 1][e + u]));
+                  d1[u] = p2 * (dp[r] - r_[MAPS - 1][e + u]);
+                  p[u] += p2;
+                }
+              }
+              pp[2 * j + e / 2] = pack2<HALF>(p[0], p[1]);
+              pd[0][2 * j + e / 2] = pack2<HALF>(d0[0], d0[1]);
+              if constexpr (MAPS == 2) pd[MAPS - 1][2 * j + e / 2] = pack2<HALF>(d1[0], d1[1]);
+            }
+          }
+          if constexpr (BIAS) {
+            if (close) {
+              if (kok) {                                   // (a masked key's entries stay zero, too)
+#pragma unroll
+                for (int r = 0; r < 8; r++) diag[(4 * g + (r & 3) + 8 * (r >> 2)) * 47 + 15 + l31] = ds0[r];
               }
               __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
               __builtin_amdgcn_wave_barrier();
               float t[4] = {0.f, 0.f, 0.f, 0.f};
+              const float* col = diag + (ps ? (lane < 47 ? lane : 47) : (lane >= 16 && lane < 63 ? lane - 16 : 47));
 #pragma unroll
-              for (int i = 0; i < 32; i++) t[i & 3] += diag[i * 64 + lane];
+              for (int i = 0; i < 16; i++) t[i & 3] += col[i * 48];
               __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
               __builtin_amdgcn_wave_barrier();
-              leave(((t[0] + t[1]) + (t[2] + t[3])) + carry, rb);
-              open = true; base = rb - 32;
-            } else {
-              float t = 0.f;
-#pragma unroll
-              for (int r = 0; r < 16; r++) t += ds0[r];
-              t = kok ? t : 0.f;
-              if (right) fr += t; else fl += t;
-              if (left && open) { leave(carry, rb); open = false; }
+              dsum += (t[0] + t[1]) + (t[2] + t[3]);
             }
           }
         }
-#pragma unroll
-        for (int hf = 0; hf < 2; hf++) {
-          const s16x8 p8 = frag(pp + 4 * hf);
-#pragma unroll
-          for (int i = 0; i < NDV; i++) {
-            const int ro = (qs * 32 + 16 * hf) * DV;
-            const s16x8 ot = cat4(lds_tr16(sO + Tile<DV>::cols(to0, 32 * i) + ro), lds_tr16(sO + Tile<DV>::cols(to1, 32 * i) + ro));
-            dv[i] = mma<HALF>(ot, p8, dv[i]);
-          }
-#pragma unroll
-          for (int m = 0; m < MAPS; m++) {
-            const s16x8 d8 = frag(pd[m] + 4 * hf);
-#pragma unroll
-            for (int i = 0; i < ND; i++) {
-              const int ro = m * QT + (qs * 32 + 16 * hf) * D;
-              const s16x8 qt_ = cat4(lds_tr16(sQ + Tile<D>::cols(tq0, 32 * i) + ro), lds_tr16(sQ + Tile<D>::cols(tq1, 32 * i) + ro));
-              dk[m][i] = mma<HALF>(qt_, d8, dk[m][i]);
+        if constexpr (BIAS) {
+          if (close) {
+            const int rel = rb + lane - 31;                // (the wave's blocks are 64 queries apart: no other one has these positions)
+            if (lane < 63) {
+              if (rel >= a.R) fr += dsum;
+              else if (rel <= -a.R) fl += dsum;
+              else if (rel >= a.glo && rel < a.glo + a.gw) part[rel - a.glo] = dsum;
             }
+          } else {
+            far = kok ? far : 0.f;
+            if (right) fr += far; else fl += far;
           }
         }
+        fence();
+        if constexpr (VLDS) { fill<2 * NP>(fa, tcol); fence(); }
+        run<2 * NP>(fa, tcol, [&](int i, s16x8 f) {
+          const int hf = i / NP, c = i % NP;
+          if (c < NDV) dv[c] = mma<HALF>(f, frag(pp + 4 * hf), dv[c]);
+          else dk[(c - NDV) / ND][(c - NDV) % ND] = mma<HALF>(f, frag(pd[(c - NDV) / ND] + 4 * hf), dk[(c - NDV) / ND][(c - NDV) % ND]);
+        });
       }
-      if (n + 1 < nqt) stats(qt + 1, buf ^ 1);
     }
     if constexpr (BIAS) {
-      if (part && k0 < a.Sk) {
-        if (open) leave(carry, base);
+      if (part) {
         fl = wave_sum_dpp(fl); fr = wave_sum_dpp(fr);
         if (lane == 0) {                                   // (position -R / +R outside the reachable window: its sum is 0)
           if (-a.R >= a.glo && -a.R < a.glo + a.gw) part[-a.R - a.glo] = fl;
@@ -1040,27 +1159,47 @@ __global__ __launch_bounds__(256, 1) void maps_bwd_k_kernel(const MapArgs a) {
     }
   }
   dma_wait();
+  // the two waves of a key block meet: the upper one hands over its dk and takes the lower one's dv, one accumulator tile of all four pairs at a time
+  constexpr int NT = MAPS * ND > NDV ? MAPS * ND : NDV;
+  float* swap = (float*)smem;                              // [8 waves][16 registers][64 lanes] = 32 KB
+#pragma unroll
+  for (int i = 0; i < NT; i++) {
+    __syncthreads();
+    float* w = swap + wave * 1024 + lane;
+    const float* o = swap + (wave ^ 4) * 1024 + lane;
+    if (qh ? i < MAPS * ND : i < NDV) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) w[r * 64] = qh ? dk[(i < MAPS * ND ? i : 0) / ND][(i < MAPS * ND ? i : 0) % ND][r] : dv[i < NDV ? i : 0][r];
+    }
+    __syncthreads();
+    if (qh ? i < NDV : i < MAPS * ND) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        if (qh) dv[i < NDV ? i : 0][r] += o[r * 64]; else dk[(i < MAPS * ND ? i : 0) / ND][(i < MAPS * ND ? i : 0) % ND][r] += o[r * 64];
+      }
+    }
+  }
   __syncthreads();
   if (k0 >= a.Sk) return;
-  bf16_t* slab = stage + wave * 32 * 72;
-  if (!kok) {                                              // lane = key: its rows are zeros, whatever the unmasked arithmetic left in them
+  bf16_t* slab = stage + wave * SLAB;
+  if (!qh) {
 #pragma unroll
-    for (int m = 0; m < MAPS; m++)
+    for (int m = 0; m < MAPS; m++) {
 #pragma unroll
-      for (int i = 0; i < ND; i++) zero(dk[m][i]);
+      for (int i = 0; i < ND; i++) if (!kok) zero(dk[m][i]);
+      store_rows<HALF, D>(dk[m], a.scale, slab, lane, [=](int row) -> bf16_t* {
+        return k0 + row < a.Sk ? a.dk + ((((size_t)b * a.Sk + k0 + row) * a.Hkv + kh) * MAPS + m) * D : nullptr; });
+    }
+  } else {
 #pragma unroll
-    for (int i = 0; i < NDV; i++) zero(dv[i]);
+    for (int i = 0; i < NDV; i++) if (!kok) zero(dv[i]);
+    store_rows<HALF, DV>(dv, 1.f, slab, lane, [=](int row) -> bf16_t* {
+      return k0 + row < a.Sk ? a.dv + (((size_t)b * a.Sk + k0 + row) * a.Hkv + kh) * DV : nullptr; });
   }
-#pragma unroll
-  for (int m = 0; m < MAPS; m++)
-    store_rows<HALF, D>(dk[m], a.scale, slab, lane, [=](int row) -> bf16_t* {
-      return k0 + row < a.Sk ? a.dk + ((((size_t)b * a.Sk + k0 + row) * a.Hkv + kh) * MAPS + m) * D : nullptr; });
-  store_rows<HALF, DV>(dv, 1.f, slab, lane, [=](int row) -> bf16_t* {
-    return k0 + row < a.Sk ? a.dv + (((size_t)b * a.Sk + k0 + row) * a.Hkv + kh) * DV : nullptr; });
 }
 
 // ------------------------------------------------------------------------------------------------
-// bias table's gradient: part [H][B x 32-key blocks][gw] -> sums over a chunk of rows -> sums over the positions of a bucket.  Fixed order.
+// bias table's gradient: part [H][B x 32-key blocks x 2][gw] -> sums over a chunk of rows -> sums over the positions of a bucket.  Fixed order.
 // ------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void diag_sum_kernel(const float* part, long long rows, int gw, int chunk, float* out) {
   __shared__ float red[4][64];
@@ -1075,17 +1214,27 @@ __global__ __launch_bounds__(256) void diag_sum_kernel(const float* part, long l
   __syncthreads();
   if (w == 0 && col < gw) out[((size_t)h * gridDim.y + blockIdx.y) * gw + col] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
 }
-__global__ __launch_bounds__(64) void bucket_sum_kernel(const float* sums, int chunks, int gw, int glo, const int* buckets, int R, int NB, int H, float* dtable) {
-  const int bk = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-  double x = 0.;
-  for (int i = lane; i < gw; i += 64) {
-    const int rel = min(max(glo + i, -R), R);
-    if (min(max(buckets[rel + R], 0), NB - 1) != bk) continue;
+// one workgroup per head: position sums in 64 bits and the positions' buckets to LDS, then a wave per bucket
+__global__ __launch_bounds__(1024) void bucket_sum_kernel(const float* sums, int chunks, int gw, int glo, const int* buckets, int R, int NB, int H, float* dtable) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem2[];
+  double* sS = (double*)smem2;
+  int* sM = (int*)(sS + gw);
+  const int h = blockIdx.x, lane = threadIdx.x & 63;
+  for (int i = threadIdx.x; i < gw; i += 1024) {
+    double x = 0.;
+#pragma unroll 8
     for (int c = 0; c < chunks; c++) x += (double)sums[((size_t)h * chunks + c) * gw + i];
+    sS[i] = x;
+    sM[i] = min(max(buckets[min(max(glo + i, -R), R) + R], 0), NB - 1);
   }
+  __syncthreads();
+  for (int bk = threadIdx.x >> 6; bk < NB; bk += 16) {
+    double x = 0.;
+    for (int i = lane; i < gw; i += 64) x += sM[i] == bk ? sS[i] : 0.;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
-  if (lane == 0) dtable[(size_t)bk * H + h] = (float)x;
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+    if (lane == 0) dtable[(size_t)bk * H + h] = (float)x;
+  }
 }
 // lam's gradient: minus the sum of a head's n partial row sums
 __global__ __launch_bounds__(256) void lam_sum_kernel(const float* part, long long n, float* dlam) {
@@ -1104,8 +1253,9 @@ __global__ __launch_bounds__(256) void lam_sum_kernel(const float* part, long lo
 // ------------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------------
-constexpr int MAX_REACH = 8191, MAX_BUCKETS = 1 << 16;
-constexpr int DIAG_BYTES = 4 * 32 * 64 * 4;                // skewed score gradients of the key kernel's waves
+constexpr int MAX_REACH = 4095, MAX_BUCKETS = 8192;
+constexpr size_t SWAP_BYTES = 8 * 32 * 72 * 2 > 8 * 16 * 64 * 4 ? 8 * 32 * 72 * 2 : 8 * 16 * 64 * 4;   // end of the key kernel: exchange, then store slabs
+constexpr int DIAG_BYTES = 8 * 768 * 4;                   // skewed score gradients of the key kernel's waves
 
 int check_attn(const uvtg_attn_dims* d, int maps) {
   if (!d) return -10;
@@ -1120,6 +1270,7 @@ int check_attn(const uvtg_attn_dims* d, int maps) {
   if ((long long)((d->Sq + 31) / 32) * d->B * d->H > 0x7fffffffll || (long long)((d->Sk + 31) / 32) * d->B * d->Hkv > 0x7fffffffll) return -34;
   const long long st[] = {d->q_sb, d->q_ss, d->q_sh, d->k_sb, d->k_ss, d->k_sh, d->v_sb, d->v_ss, d->v_sh, maps == 2 ? d->q_sm : 0, maps == 2 ? d->k_sm : 0};
   for (long long s : st) if (s % 8 || s < 0) return -35;
+  if (d->q_ss > (1 << 26) || d->k_ss > (1 << 26) || d->v_ss > (1 << 26)) return -38;
   if (maps == 1) {
     if (d->reach < 1 || d->reach > MAX_REACH) return -36;
     if (d->n_buckets < 1 || d->n_buckets > MAX_BUCKETS) return -37;
@@ -1144,7 +1295,7 @@ SplitPlan plan_split(const uvtg_attn_dims* d, int maps) {
   }
   p.blocks = ((G + p.hb - 1) / p.hb) * ((p.hb * d->Sq + 31) / 32);
   const long long base = (long long)p.blocks * d->B * d->Hkv;
-  const long long want = (512 + base - 1) / base, most = (d->Sk + 127) / 128;
+  const long long want = (512 + base - 1) / base, most = d->Sk / 256;
   p.nsplit = (int)(want < most ? want : most);
   if (p.nsplit > 128) p.nsplit = 128;
   if (p.nsplit < 1) p.nsplit = 1;
@@ -1162,13 +1313,13 @@ struct BwdWs { size_t rvec, part, sums, total; long long rows; int chunk, chunks
 BwdWs bwd_ws(const uvtg_attn_dims* d, int maps) {
   BwdWs w;
   w.rvec = 0;
-  size_t at = align256((size_t)d->B * d->H * maps * d->Sq * 4);
+  size_t at = align256((size_t)d->B * d->H * ((d->Sq + 63) / 64) * maps * 512 + 512);     // (a tile's statistics are fetched 1024 bytes at a time)
   w.part = at;
   if (maps == 1) {
     int glo, gw;
     reachable(d, glo, gw);
-    w.rows = (long long)d->B * ((d->Sk + 31) / 32);
-    w.chunk = w.rows > 256 * 1024 ? (int)((w.rows + 1023) / 1024) : 256;
+    w.rows = (long long)d->B * ((d->Sk + 31) / 32) * 2;
+    w.chunk = w.rows > 64 * 128 ? (int)((w.rows + 63) / 64) : 128;
     w.chunks = (int)((w.rows + w.chunk - 1) / w.chunk);
     at += align256((size_t)d->H * w.rows * gw * 4);
     w.sums = at;
@@ -1194,6 +1345,9 @@ MapArgs map_args(const uvtg_attn_dims* d) {
   return a;
 }
 
+// 8 waves to a row block share a tile's requests where the rows fill them
+bool wide_rows(const uvtg_attn_dims* d) { return d->Sq >= 512; }
+
 // entries of the bias window of a workgroup of `rows` rows
 size_t window_bytes(const uvtg_attn_dims* d, int maps, int rows, long long other) {
   if (maps == 2) return 0;
@@ -1201,12 +1355,17 @@ size_t window_bytes(const uvtg_attn_dims* d, int maps, int rows, long long other
   return (size_t)(w < most ? w : most) * 4;
 }
 
+// LDS of the kernels that walk key tiles: two stages (or, at the end, the waves' store slabs), masks, bias window
+template <int D, int MAPS, int NW> size_t lds_rows(const uvtg_attn_dims* d) {
+  const size_t tiles = 2 * 64 * 2 * MAPS * D * 2, slabs = NW * SLAB * 2, t = (tiles > slabs ? tiles : slabs);
+  return t + WIN * 8 + window_bytes(d, MAPS, 32 * NW, d->Sk);
+}
 template <bool HALF, int D, int MAPS> int run_fwd(const uvtg_attn_dims* d, MapArgs a, hipStream_t s) {
   constexpr int DV = MAPS * D;
   const SplitPlan p = plan_split(d, MAPS);
   if (!p.use) {
-    const size_t lds = 2 * 64 * (MAPS * D + DV) * 2 + WIN * 8 + window_bytes(d, MAPS, 128, d->Sk);
-    hipLaunchKernelGGL((maps_fwd_kernel<HALF, D, MAPS>), dim3((unsigned)((d->Sq + 127) / 128) * d->H * d->B), dim3(256), lds, s, a);
+    if (wide_rows(d)) hipLaunchKernelGGL((maps_fwd_kernel<HALF, D, MAPS, 8>), dim3((unsigned)((d->Sq + 255) / 256) * d->H * d->B), dim3(512), (lds_rows<D, MAPS, 8>(d)), s, a);
+    else hipLaunchKernelGGL((maps_fwd_kernel<HALF, D, MAPS, 4>), dim3((unsigned)((d->Sq + 127) / 128) * d->H * d->B), dim3(256), (lds_rows<D, MAPS, 4>(d)), s, a);
     UVTG_CHECK_LAUNCH();
     return 0;
   }
@@ -1226,20 +1385,21 @@ template <bool HALF, int D, int MAPS> int run_bwd(const uvtg_attn_dims* d, MapAr
   constexpr int DV = MAPS * D;
   const BwdWs w = bwd_ws(d, MAPS);
   a.rvec = (float*)(ws + w.rvec);
-  a.part = (MAPS == 2 || dsum) ? (float*)(ws + w.part) : nullptr;
+  a.part = (float*)(ws + w.part);
   if (MAPS == 1) reachable(d, a.glo, a.gw);
-  const size_t lds_q = 2 * 64 * (MAPS * D + DV) * 2 + WIN * 8 + window_bytes(d, MAPS, 128, d->Sk);
-  hipLaunchKernelGGL((maps_bwd_q_kernel<HALF, D, MAPS>), dim3((unsigned)((d->Sq + 127) / 128) * d->H * d->B), dim3(256), lds_q, s, a);
+  if (wide_rows(d)) hipLaunchKernelGGL((maps_bwd_q_kernel<HALF, D, MAPS, 8>), dim3((unsigned)((d->Sq + 255) / 256) * d->H * d->B), dim3(512), (lds_rows<D, MAPS, 8>(d)), s, a);
+  else hipLaunchKernelGGL((maps_bwd_q_kernel<HALF, D, MAPS, 4>), dim3((unsigned)((d->Sq + 127) / 128) * d->H * d->B), dim3(256), (lds_rows<D, MAPS, 4>(d)), s, a);
   UVTG_CHECK_LAUNCH();
-  const size_t lds_k = 2 * 64 * (MAPS * D + DV) * 2 + 2 * MAPS * 2 * 64 * 4 + (MAPS == 1 ? DIAG_BYTES : 0) + window_bytes(d, MAPS, 128, d->Sq);
-  hipLaunchKernelGGL((maps_bwd_k_kernel<HALF, D, MAPS>), dim3((unsigned)((d->Sk + 127) / 128) * d->Hkv * d->B), dim3(256), lds_k, s, a);
+  const size_t need_k = 2 * 64 * (MAPS * D + DV) * 2 + (DV == 128 ? 128 * DV * 2 : 0) + 2 * 1024 + (MAPS == 1 ? DIAG_BYTES : 0) + 32 + window_bytes(d, MAPS, 128, d->Sq);
+  const size_t lds_k = need_k > SWAP_BYTES ? need_k : SWAP_BYTES;
+  hipLaunchKernelGGL((maps_bwd_k_kernel<HALF, D, MAPS>), dim3((unsigned)((d->Sk + 127) / 128) * d->Hkv * d->B), dim3(512), lds_k, s, a);
   UVTG_CHECK_LAUNCH();
   if (!dsum) return 0;
   if (MAPS == 1) {
     float* sums = (float*)(ws + w.sums);
     hipLaunchKernelGGL(diag_sum_kernel, dim3((a.gw + 63) / 64, w.chunks, d->H), dim3(256), 0, s, a.part, w.rows, a.gw, w.chunk, sums);
     UVTG_CHECK_LAUNCH();
-    hipLaunchKernelGGL(bucket_sum_kernel, dim3(d->n_buckets, d->H), dim3(64), 0, s, sums, w.chunks, a.gw, a.glo, a.buckets, a.R, a.NB, a.H, dsum);
+    hipLaunchKernelGGL(bucket_sum_kernel, dim3(d->H), dim3(1024), (size_t)a.gw * 12, s, sums, w.chunks, a.gw, a.glo, a.buckets, a.R, a.NB, a.H, dsum);
   } else hipLaunchKernelGGL(lam_sum_kernel, dim3(d->H), dim3(256), 0, s, a.part, w.rows, dsum);
   UVTG_CHECK_LAUNCH();
   return 0;

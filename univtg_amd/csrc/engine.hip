@@ -540,7 +540,8 @@ extern "C" const char* uvtg_strerror(int code) {
     case -33: return "attention: scale must be positive and finite";
     case -34: return "attention: length, offset or batch x heads beyond what the kernels address";
     case -35: return "attention: strides and addresses must be non-negative multiples of 16 bytes";
-    case -36: return "attention: reach must be 1 .. 8191";
+    case -38: return "attention: positions more than 2^26 elements apart";
+    case -36: return "attention: reach must be 1 .. 4095";
     case -37: return "attention: n_buckets must be 1 .. 65536";
     default: return "invalid argument";
   }
