@@ -182,7 +182,7 @@ template <int W> __device__ __forceinline__ void clear_rows(bf16_t* tile, unsign
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // Key masks of the tiles of 64 keys, one 64-bit word each: of up to WIN tiles from w0 on in LDS, or plain arithmetic where there is no mask
-template <int NW> struct Masks {
+struct Masks {
   const unsigned char* kv;
   unsigned long long* words;
   int w0, Sk, ntiles, wave, lane;
@@ -192,7 +192,7 @@ template <int NW> struct Masks {
     if (!kv) return;
     const int n = min(WIN, ntiles - w0);
 #pragma unroll 4
-    for (int t = wave; t < n; t += NW) {
+    for (int t = wave; t < n; t += 4) {
       const int key = (w0 + t) * 64 + lane;
       const unsigned long long m = __builtin_amdgcn_ballot_w64(key < Sk && kv[min(key, Sk - 1)] != 0);
       if (lane == 0) words[t] = m;
@@ -290,11 +290,11 @@ __device__ __forceinline__ void mask_scores(f32x16& s, unsigned mask32, int lim,
 }
 
 // ------------------------------------------------------------------------------------------------
-// forward: one workgroup = 32 NW queries of one head, a wave of 32 each, 64-key tiles in two LDS stages.  The first two tiles are requested before
+// forward: one workgroup = 128 queries of one head, a wave of 32 each, 64-key tiles in two LDS stages.  The first two tiles are requested before
 // anything else is known; from then on the requests of the next tile go out between the MFMAs of the current one.
 // ------------------------------------------------------------------------------------------------
-template <bool HALF, int D, int MAPS, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void maps_fwd_kernel(const MapArgs a) {
+template <bool HALF, int D, int MAPS>
+__global__ __launch_bounds__(256, 2) void maps_fwd_kernel(const MapArgs a) {
   constexpr int DV = MAPS * D, KT = 64 * D, STAGE = MAPS * KT + 64 * DV, NK = D / 16, ND = DV / 32, NB = MAPS == 2 ? 1 : 2, RA = 4;
   constexpr bool BIAS = MAPS == 1;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -302,17 +302,17 @@ __global__ __launch_bounds__(64 * NW, 2) void maps_fwd_kernel(const MapArgs a) {
   unsigned long long* sMask = (unsigned long long*)(smem + 2 * STAGE * 2);
   float* sB = (float*)(sMask + WIN);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;
-  const int nqb = (a.Sq + 32 * NW - 1) / (32 * NW);
+  const int nqb = (a.Sq + 127) / 128;
   int blk, b, h;
   block_id(nqb, a, a.H, blk, b, h);
   if (a.causal) blk = nqb - 1 - blk;                     // the longest rows first
-  const int kh = h / a.G, qb = blk * 32 * NW, q0 = qb + wave * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1);
+  const int kh = h / a.G, qb = blk * 128, q0 = qb + wave * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1);
   const bool live = q0 < a.Sq;
-  const int last_q = min(qb + 32 * NW - 1, a.Sq - 1);
+  const int last_q = min(qb + 127, a.Sq - 1);
   int ntiles = (a.Sk + 63) / 64;
   if (a.causal) ntiles = last_q + a.off < 0 ? 0 : min(ntiles, (last_q + a.off) / 64 + 1);
-  typedef Loader<D, 64, NW> KL;
-  typedef Loader<DV, 64, NW> VL;
+  typedef Loader<D, 64, 4> KL;
+  typedef Loader<DV, 64, 4> VL;
   const KL kl(a.k + (long long)b * a.k_sb + (long long)kh * a.k_sh, a.k_ss, a.Sk - 1, wave, lane);
   const VL vl(a.v + (long long)b * a.v_sb + (long long)kh * a.v_sh, a.v_ss, a.Sk - 1, wave, lane);
   auto request = [&](int kt, int buf) {
@@ -330,11 +330,11 @@ __global__ __launch_bounds__(64 * NW, 2) void maps_fwd_kernel(const MapArgs a) {
 #pragma unroll
     for (int ks = 0; ks < NK; ks++)
       qf[m][ks] = *(const s16x8*)(a.q + (long long)b * a.q_sb + (long long)qrow * a.q_ss + (long long)h * a.q_sh + m * a.q_sm + 16 * ks + 8 * g);
-  Masks<NW> masks(a, b, ntiles, sMask, wave, lane);
+  Masks masks(a, b, ntiles, sMask, wave, lane);
   masks.load();
   int rlo, rhi;
   bias_window(a, -(last_q + a.off), ntiles * 64 - 1 - qb - a.off, rlo, rhi);
-  if constexpr (BIAS) load_bias(a, h, rlo, rhi, sB, tid, 64 * NW);
+  if constexpr (BIAS) load_bias(a, h, rlo, rhi, sB, tid, 256);
   f32x16 oacc[MAPS][ND];
   float m_run[MAPS], l_run[MAPS];
 #pragma unroll
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(64 * NW, 2) void maps_fwd_kernel(const MapArgs a) {
     bf16_t* sK = stage + buf * STAGE;
     bf16_t* sV = sK + MAPS * KT;
     if (mask != ~0ull) {
-      clear_rows<DV>(sV, mask, 64, tid, 64 * NW);
+      clear_rows<DV>(sV, mask, 64, tid, 256);
       __syncthreads();
     }
     const int key0 = t * 64;
@@ -731,13 +731,13 @@ __global__ __launch_bounds__(256) void maps_join_kernel(const MapArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// backward, queries: dq and the row sums r_i = sum_j p_ij dp_ij.  One workgroup = 32 NW queries of one head, tiles as in the forward.
+// backward, queries: dq and the row sums r_i = sum_j p_ij dp_ij.  One workgroup = 128 queries of one head, tiles as in the forward.
 // ds = p (dp - r) needs r before the first key: rowsum(dO o) gives it up to the rounding of o, which is enough for dq (16 bits), and the exact
 // fp32 sum falls out of the same registers (one FMA per element): the key kernel forms ds, the bias table's and lam's gradients from that.
 // Row statistics leave as [B][H][64-query tile][MAPS][2][64] floats: log2 of the row sum (ROW_OFF for a row without one), r.
 // ------------------------------------------------------------------------------------------------
-template <bool HALF, int D, int MAPS, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void maps_bwd_q_kernel(const MapArgs a) {
+template <bool HALF, int D, int MAPS>
+__global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
   constexpr int DV = MAPS * D, KT = 64 * D, STAGE = MAPS * KT + 64 * DV, NK = D / 16, NV = DV / 16, ND = D / 32, RA = 4;
   constexpr bool BIAS = MAPS == 1;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -745,17 +745,17 @@ __global__ __launch_bounds__(64 * NW, 2) void maps_bwd_q_kernel(const MapArgs a)
   unsigned long long* sMask = (unsigned long long*)(smem + 2 * STAGE * 2);
   float* sB = (float*)(sMask + WIN);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;
-  const int nqb = (a.Sq + 32 * NW - 1) / (32 * NW);
+  const int nqb = (a.Sq + 127) / 128;
   int blk, b, h;
   block_id(nqb, a, a.H, blk, b, h);
   if (a.causal) blk = nqb - 1 - blk;
-  const int kh = h / a.G, qb = blk * 32 * NW, q0 = qb + wave * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1);
+  const int kh = h / a.G, qb = blk * 128, q0 = qb + wave * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1);
   const bool live = q0 < a.Sq;
-  const int last_q = min(qb + 32 * NW - 1, a.Sq - 1);
+  const int last_q = min(qb + 127, a.Sq - 1);
   int ntiles = (a.Sk + 63) / 64;
   if (a.causal) ntiles = last_q + a.off < 0 ? 0 : min(ntiles, (last_q + a.off) / 64 + 1);
-  typedef Loader<D, 64, NW> KL;
-  typedef Loader<DV, 64, NW> VL;
+  typedef Loader<D, 64, 4> KL;
+  typedef Loader<DV, 64, 4> VL;
   const KL kl(a.k + (long long)b * a.k_sb + (long long)kh * a.k_sh, a.k_ss, a.Sk - 1, wave, lane);
   const VL vl(a.v + (long long)b * a.v_sb + (long long)kh * a.v_sh, a.v_ss, a.Sk - 1, wave, lane);
   auto request = [&](int kt, int buf) {
@@ -800,11 +800,11 @@ __global__ __launch_bounds__(64 * NW, 2) void maps_bwd_q_kernel(const MapArgs a)
 #pragma unroll
     for (int m = 0; m < MAPS; m++) del[m] = half_sum(del[m]);
   }
-  Masks<NW> masks(a, b, ntiles, sMask, wave, lane);
+  Masks masks(a, b, ntiles, sMask, wave, lane);
   masks.load();
   int rlo, rhi;
   bias_window(a, -(last_q + a.off), ntiles * 64 - 1 - qb - a.off, rlo, rhi);
-  if constexpr (BIAS) load_bias(a, h, rlo, rhi, sB, tid, 64 * NW);
+  if constexpr (BIAS) load_bias(a, h, rlo, rhi, sB, tid, 256);
   f32x16 acc[MAPS][ND];
 #pragma unroll
   for (int m = 0; m < MAPS; m++)
@@ -825,8 +825,8 @@ __global__ __launch_bounds__(64 * NW, 2) void maps_bwd_q_kernel(const MapArgs a)
     bf16_t* sV = sK + MAPS * KT;
     if (mask != ~0ull) {
 #pragma unroll
-      for (int m = 0; m < MAPS; m++) clear_rows<D>(sK + m * KT, mask, 64, tid, 64 * NW);
-      clear_rows<DV>(sV, mask, 64, tid, 64 * NW);
+      for (int m = 0; m < MAPS; m++) clear_rows<D>(sK + m * KT, mask, 64, tid, 256);
+      clear_rows<DV>(sV, mask, 64, tid, 256);
       __syncthreads();
     }
     const int key0 = t * 64;
@@ -1345,9 +1345,6 @@ MapArgs map_args(const uvtg_attn_dims* d) {
   return a;
 }
 
-// 8 waves to a row block share a tile's requests where the rows fill them
-bool wide_rows(const uvtg_attn_dims* d) { return d->Sq >= 512; }
-
 // entries of the bias window of a workgroup of `rows` rows
 size_t window_bytes(const uvtg_attn_dims* d, int maps, int rows, long long other) {
   if (maps == 2) return 0;
@@ -1356,16 +1353,15 @@ size_t window_bytes(const uvtg_attn_dims* d, int maps, int rows, long long other
 }
 
 // LDS of the kernels that walk key tiles: two stages (or, at the end, the waves' store slabs), masks, bias window
-template <int D, int MAPS, int NW> size_t lds_rows(const uvtg_attn_dims* d) {
-  const size_t tiles = 2 * 64 * 2 * MAPS * D * 2, slabs = NW * SLAB * 2, t = (tiles > slabs ? tiles : slabs);
-  return t + WIN * 8 + window_bytes(d, MAPS, 32 * NW, d->Sk);
+template <int D, int MAPS> size_t lds_rows(const uvtg_attn_dims* d) {
+  const size_t tiles = 2 * 64 * 2 * MAPS * D * 2, slabs = 4 * SLAB * 2;
+  return (tiles > slabs ? tiles : slabs) + WIN * 8 + window_bytes(d, MAPS, 128, d->Sk);
 }
 template <bool HALF, int D, int MAPS> int run_fwd(const uvtg_attn_dims* d, MapArgs a, hipStream_t s) {
   constexpr int DV = MAPS * D;
   const SplitPlan p = plan_split(d, MAPS);
   if (!p.use) {
-    if (wide_rows(d)) hipLaunchKernelGGL((maps_fwd_kernel<HALF, D, MAPS, 8>), dim3((unsigned)((d->Sq + 255) / 256) * d->H * d->B), dim3(512), (lds_rows<D, MAPS, 8>(d)), s, a);
-    else hipLaunchKernelGGL((maps_fwd_kernel<HALF, D, MAPS, 4>), dim3((unsigned)((d->Sq + 127) / 128) * d->H * d->B), dim3(256), (lds_rows<D, MAPS, 4>(d)), s, a);
+    hipLaunchKernelGGL((maps_fwd_kernel<HALF, D, MAPS>), dim3((unsigned)((d->Sq + 127) / 128) * d->H * d->B), dim3(256), (lds_rows<D, MAPS>(d)), s, a);
     UVTG_CHECK_LAUNCH();
     return 0;
   }
@@ -1387,8 +1383,7 @@ template <bool HALF, int D, int MAPS> int run_bwd(const uvtg_attn_dims* d, MapAr
   a.rvec = (float*)(ws + w.rvec);
   a.part = (float*)(ws + w.part);
   if (MAPS == 1) reachable(d, a.glo, a.gw);
-  if (wide_rows(d)) hipLaunchKernelGGL((maps_bwd_q_kernel<HALF, D, MAPS, 8>), dim3((unsigned)((d->Sq + 255) / 256) * d->H * d->B), dim3(512), (lds_rows<D, MAPS, 8>(d)), s, a);
-  else hipLaunchKernelGGL((maps_bwd_q_kernel<HALF, D, MAPS, 4>), dim3((unsigned)((d->Sq + 127) / 128) * d->H * d->B), dim3(256), (lds_rows<D, MAPS, 4>(d)), s, a);
+  hipLaunchKernelGGL((maps_bwd_q_kernel<HALF, D, MAPS>), dim3((unsigned)((d->Sq + 127) / 128) * d->H * d->B), dim3(256), (lds_rows<D, MAPS>(d)), s, a);
   UVTG_CHECK_LAUNCH();
   const size_t need_k = 2 * 64 * (MAPS * D + DV) * 2 + (DV == 128 ? 128 * DV * 2 : 0) + 2 * 1024 + (MAPS == 1 ? DIAG_BYTES : 0) + 32 + window_bytes(d, MAPS, 128, d->Sq);
   const size_t lds_k = need_k > SWAP_BYTES ? need_k : SWAP_BYTES;
