@@ -1435,25 +1435,35 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_short_kernel(const MapArgs a)
     }
     __syncthreads();
     if (32 * w4 < a.Sk) {
-      const int n16 = (min(RQ, a.Sq - qr) + 15) / 16;
-#pragma unroll 1
-      for (int c = 0; c < n16; c++) {
-        const bf16_t* xt = sK + (half * RQ + 16 * c) * 128;                      // waves 4 - 7: the first map's dS
-        s16x8 fb[MAPS], fa[NDV];
+      // chunks of 16 queries, the next one's fragments on their way under the MFMAs of the current one.  dv: P and dO's channels; dk: the maps' dS
+      // and q's channels of the map; the same code with other addresses
+      const int n16 = (min(RQ, a.Sq - qr) + 15) / 16, arow = half ? 32 * D : 32 * DV;                      // bytes of 16 rows
+      const unsigned a0 = opaque(half ? lds_at(sQ + qr * D) + toff0 : lds_at(sO + qr * DV) + ooff0), a1 = opaque(half ? lds_at(sQ + qr * D) + toff1 : lds_at(sO + qr * DV) + ooff1);
+      const unsigned x0 = opaque(lds_at(sK) + half * RQ * 256 + xoff0), x1 = opaque(lds_at(sK) + half * RQ * 256 + xoff1);
+      auto load = [&](int c, s16x8 (&fb)[MAPS], s16x8 (&fa)[NDV]) {
 #pragma unroll
-        for (int m = 0; m < MAPS; m++)
-          if (m == 0 || half) fb[m] = col_frag(lds_at(xt + m * RQ * 128) + xoff0, lds_at(xt + m * RQ * 128) + xoff1, w4, 0);
-        if (half) {
+        for (int m = 0; m < MAPS; m++) fb[m] = col_frag(x0 + c * 4096 + (half ? m * RQ * 256 : 0), x1 + c * 4096 + (half ? m * RQ * 256 : 0), w4, 0);
 #pragma unroll
-          for (int i = 0; i < NDV; i++) fa[i] = col_frag(lds_at(sQ + (i / ND) * KT + (qr + 16 * c) * D) + toff0, lds_at(sQ + (i / ND) * KT + (qr + 16 * c) * D) + toff1, i % ND, 0);
-#pragma unroll
-          for (int i = 0; i < NDV; i++) acc[i] = mma<HALF>(fa[i], fb[i / ND], acc[i]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < NDV; i++) fa[i] = col_frag(lds_at(sO + (qr + 16 * c) * DV) + ooff0, lds_at(sO + (qr + 16 * c) * DV) + ooff1, i, 0);
-#pragma unroll
-          for (int i = 0; i < NDV; i++) acc[i] = mma<HALF>(fa[i], fb[0], acc[i]);
+        for (int i = 0; i < NDV; i++) {
+          const int col = half ? i % ND : i, tile = half ? i / ND * KT * 2 : 0;
+          fa[i] = col_frag(a0 + c * arow, a1 + c * arow, col, tile);
         }
+      };
+      auto mul = [&](const s16x8 (&fb)[MAPS], const s16x8 (&fa)[NDV]) {
+#pragma unroll
+        for (int i = 0; i < NDV; i++) acc[i] = mma<HALF>(fa[i], fb[i / ND], acc[i]);
+      };
+      s16x8 fb0[MAPS], fa0[NDV], fb1[MAPS], fa1[NDV];
+      load(0, fb0, fa0);
+#pragma unroll 1
+      for (int c = 0; c < n16; c += 2) {
+        load(min(c + 1, n16 - 1), fb1, fa1);
+        fence();
+        mul(fb0, fa0);
+        fence();
+        load(min(c + 2, n16 - 1), fb0, fa0);
+        fence();
+        if (c + 1 < n16) mul(fb1, fa1);
       }
     }
   }
