@@ -253,12 +253,15 @@ int uvtg_sine_position(const float* vid_mask, const float* txt_mask, const float
  *   relpos  o_i = sum_j softmax_j(scale q_i.k_j + table[buckets[clamp(j - i - q_offset, -reach, reach) + reach], h]) v_j
  *   diff    o_i = sum_j (softmax_j(scale q1_i.k1_j) - lam[h] softmax_j(scale q2_i.k2_j)) v_j
  * q [B, Sq, H, (2,) D], k [B, Sk, Hkv, (2,) D], v [B, Sk, Hkv, D | 2 D] in 16 bits, addressed by the element strides below (channels
- * contiguous; every stride in use and every address a multiple of 16 bytes; 0 repeats a row).  Head h reads key head h / (H / Hkv).
+ * contiguous; every stride in use and every address a multiple of 16 bytes; 0 repeats a row; positions at most 2^26 elements apart).  Head h
+ * reads key head h / (H / Hkv).  Sq and Sk up to 2^24, |q_offset| up to 2^28.
  * o, o2, dO, dq, dk, dv are contiguous [B, S, heads, (2,) channels] of the same type; lse [B, H, (2,) Sq] fp32 is the natural logarithm of the
  * row sums.  table [n_buckets, H], lam [H], dtable and dlam are fp32; buckets [2 reach + 1] int32 (entries outside 0 .. n_buckets - 1 are
  * read as the nearest one inside).  kvalid [B, Sk] uint8, rows kvalid_sb bytes apart, 0 = the key is masked (its k / v rows may hold anything);
- * NULL = no mask.  causal: query i sees keys j <= i + q_offset.  A row that sees no key: o = 0, lse = -inf, no gradient.
+ * NULL = no mask.  causal: query i sees keys j <= i + q_offset.  A table entry of -inf, or below -2.3e38, takes its positions out of the row.
+ * A row that sees no key: o = 0, lse = -inf, no gradient.
  * Scores, statistics and sums are fp32; probabilities and score gradients are rounded to the operands' type for the products with v, k, q, dO.
+ * The backward pass forms the probabilities from lse: their relative error grows with a row's largest score, 2^-23 of it, and none exceeds 1.
  * Results are bit-reproducible (no floating-point atomics on memory, fixed orders of summation).
  * D: 32, 64, or 128 (relpos only).  ws: uvtg_attn_ws_bytes(dims, maps, backward) bytes, 16-byte aligned, no initial value, may be NULL if 0;
  * maps = 1 relpos, 2 diff.  Calls in flight at the same time need a ws each. */
@@ -268,7 +271,7 @@ typedef struct uvtg_attn_dims {
   int B, H, Hkv, D, Sq, Sk;    /* H a multiple of Hkv                                         */
   int causal, q_offset;        /* position of query 0 on the keys' axis                       */
   float scale;                 /* > 0                                                         */
-  int n_buckets, reach;        /* relpos: rows of table; 1 <= reach <= 4095                   */
+  int n_buckets, reach;        /* relpos: rows of table, 1 .. 8192; reach 1 .. 4095           */
   long long q_sb, q_ss, q_sh, q_sm, k_sb, k_ss, k_sh, k_sm, v_sb, v_ss, v_sh;   /* batch, position, head, map (diff) */
   long long kvalid_sb;
 } uvtg_attn_dims;

@@ -205,6 +205,8 @@ def _dims(**kw):
     (1, dict(B=0), -11), (1, dict(Sk=0), -11), (2, dict(Sq=-1), -11), (1, dict(dtype=2), -30), (2, dict(Hkv=3), -31), (1, dict(D=48), -5), (2, dict(D=128), -32),
     (1, dict(scale=0.0), -33), (2, dict(scale=float("inf")), -33), (1, dict(scale=float("nan")), -33), (1, dict(q_offset=1 << 30), -34), (1, dict(Sk=1 << 25), -34),
     (1, dict(q_ss=257), -35), (2, dict(k_sm=4), -35), (1, dict(v_sh=-64), -35), (1, dict(reach=0), -36), (1, dict(reach=4096), -36), (1, dict(n_buckets=0), -37),
+    (1, dict(n_buckets=8193), -37), (2, dict(q_ss=(1 << 26) + 8), -38), (1, dict(k_ss=1 << 27), -38), (2, dict(v_ss=1 << 40), -38), (1, dict(kvalid_sb=-1), -35),
+    (1, dict(H=65536, Hkv=1), -34), (2, dict(Sq=1 << 24, H=64, Hkv=64), -34), (1, dict(Sk=1 << 24, H=64, Hkv=64), -34),
     (1, dict(B=1 << 16, H=1 << 10, Hkv=1 << 10), -34), (1, {}, -20), (2, {}, -20)])
 def test_c_abi_refuses(maps, bad, code):
     """Every refusal comes back before anything is enqueued (no GPU here, null pointers)."""
@@ -269,6 +271,33 @@ def test_capture_is_refused_while_a_foreign_graph_of_a_leaf_lives():
     del kept
     attention._refuse_foreign([x], 2)
     assert not hasattr(y, "_attention_graphs")
+
+
+def test_leaves_are_copied_and_saved_as_before():
+    """What a call notes on its leaves goes through copies and files."""
+    import copy
+    import io
+
+    from univtg_amd import attention
+
+    class Twice(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return x * 2
+
+        @staticmethod
+        def backward(ctx, g):
+            return g * 2
+
+    x = torch.nn.Parameter(torch.arange(3.0))
+    alive = attention._apply(Twice, (x,), x)
+    with io.BytesIO() as f:
+        torch.save(x, f)
+        f.seek(0)
+        y = torch.load(f, weights_only=True)
+    assert torch.equal(x, y) and torch.equal(x, copy.deepcopy(x)) and y.requires_grad
+    del alive
+    attention._refuse_foreign([x, y], 5)
 
 
 def test_reference_against_differences():
@@ -391,6 +420,42 @@ def test_large_and_equal_scores(op):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("low", [-math.inf, torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("H, Hkv, Sq, Sk", [(2, 2, 70, 100), (4, 2, 150, 200), (2, 1, 1, 700)])
+@pytest.mark.parametrize("D", HEADS["relpos"])
+def test_positions_the_table_takes_out(D, H, Hkv, Sq, Sk, low):
+    """Table entries of -inf, and of the type's lowest value: some positions, all of one head's, and the outermost buckets of another."""
+    q, k, v, w, bk, do = make("relpos", torch.bfloat16, 2, H, Hkv, D, Sq, Sk, buckets=8, reach=40)
+    kv = mask("holes", 2, Sk)
+    off = Sk - Sq
+    gone = torch.zeros(w.shape, dtype=torch.bool, device="cuda")
+    gone[1::3, 0] = True                                     # (buckets behind the query and ahead of it)
+    gone[:, 1] = True
+    if H > 2:
+        gone[bk[0].item(), 2] = gone[bk[-1].item(), 2] = True
+    got = run("relpos", q, k, v, w.masked_fill(gone, low), bk, do, kvalid=kv, q_offset=off)
+    check(got, reference("relpos", q, k, v, w.masked_fill(gone, -math.inf), bk, do=do, kvalid=kv, q_offset=off))
+    assert not got["o"][:, :, 1].any() and bool((got["lse"][:, 1] == -math.inf).all()) and not got["dq"][:, :, 1].any() and not got["dw"][gone].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+@pytest.mark.parametrize("Sq, Sk", [(70, 100), (150, 200)])
+@pytest.mark.parametrize("D", HEADS["relpos"])
+def test_rows_at_a_large_negative_bias_stay_finite(D, Sq, Sk, t):
+    """Head 0 has -1e9 at every position: its statistics are tens of units coarse, its gradients must be finite all the same, head 1 exact."""
+    q, k, v, w, bk, do = make("relpos", TYPES[t], 2, 2, 2, D, Sq, Sk, buckets=8, reach=40)
+    w[:, 0] = -1e9
+    got = run("relpos", q, k, v, w, bk, do)
+    for n, x in got.items():
+        assert bool(torch.isfinite(x).all()), n
+    assert got["o"][:, :, 0].abs().max() <= v[:, :, 0].abs().max()
+    want = reference("relpos", q, k, v, w, bk, do=do)
+    head1 = lambda n, x: x[:, 1] if n in ("lse", "dw") else x[:, :, 1]
+    check({n: head1(n, x) for n, x in got.items()}, {n: tuple(head1(n, y) for y in want[n]) for n in got})
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("op", ["relpos", "diff"])
 def test_strides(op):
     """Views of a packed projection, head-major storage, a key shared over the batch, a slice of a longer cache, operands that have to be copied."""
@@ -410,6 +475,10 @@ def test_strides(op):
     assert same(run(op, *off[:3], w, bk, off[3]))
     shared = [x[:1].expand(x.shape) for x in (k, v)]
     got, ref = run(op, q, *shared, w, bk, do), run(op, q, *(x.contiguous() for x in shared), w, bk, do)
+    assert all(torch.equal(got[n], ref[n]) for n in got)
+    far = torch.empty(3 * ((1 << 26) + 8), dtype=torch.bfloat16, device="cuda").view(3, -1)[:, : q[0, 0].numel()].unflatten(1, q.shape[2:])[None]
+    far.copy_(q[:1, :3])                                     # positions more than 2^26 elements apart
+    got, ref = (run(op, x, k[:1], v[:1], w, bk, do[:1, :3]) for x in (far, q[:1, :3]))
     assert all(torch.equal(got[n], ref[n]) for n in got)
     m = mask("holes", 2, 180)
     got, ref = run(op, q, k, v, w, bk, do, kvalid=m[:, ::2]), run(op, q, k, v, w, bk, do, kvalid=m[:, ::2].contiguous().bool())
@@ -618,6 +687,7 @@ def test_refusals_name_the_argument():
         (ValueError, "buckets", lambda: ops.relpos_attention_fwd(q, k, v, w, bk[:-1])),
         (ValueError, "buckets", lambda: ops.relpos_attention_fwd(q, k, v, w, bk.long())),
         (RuntimeError, "scale", lambda: ops.relpos_attention_fwd(q, k, v, w, bk, scale=-1.0)),
+        (ValueError, "q_offset", lambda: ops.relpos_attention_fwd(q, k, v, w, bk, q_offset=1 << 32, causal=True)),
         (RuntimeError, "head_dim", lambda: ops.relpos_attention_fwd(q[..., :16], k[..., :16], v[..., :16], w, bk)),
         (RuntimeError, "H must be", lambda: ops.relpos_attention_fwd(q, k.repeat(1, 1, 2, 1)[:, :, :3], v.repeat(1, 1, 2, 1)[:, :, :3], w, bk)),
         (RuntimeError, "non-positive", lambda: ops.relpos_attention_fwd(q[:, :0], k, v, w, bk)),

@@ -10,12 +10,19 @@ Under `torch.no_grad()`, or when nothing requires a gradient, they are the forwa
 values (`q_offset` = how many came before) run the kernel that splits the keys."""
 from __future__ import annotations
 
+import itertools
+import random
 import weakref
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import ops
+
+# autograd nodes of this module that are alive, by a number; their leaves carry (number, stream) pairs, which are copied and saved with a leaf without
+# harm: numbers start at random, so that another process's mean nothing here
+_nodes = {}
+_numbers = itertools.count(random.getrandbits(62))
 
 
 class _RelposAttention(torch.autograd.Function):
@@ -55,14 +62,15 @@ def _apply(function, leaves, *args):
         _refuse_foreign(leaves, stream)
     o = function.apply(*args)
     if leaves:
-        note = (weakref.ref(o.grad_fn), stream)
+        n = next(_numbers)
+        _nodes[n] = weakref.ref(o.grad_fn, lambda _: _nodes.pop(n, None))
         for t in leaves:
-            t._attention_graphs = [n for n in getattr(t, "_attention_graphs", ()) if n[0]() is not None] + [note]
+            t._attention_graphs = [p for p in getattr(t, "_attention_graphs", ()) if p[0] in _nodes] + [(n, stream)]
     return o
 
 
 def _refuse_foreign(leaves, stream):
-    if any(ref() is not None and s != stream for t in leaves for ref, s in getattr(t, "_attention_graphs", ())):
+    if any(n in _nodes and s != stream for t in leaves for n, s in getattr(t, "_attention_graphs", ())):
         raise RuntimeError("attention: an autograd graph made outside this capture still holds a leaf of the captured call; release its outputs "
                            "before the capture, or pass the captured call leaves of its own")
 
@@ -80,8 +88,7 @@ def relpos_attention(q, k, v, table, buckets, kvalid=None, q_offset=0, causal=Fa
     if ops._elsewhere(q):
         with torch.cuda.device(q.device):
             return relpos_attention(q, k, v, table, buckets, kvalid, *opts)
-    table = table.float()
-    return _apply(_RelposAttention, (q, k, v, table), q, k, v, table, buckets, kvalid, opts)
+    return _apply(_RelposAttention, (q, k, v, table), q, k, v, table.float(), buckets, kvalid, opts)
 
 
 def diff_attention(q, k, v, lam, kvalid=None, q_offset=0, causal=False, scale=None):
@@ -92,5 +99,4 @@ def diff_attention(q, k, v, lam, kvalid=None, q_offset=0, causal=False, scale=No
     if ops._elsewhere(q):
         with torch.cuda.device(q.device):
             return diff_attention(q, k, v, lam, kvalid, *opts)
-    lam = lam.float()
-    return _apply(_DiffAttention, (q, k, v, lam), q, k, v, lam, kvalid, opts)
+    return _apply(_DiffAttention, (q, k, v, lam), q, k, v, lam.float(), kvalid, opts)

@@ -54,6 +54,9 @@ template <bool HALF> __device__ __forceinline__ bf16_t from_f(float x) {
 __device__ __forceinline__ s16x8 frag(const unsigned* p) { return __builtin_bit_cast(s16x8, (u32x4){p[0], p[1], p[2], p[3]}); }
 __device__ __forceinline__ s16x8 cat4(s16x4 a, s16x4 b) { return (s16x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}; }
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+// a probability from its log2: the statistics of a row with scores of 1e9 are tens of units coarse, and no probability may exceed 1 for that (the
+// clamp is a modifier of the exponential itself)
+__device__ __forceinline__ float prob(float x) { return __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(x), 0.f, 1.f); }
 // the other half-wave's value, without LDS
 __device__ __forceinline__ float half_sum(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
@@ -878,7 +881,7 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
           const float f = m == 0 ? 1.f : -lam;
 #pragma unroll
           for (int r = 0; r < 16; r += 2) {
-            const float p0 = ex2(fmaf(s[m][r], cc, e0)), p1 = ex2(fmaf(s[m][r + 1], cc, e0));
+            const float p0 = prob(fmaf(s[m][r], cc, e0)), p1 = prob(fmaf(s[m][r + 1], cc, e0));
             racc[m] = fmaf(p0, dp[r], racc[m]); racc[m] = fmaf(p1, dp[r + 1], racc[m]);
             pk[m][r / 2] = pack2<HALF>((m ? f * p0 : p0) * (dp[r] - del[m]), (m ? f * p1 : p1) * (dp[r + 1] - del[m]));
           }
@@ -1096,11 +1099,11 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
 #pragma unroll
               for (int u = 0; u < 2; u++) {
                 const int r = 4 * j + e + u;
-                p[u] = ex2(fmaf(s[0][r], cc, cb - L[0][e + u]));
+                p[u] = prob(fmaf(s[0][r], cc, cb - L[0][e + u]));
                 d0[u] = p[u] * (dp[r] - r_[0][e + u]);
                 if constexpr (BIAS) { far += d0[u]; ds0[r - 8 * ps] = d0[u]; }
                 if constexpr (MAPS == 2) {
-                  const float p2 = -lam * ex2(fmaf(s[MAPS - 1][r], cc, -L[MAPS - 1][e + u]));
+                  const float p2 = -lam * prob(fmaf(s[MAPS - 1][r], cc, -L[MAPS - 1][e + u]));
                   d1[u] = p2 * (dp[r] - r_[MAPS - 1][e + u]);
                   p[u] += p2;
                 }
@@ -1315,7 +1318,7 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_short_kernel(const MapArgs a)
         if (part) mask_scores(p[m][kb], mk, a.causal ? q_raw + a.off - key0 - 32 * kb : 32, g, -INFINITY);
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-          p[m][kb][r] = ex2(fmaf(p[m][kb][r], cc, -L[m]));
+          p[m][kb][r] = prob(fmaf(p[m][kb][r], cc, -L[m]));
           rs[m] = fmaf(p[m][kb][r], dp[kb][r], rs[m]);
         }
       }
@@ -1583,9 +1586,11 @@ int check_attn(const uvtg_attn_dims* d, int maps) {
   if (!(d->scale > 0.f) || !isfinite(d->scale)) return -33;
   if (d->Sq > (1 << 24) || d->Sk > (1 << 24) || d->q_offset > (1 << 28) || d->q_offset < -(1 << 28)) return -34;
   if ((long long)d->B * d->H > 65535 * 64ll || (long long)d->B * d->Hkv > 65535) return -34;
-  if ((long long)((d->Sq + 31) / 32) * d->B * d->H > 0x7fffffffll || (long long)((d->Sk + 31) / 32) * d->B * d->Hkv > 0x7fffffffll) return -34;
+  // a grid holds less than 2^32 threads: 512 for 128 rows of the key kernel
+  if ((long long)((d->Sq + 127) / 128) * d->B * d->H >= 1 << 23 || (long long)((d->Sk + 127) / 128) * d->B * d->Hkv >= 1 << 23 || d->H > 65535) return -34;
   const long long st[] = {d->q_sb, d->q_ss, d->q_sh, d->k_sb, d->k_ss, d->k_sh, d->v_sb, d->v_ss, d->v_sh, maps == 2 ? d->q_sm : 0, maps == 2 ? d->k_sm : 0};
   for (long long s : st) if (s % 8 || s < 0) return -35;
+  if (d->kvalid_sb < 0) return -35;
   if (d->q_ss > (1 << 26) || d->k_ss > (1 << 26) || d->v_ss > (1 << 26)) return -38;
   if (maps == 1) {
     if (d->reach < 1 || d->reach > MAX_REACH) return -36;

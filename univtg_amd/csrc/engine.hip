@@ -542,7 +542,7 @@ extern "C" const char* uvtg_strerror(int code) {
     case -35: return "attention: strides and addresses must be non-negative multiples of 16 bytes";
     case -38: return "attention: positions more than 2^26 elements apart";
     case -36: return "attention: reach must be 1 .. 4095";
-    case -37: return "attention: n_buckets must be 1 .. 65536";
+    case -37: return "attention: n_buckets must be 1 .. 8192";
     default: return "invalid argument";
   }
 }

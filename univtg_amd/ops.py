@@ -239,17 +239,18 @@ def relpos_buckets(num_buckets, max_distance, bidirectional=True, device="cuda")
 
 
 def _attn_operand(t):
-    """t as the kernels address it and its strides: channels contiguous, every other stride and the address a multiple of 16 bytes (else a contiguous
-    copy); the stride of an axis of one entry is never used."""
+    """t as the kernels address it and its strides: channels contiguous, every other stride and the address a multiple of 16 bytes, positions at most
+    2^26 elements apart (else a contiguous copy); the stride of an axis of one entry is never used."""
     st = t.stride()
     if st[-1] == 1 and t.data_ptr() % 16 == 0:
         if 1 in t.shape:
-            st = [s if n > 1 else 0 for n, s in zip(t.shape, st)]
+            st = [s if n > 1 else 0 for n, s in zip(t.shape[:-1], st)] + [1]
         for s in st[:-1]:
             if s % 8:
                 break
         else:
-            return t, st
+            if st[1] <= 1 << 26:
+                return t, st
     t = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
     return t, t.stride()
 
@@ -276,6 +277,8 @@ def _attn_call(name, maps, q, k, v, kvalid, q_offset, causal, scale):
         if kvalid.stride(1) != 1:
             kvalid = kvalid.contiguous()
         mask_sb = kvalid.stride(0)
+    if not -(1 << 28) <= q_offset <= 1 << 28:
+        raise ValueError(f"{name}: q_offset must lie within +-2^28, got {q_offset}")
     d = _lib.AttnDims(0, _ATTN_TYPES[dtype], B, H, Hkv, D, Sq, Sk, 1 if causal else 0, int(q_offset), D ** -0.5 if scale is None else float(scale), 0, 0,
                       qs[0], qs[1], qs[2], qs[3] if maps == 2 else 0, ks[0], ks[1], ks[2], ks[3] if maps == 2 else 0, vs[0], vs[1], vs[2], mask_sb)
     return d, q, k, v, kvalid
@@ -345,8 +348,8 @@ def _relpos_bwd(do, d, q, k, v, table, buckets, kvalid, o, lse, need_dtable):
 def relpos_attention_fwd(q, k, v, table, buckets, kvalid=None, q_offset=0, causal=False, scale=None):
     """softmax(scale q k^T + table[buckets[clamp(j - i - q_offset)], h]) v: q [B, Sq, H, D], k and v [B, Sk, Hkv, D] (bf16 or fp16, D 32 / 64 / 128,
     any strides), table [n_buckets, H] fp32, buckets int32 [2 reach + 1] (relpos_buckets), kvalid [B, Sk] uint8 / bool (0 = masked key).  causal:
-    query i sees keys up to i + q_offset.  scale defaults to D ** -0.5.  Returns o [B, Sq, H, D] and lse [B, H, Sq] (fp32); a row that sees no key
-    is 0 with lse -inf."""
+    query i sees keys up to i + q_offset.  A table entry of -inf takes its positions out of the row.  scale defaults to D ** -0.5.  Returns o
+    [B, Sq, H, D] and lse [B, H, Sq] (fp32); a row that sees no key is 0 with lse -inf."""
     if _elsewhere(q):
         with torch.cuda.device(q.device):
             return relpos_attention_fwd(q, k, v, table, buckets, kvalid, q_offset, causal, scale)
