@@ -162,7 +162,7 @@ template <int W, int ROWS, int NW> __device__ __forceinline__ void load_tile(con
 // few MFMAs instead of all of a tile's together measured 5 - 12 % slower: a request holds its wave about as long wherever it stands.)
 template <int W, int ROWS, int NW> struct Loader {
   static constexpr int RPI = 512 / W, NI = ROWS / RPI, PIECES = (NI + NW - 1) / NW, PERIOD = W == 128 ? 4 : W == 64 ? 2 : 1;
-  static_assert(NW % PERIOD == 0, "a wave's requests of a tile share one lane offset");
+  static_assert(NW == 1 || NW % PERIOD == 0, "a wave's requests of a tile share one lane offset, or differ from it by an XOR");
   const char* base;
   unsigned stride;                              // bytes (the host refuses rows further than 128 MB apart)
   int last, wave, row, chunk;
@@ -175,7 +175,7 @@ template <int W, int ROWS, int NW> struct Loader {
     for (int i = 0; i < PIECES; i++) {
       const int n = i * NW + wave, r0 = min(row0 + n * RPI, last);
       if (NI % NW == 0 || n < NI)
-        dma16(base + disp + (unsigned long long)(unsigned)r0 * stride, (unsigned)min((int)opaque(row), last - r0) * stride + chunk, lds + n * 1024);   // (opaque: not kept ready)
+        dma16(base + disp + (unsigned long long)(unsigned)r0 * stride, (unsigned)min((int)opaque(row), last - r0) * stride + (chunk ^ (16 * Tile<W>::f(NW == 1 ? i % PERIOD * RPI : 0))), lds + n * 1024);   // (opaque: not kept ready)
     }
   }
 };
@@ -488,7 +488,7 @@ __global__ __launch_bounds__(256, 2) void maps_fwd_kernel(const MapArgs a) {
 // ------------------------------------------------------------------------------------------------
 template <bool HALF, int D, int MAPS>
 __global__ __launch_bounds__(256, 2) void maps_fwd_split_kernel(const MapArgs a) {
-  constexpr int DV = MAPS * D, KT = 32 * D, STAGE = MAPS * KT + 32 * DV, NK = D / 16, ND = DV / 32;
+  constexpr int DV = MAPS * D, KT = 32 * D, STAGE = MAPS * KT + 32 * DV, NK = D / 16, ND = DV / 32, RA = DV == 2 * D && D == 64 ? 3 : 4;
   constexpr int NLK = MAPS * 32 * D / 512, NLV = 32 * DV / 512;                 // LDS-DMA instructions of a tile's k and v
   constexpr bool BIAS = MAPS == 1;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -531,13 +531,17 @@ __global__ __launch_bounds__(256, 2) void maps_fwd_split_kernel(const MapArgs a)
 
   bf16_t* sK = stage + wave * STAGE;
   bf16_t* sV = sK + MAPS * KT;
-  const int koff = Tile<D>::off(l31, 8 * g);
-  const int toff0 = Tile<DV>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), toff1 = Tile<DV>::rows8(toff0);
+  const int koff = 2 * Tile<D>::off(l31, 8 * g);                                                      // bytes
+  const int toff0 = 2 * Tile<DV>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), toff1 = 2 * Tile<DV>::rows8(toff0 / 2);
+  typedef Loader<D, 32, 1> KL;
+  typedef Loader<DV, 32, 1> VL;
+  const KL kl(kb_, a.k_ss, a.Sk - 1, 0, lane);
+  const VL vl(vb_, a.v_ss, a.Sk - 1, 0, lane);
   auto request_k = [&](int kt) {
 #pragma unroll
-    for (int m = 0; m < MAPS; m++) load_tile<D, 32, 1>(kb_ + m * a.k_sm, a.k_ss, kt * 32, a.Sk - 1, sK + m * KT, 0, lane);
+    for (int m = 0; m < MAPS; m++) kl.tile(kt * 32, lds_at(sK) + m * KT * 2, 2 * m * a.k_sm);
   };
-  auto request_v = [&](int kt) { load_tile<DV, 32, 1>(vb_, a.v_ss, kt * 32, a.Sk - 1, sV, 0, lane); };
+  auto request_v = [&](int kt) { vl.tile(kt * 32, lds_at(sV), 0); };
   const unsigned char* kv = a.kvalid ? a.kvalid + (size_t)b * a.mask_sb : nullptr;
   for (int w0 = t0; w0 < t1; w0 += 2 * WIN) {
     const int wn = min(2 * WIN, t1 - w0);
@@ -558,35 +562,34 @@ __global__ __launch_bounds__(256, 2) void maps_fwd_split_kernel(const MapArgs a)
       const unsigned mask = (unsigned)__builtin_amdgcn_readfirstlane((int)sMask[t]);
       const int key0 = (w0 + t) * 32;
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NLV) : "memory");          // k of this tile has landed (its v was requested behind it)
-      f32x16 s[MAPS];
-#pragma unroll
-      for (int m = 0; m < MAPS; m++) {
-        zero(s[m]);
-#pragma unroll
-        for (int ks = 0; ks < NK; ks++) s[m] = mma<HALF>(*(const s16x8*)(sK + m * KT + Tile<D>::cols(koff, 16 * ks)), qf[m][ks], s[m]);
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                  // the reads of k are done: its place may be written
-      if (more) {
-        request_k(w0 + tn);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NLK) : "memory");        // v of this tile
-      } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      if (mask != ~0u) { clear_rows<DV>(sV, mask, 32, lane, 64); asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
       unsigned pk[MAPS][8];
+      s16x8 fa[RA];
 #pragma unroll
-      for (int m = 0; m < MAPS; m++) {
+      for (int m = 0; m < MAPS; m++) {                     // one map's scores at a time: the accumulators of two leave no registers for both
+        f32x16 s;
+        zero(s);
+        const unsigned ka = opaque(lds_at(sK) + koff);
+        auto krow = [&](int i) { return row_frag(ka, i, m * KT * 2); };
+        fill<NK>(fa, krow);
+        fence();
+        run<NK>(fa, krow, [&](int i, s16x8 x) { s = mma<HALF>(x, qf[m][i], s); });
+        if (m == MAPS - 1) {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");              // the reads of k are done: its place may be written
+          if (more) request_k(w0 + tn);
+        }
         if constexpr (BIAS) {
           const float* bp = sB + hl * bw;
           const int rel = key0 + 4 * g - qi - a.off;
 #pragma unroll
-          for (int r = 0; r < 16; r++) s[m][r] = fmaf(s[m][r], a.c, bp[min(max(rel + (r & 3) + 8 * (r >> 2), rlo), rhi) - rlo]);
+          for (int r = 0; r < 16; r++) s[r] = fmaf(s[r], a.c, bp[min(max(rel + (r & 3) + 8 * (r >> 2), rlo), rhi) - rlo]);
         } else {
 #pragma unroll
-          for (int r = 0; r < 16; r++) s[m][r] *= a.c;
+          for (int r = 0; r < 16; r++) s[r] *= a.c;
         }
-        mask_scores(s[m], mask, a.causal ? qi + a.off - key0 : 32, g, -INFINITY);
-        float mx = s[m][0];
+        mask_scores(s, mask, a.causal ? qi + a.off - key0 : 32, g, -INFINITY);
+        float mx = s[0];
 #pragma unroll
-        for (int r = 1; r < 16; r++) mx = fmaxf(mx, s[m][r]);
+        for (int r = 1; r < 16; r++) mx = fmaxf(mx, s[r]);
         mx = half_max(mx);
         if (__builtin_amdgcn_ballot_w64(mx > m_run[m] + 8.f)) {
           const float mn = fmaxf(m_run[m], mx);
@@ -601,21 +604,24 @@ __global__ __launch_bounds__(256, 2) void maps_fwd_split_kernel(const MapArgs a)
         float rs = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
-          const float p0 = ex2(s[m][r] + e0), p1 = ex2(s[m][r + 1] + e0);
+          const float p0 = ex2(s[r] + e0), p1 = ex2(s[r + 1] + e0);
           rs += p0 + p1;
           pk[m][r / 2] = pack2<HALF>(p0, p1);
         }
         l_run[m] += rs;
+        fence();
       }
+      if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NLK) : "memory");                        // v of this tile
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (mask != ~0u) { clear_rows<DV>(sV, mask, 32, lane, 64); asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+      const unsigned va0 = opaque(lds_at(sV) + toff0), va1 = opaque(lds_at(sV) + toff1);
+      auto vcol = [&](int i) { return col_frag(va0, va1, i % ND, (i / ND) * 16 * DV * 2); };
+      fill<2 * ND>(fa, vcol);
+      fence();
+      run<2 * ND>(fa, vcol, [&](int i, s16x8 x) {
 #pragma unroll
-      for (int hf = 0; hf < 2; hf++)
-#pragma unroll
-        for (int i = 0; i < ND; i++) {
-          const int ro = 16 * hf * DV;
-          const s16x8 vt = cat4(lds_tr16(sV + Tile<DV>::cols(toff0, 32 * i) + ro), lds_tr16(sV + Tile<DV>::cols(toff1, 32 * i) + ro));
-#pragma unroll
-          for (int m = 0; m < MAPS; m++) oacc[m][i] = mma<HALF>(vt, frag(pk[m] + 4 * hf), oacc[m][i]);
-        }
+        for (int m = 0; m < MAPS; m++) oacc[m][i % ND] = mma<HALF>(x, frag(pk[m] + 4 * (i / ND)), oacc[m][i % ND]);
+      });
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       if (more) request_v(w0 + tn);
       t = tn;
@@ -1034,7 +1040,6 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
         for (int m = 0; m < MAPS; m++) zero(s[m]);
         s16x8 fa[RA], fv[VLDS ? RV : 1];
         const unsigned qa = opaque(lds_at(sQ) + qoff), oa = DV == D ? qa : opaque(lds_at(sO) + ooff);
-        const unsigned qt0 = opaque(lds_at(sQ) + tq0), qt1 = opaque(lds_at(sQ) + tq1), ot0 = DV == D ? qt0 : opaque(lds_at(sO) + to0), ot1 = DV == D ? qt1 : opaque(lds_at(sO) + to1);
         constexpr int OB = DV == D ? MAPS * QT * 2 : 0;    // (one map: dO's tile is q's, one tile further)
         auto qorow = [&](int i) { return i < NS ? row_frag(qa, i % NK, i / NK * QT * 2) : row_frag(oa, i - NS, OB); };
         const unsigned va = VLDS ? opaque(lds_at(sV) + kw * 64 * DV + ooff) : 0;
@@ -1049,6 +1054,7 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
           fence();
         }
         if (req) request(qt + 1, buf ^ 1);                 // (while the score MFMAs run)
+        const unsigned qt0 = opaque(lds_at(sQ) + tq0), qt1 = opaque(lds_at(sQ) + tq1), ot0 = DV == D ? qt0 : opaque(lds_at(sO) + to0), ot1 = DV == D ? qt1 : opaque(lds_at(sO) + to1);
         // transposed fragments, 16 queries (hf) x 32 channels: dO's NDV blocks, then q's ND blocks of each map
         auto tcol = [&](int i) {
           const int hf = i / NP, c = i % NP;
@@ -1112,6 +1118,7 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
               pd[0][2 * j + e / 2] = pack2<HALF>(d0[0], d0[1]);
               if constexpr (MAPS == 2) pd[MAPS - 1][2 * j + e / 2] = pack2<HALF>(d1[0], d1[1]);
             }
+            if constexpr (MAPS == 2) fence();              // (the next statistics would not fit beside both maps)
           }
           if constexpr (BIAS) {
             if (close) {
