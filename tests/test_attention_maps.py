@@ -385,6 +385,14 @@ def test_few_rows_over_long_keys(op, D, B, H, Hkv, Sq, Sk):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["none", "empty"])
+@pytest.mark.parametrize("op, D", OPS)
+def test_many_short_heads(op, D, kind):
+    """More heads of short rows than workgroups that stay on the chip: each takes several, of other samples."""
+    both(op, *make(op, torch.bfloat16, 75, 15, 15, D, 37, 70, seed=24), kvalid=mask(kind, 75, 70))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("op, D", OPS)
 def test_long_rows(op, D):
     """More key tiles than a workgroup holds masks for at a time (16384 keys), and training rows of a few thousand positions."""

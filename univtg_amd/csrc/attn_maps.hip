@@ -242,8 +242,8 @@ __device__ __forceinline__ void bias_window(const MapArgs& a, int lowest, int hi
 // 1-D grid -> (row block, batch, head).  Workgroups go round-robin over the 8 XCDs, each with an L2 of its own: XCD x takes a contiguous range
 // of the list, so that the blocks of a head, then the heads that share its keys, run on one XCD; batch before key head, because the samples of
 // a ragged batch differ in cost and a launch ends with its slowest XCD.
-__device__ __forceinline__ void block_id(int nblk, const MapArgs& a, int heads, int& blk, int& b, int& h) {
-  const int total = gridDim.x, qn = total / 8, r = total % 8, xcd = blockIdx.x % 8, idx = blockIdx.x / 8;
+__device__ __forceinline__ void block_id(int id, int total, int nblk, const MapArgs& a, int heads, int& blk, int& b, int& h) {
+  const int qn = total / 8, r = total % 8, xcd = id % 8, idx = id / 8;
   const int v = (xcd < r ? xcd * (qn + 1) : r * (qn + 1) + (xcd - r) * qn) + idx;
   blk = v % nblk;
   const int g = heads / a.Hkv, p = v / nblk, hi = p / g;
@@ -309,7 +309,7 @@ __global__ __launch_bounds__(256, 2) void maps_fwd_kernel(const MapArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;
   const int nqb = (a.Sq + 127) / 128;
   int blk, b, h;
-  block_id(nqb, a, a.H, blk, b, h);
+  block_id(blockIdx.x, gridDim.x, nqb, a, a.H, blk, b, h);
   if (a.causal) blk = nqb - 1 - blk;                     // the longest rows first
   const int kh = h / a.G, qb = blk * 128, q0 = qb + wave * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1);
   const bool live = q0 < a.Sq;
@@ -758,7 +758,7 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;
   const int nqb = (a.Sq + 127) / 128;
   int blk, b, h;
-  block_id(nqb, a, a.H, blk, b, h);
+  block_id(blockIdx.x, gridDim.x, nqb, a, a.H, blk, b, h);
   if (a.causal) blk = nqb - 1 - blk;
   const int kh = h / a.G, qb = blk * 128, q0 = qb + wave * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1);
   const bool live = q0 < a.Sq;
@@ -944,7 +944,7 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
   const int kw = wave & 3, qh = wave >> 2;
   const int nkb = (a.Sk + 127) / 128;
   int blk, b, kh;
-  block_id(nkb, a, a.Hkv, blk, b, kh);
+  block_id(blockIdx.x, gridDim.x, nkb, a, a.Hkv, blk, b, kh);
   const int k0 = blk * 128 + kw * 32, key = k0 + l31, krow = min(key, a.Sk - 1);
   const int first = a.causal ? max(0, (blk * 128 - a.off)) / 64 : 0, nq64 = (a.Sq + 63) / 64;          // tiles of queries that see a key
   typedef Loader<D, 64, 8> QL;
@@ -1217,11 +1217,12 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
 // over queries: waves 0 - 3 form dv, waves 4 - 7 dk, of keys 32 (w & 3) ...
 // Bound by memory: q, k, v, dO in, dq, dk, dv out.  256 x 107 positions, 8 heads of 128: 392 MB.
 // ------------------------------------------------------------------------------------------------
+template <int DV> constexpr bool SHORT_ROOM = 2 * 128 * DV * 2 >= 8 * SLAB * 2;
 template <bool HALF, int D, int MAPS>
-__global__ __launch_bounds__(512, 2) void maps_bwd_short_kernel(const MapArgs a) {
+__global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_kernel(const MapArgs a) {
   constexpr int DV = MAPS * D, KT = 128 * D, HALFSTAGE = 2 * 128 * DV, NK = D / 16, NV = DV / 16, NDV = DV / 32, ND = D / 32, RA = 4;
   constexpr int RQ = D < 128 ? D : 128, NX = 1 + MAPS;     // queries of a round; P and the maps' dS
-  constexpr bool BIAS = MAPS == 1, DIAG_IN_V = 128 * DV * 2 >= 8 * 768 * 4;
+  constexpr bool BIAS = MAPS == 1, DIAG_IN_V = 128 * DV * 2 >= 8 * 768 * 4, ROOM = SHORT_ROOM<DV>;
   static_assert(NX * RQ * 128 <= HALFSTAGE, "P and dS of a round take the place of k and v");
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   bf16_t* sK = (bf16_t*)smem;                              // [MAPS][128][D]
@@ -1231,18 +1232,25 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_short_kernel(const MapArgs a)
   float* sR = (float*)(sK + 2 * HALFSTAGE);                // [2 halves][MAPS][128] row sums
   float* sRow = sR + 2 * MAPS * 128;                       // [8 waves][256] bias gradient by position
   float* sB = sRow + (BIAS ? 8 * 256 : 0);                 // [256] bias by position
-  float* sDiag = DIAG_IN_V ? (float*)sV : sB + 256;        // [8 waves][16 keys][48], as in the key kernel
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;
-  const int w4 = wave & 3, half = wave >> 2;
-  int blk, b, h;
-  block_id(1, a, a.H, blk, b, h);
-  load_tile<DV, 128, 8>(a.v + (long long)b * a.v_sb + (long long)h * a.v_sh, a.v_ss, 0, a.Sk - 1, sV, wave, lane);
-  load_tile<DV, 128, 8>(a.dO + ((size_t)b * a.Sq * a.H + h) * DV, (long long)a.H * DV, 0, a.Sq - 1, sO, wave, lane);
+  float* extra = sB + (BIAS ? 256 : 0);
+  float* sDiag = DIAG_IN_V ? (float*)sV : extra;           // [8 waves][16 keys][48], as in the key kernel
+  bf16_t* sOut = ROOM ? sK : (bf16_t*)extra;               // exchange, then the waves' store slabs: in the place of k and v where that is large enough
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w4 = wave & 3, half = wave >> 2;
+  auto request_queries = [&](int b, int h, int lane) {
+    load_tile<DV, 128, 8>(a.dO + ((size_t)b * a.Sq * a.H + h) * DV, (long long)a.H * DV, 0, a.Sq - 1, sO, wave, lane);
 #pragma unroll
-  for (int m = 0; m < MAPS; m++) {
-    load_tile<D, 128, 8>(a.k + (long long)b * a.k_sb + (long long)h * a.k_sh + m * a.k_sm, a.k_ss, 0, a.Sk - 1, sK + m * KT, wave, lane);
-    load_tile<D, 128, 8>(a.q + (long long)b * a.q_sb + (long long)h * a.q_sh + m * a.q_sm, a.q_ss, 0, a.Sq - 1, sQ + m * KT, wave, lane);
-  }
+    for (int m = 0; m < MAPS; m++)
+      load_tile<D, 128, 8>(a.q + (long long)b * a.q_sb + (long long)h * a.q_sh + m * a.q_sm, a.q_ss, 0, a.Sq - 1, sQ + m * KT, wave, lane);
+  };
+  int blk, b, h, b_next, h_next;
+  block_id(blockIdx.x, a.B * a.H, 1, a, a.H, blk, b, h);
+  request_queries(b, h, threadIdx.x & 63);
+#pragma unroll 1
+  for (int id = blockIdx.x; id < a.B * a.H; id += gridDim.x, b = b_next, h = h_next) {
+  const int tid = opaque(threadIdx.x), lane = tid & 63, g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;     // (opaque: nothing is kept ready over the loop)
+  load_tile<DV, 128, 8>(a.v + (long long)b * a.v_sb + (long long)h * a.v_sh, a.v_ss, 0, a.Sk - 1, sV, wave, lane);
+#pragma unroll
+  for (int m = 0; m < MAPS; m++) load_tile<D, 128, 8>(a.k + (long long)b * a.k_sb + (long long)h * a.k_sh + m * a.k_sm, a.k_ss, 0, a.Sk - 1, sK + m * KT, wave, lane);
   const int q0 = w4 * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1), key0 = half * 64;
   const bool live = q0 < a.Sq;
   float L[MAPS];
@@ -1480,8 +1488,13 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_short_kernel(const MapArgs a)
   // ---- the halves of dq meet: the lower wave finishes the first HB channel blocks, the upper one the others
   constexpr int HB = (NDV + 1) / 2, HO = NDV - HB;
   __syncthreads();
-  float* ex = (float*)smem + wave * HB * 1024 + lane;
-  const float* ox = (const float*)smem + (wave ^ 4) * HB * 1024 + lane;
+  if (id + (int)gridDim.x < a.B * a.H) {                   // q and dO are read: the next head's arrive under the exchange and the stores
+    block_id(id + gridDim.x, a.B * a.H, 1, a, a.H, blk, b_next, h_next);
+    request_queries(b_next, h_next, opaque(lane));
+  }
+  float* ex = (float*)sOut + wave * HB * 1024 + lane;
+  const float* ox = (const float*)sOut + (wave ^ 4) * HB * 1024 + lane;
+  static_assert(ROOM ? 8 * HB * 4096 <= HALFSTAGE * 2 : 8 * HB * 4096 <= 8 * SLAB * 2, "the exchange fits its place");
 #pragma unroll
   for (int i = 0; i < HB; i++) {
     if (half || i < HO) {
@@ -1509,7 +1522,7 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_short_kernel(const MapArgs a)
     }
   }
   __syncthreads();
-  bf16_t* slab = sK + wave * SLAB;
+  bf16_t* slab = sOut + wave * SLAB;
   if (live) {
     auto row = [=](int c) {
       return [=](int r) -> bf16_t* { return q0 + r < a.Sq ? a.dq + (((size_t)b * a.Sq + q0 + r) * a.H + h) * DV + c : nullptr; };
@@ -1521,6 +1534,8 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_short_kernel(const MapArgs a)
     bf16_t* out = half ? a.dk : a.dv;
     store_rows<HALF, DV>(acc, half ? a.scale : 1.f, slab, lane, [=](int r) -> bf16_t* {
       return 32 * w4 + r < a.Sk ? out + (((size_t)b * a.Sk + 32 * w4 + r) * a.H + h) * DV : nullptr; });
+  }
+  __syncthreads();                                         // the slabs are read
   }
 }
 
@@ -1714,9 +1729,11 @@ template <bool HALF, int D, int MAPS> int run_bwd(const uvtg_attn_dims* d, MapAr
   a.part = (float*)(ws + w.part);
   if (MAPS == 1) reachable(d, a.glo, a.gw);
   if (short_rows(d)) {
-    const size_t slabs = 8 * SLAB * 2, tiles = 4 * 128 * DV * 2, lds = (tiles > slabs ? tiles : slabs) + 2 * MAPS * 512 + (MAPS == 1 ? 8 * 1024 + 1024 : 0) +
-                                                             (MAPS == 1 && 128 * DV * 2 < DIAG_BYTES ? DIAG_BYTES : 0);
-    hipLaunchKernelGGL((maps_bwd_short_kernel<HALF, D, MAPS>), dim3(d->H * d->B), dim3(512), lds, s, a);
+    constexpr size_t slabs = 8 * SLAB * 2, diag = MAPS == 1 && 128 * DV * 2 < DIAG_BYTES ? DIAG_BYTES : 0, extra = SHORT_ROOM<DV> ? diag : slabs > diag ? slabs : diag;
+    constexpr size_t lds = 4 * 128 * DV * 2 + 2 * MAPS * 512 + (MAPS == 1 ? 8 * 1024 + 1024 : 0) + extra;
+    // workgroups that stay: one per CU, two where registers allow
+    const int wgs = DV == 32 ? 512 : 256;
+    hipLaunchKernelGGL((maps_bwd_short_kernel<HALF, D, MAPS>), dim3(d->H * d->B < wgs ? d->H * d->B : wgs), dim3(512), lds, s, a);
     UVTG_CHECK_LAUNCH();
   } else {
     hipLaunchKernelGGL((maps_bwd_q_kernel<HALF, D, MAPS>), dim3((unsigned)((d->Sq + 127) / 128) * d->H * d->B), dim3(256), (lds_rows<D, MAPS>(d)), s, a);
