@@ -242,8 +242,8 @@ __device__ __forceinline__ void bias_window(const MapArgs& a, int lowest, int hi
 // 1-D grid -> (row block, batch, head).  Workgroups go round-robin over the 8 XCDs, each with an L2 of its own: XCD x takes a contiguous range
 // of the list, so that the blocks of a head, then the heads that share its keys, run on one XCD; batch before key head, because the samples of
 // a ragged batch differ in cost and a launch ends with its slowest XCD.
-__device__ __forceinline__ void block_id(int id, int total, int nblk, const MapArgs& a, int heads, int& blk, int& b, int& h) {
-  const int qn = total / 8, r = total % 8, xcd = id % 8, idx = id / 8;
+__device__ __forceinline__ void block_id(int nblk, const MapArgs& a, int heads, int& blk, int& b, int& h) {
+  const int total = gridDim.x, qn = total / 8, r = total % 8, xcd = blockIdx.x % 8, idx = blockIdx.x / 8;
   const int v = (xcd < r ? xcd * (qn + 1) : r * (qn + 1) + (xcd - r) * qn) + idx;
   blk = v % nblk;
   const int g = heads / a.Hkv, p = v / nblk, hi = p / g;
@@ -309,7 +309,7 @@ __global__ __launch_bounds__(256, 2) void maps_fwd_kernel(const MapArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;
   const int nqb = (a.Sq + 127) / 128;
   int blk, b, h;
-  block_id(blockIdx.x, gridDim.x, nqb, a, a.H, blk, b, h);
+  block_id(nqb, a, a.H, blk, b, h);
   if (a.causal) blk = nqb - 1 - blk;                     // the longest rows first
   const int kh = h / a.G, qb = blk * 128, q0 = qb + wave * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1);
   const bool live = q0 < a.Sq;
@@ -758,7 +758,7 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;
   const int nqb = (a.Sq + 127) / 128;
   int blk, b, h;
-  block_id(blockIdx.x, gridDim.x, nqb, a, a.H, blk, b, h);
+  block_id(nqb, a, a.H, blk, b, h);
   if (a.causal) blk = nqb - 1 - blk;
   const int kh = h / a.G, qb = blk * 128, q0 = qb + wave * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1);
   const bool live = q0 < a.Sq;
@@ -944,7 +944,7 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
   const int kw = wave & 3, qh = wave >> 2;
   const int nkb = (a.Sk + 127) / 128;
   int blk, b, kh;
-  block_id(blockIdx.x, gridDim.x, nkb, a, a.Hkv, blk, b, kh);
+  block_id(nkb, a, a.Hkv, blk, b, kh);
   const int k0 = blk * 128 + kw * 32, key = k0 + l31, krow = min(key, a.Sk - 1);
   const int first = a.causal ? max(0, (blk * 128 - a.off)) / 64 : 0, nq64 = (a.Sq + 63) / 64;          // tiles of queries that see a key
   typedef Loader<D, 64, 8> QL;
@@ -1211,46 +1211,53 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// backward of short rows (Sq, Sk <= 128, every head its own keys): one workgroup = one head of one sample, everything in LDS, every operand read once.
-// 8 waves: wave w has queries 32 (w & 3) .. and keys 64 (w >> 2) .. of the scores (lane <-> query); the two halves of a row meet in r, so that ds is
-// formed from the exact row sums without a second pass.  P and dS then go through LDS, RQ queries at a time in the place of k and v, to the products
-// over queries: waves 0 - 3 form dv, waves 4 - 7 dk, of keys 32 (w & 3) ...
-// Bound by memory: q, k, v, dO in, dq, dk, dv out.  256 x 107 positions, 8 heads of 128: 392 MB.
+// backward of short rows (Sq, Sk <= 128, every head its own keys): one workgroup = one head of one sample at a time, everything in LDS, every operand
+// read once.  8 waves: wave w has queries 32 (w & 3) .. and keys 64 (w >> 2) .. of the scores (lane <-> query); the two halves of a row meet in r, so
+// that ds is formed from the exact row sums without a second pass.  dS and then P go through LDS in 16 bits to the products, whose 32 x 32 tiles of
+// dq, dk and dv the waves share evenly.  Workgroups stay and fetch their next head under the stores.
+// Bound by memory and by the phases' latency: q, k, v, dO in, dq, dk, dv out, 392 MB for 256 x 107 positions and 8 heads of 128: 77 us at the rate of a
+// copy, 125 us measured (220 us by the two passes of longer rows).
 // ------------------------------------------------------------------------------------------------
-template <int DV> constexpr bool SHORT_ROOM = 2 * 128 * DV * 2 >= 8 * SLAB * 2;
 template <bool HALF, int D, int MAPS>
 __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_kernel(const MapArgs a) {
-  constexpr int DV = MAPS * D, KT = 128 * D, HALFSTAGE = 2 * 128 * DV, NK = D / 16, NV = DV / 16, NDV = DV / 32, ND = D / 32, RA = 4;
-  constexpr int RQ = D < 128 ? D : 128, NX = 1 + MAPS;     // queries of a round; P and the maps' dS
-  constexpr bool BIAS = MAPS == 1, DIAG_IN_V = 128 * DV * 2 >= 8 * 768 * 4, ROOM = SHORT_ROOM<DV>;
-  static_assert(NX * RQ * 128 <= HALFSTAGE, "P and dS of a round take the place of k and v");
+  constexpr int DV = MAPS * D, KT = 128 * D, VT = 128 * DV, NK = D / 16, NV = DV / 16, NC = DV / 32, ND = D / 32, RA = DV == 32 ? 2 : 4;
+  constexpr int NT = NC == 4 ? 2 : 1;                      // 32 x 32 tiles of dq, of dk and of dv per wave (DV = 32: of the first four waves)
+  constexpr bool BIAS = MAPS == 1;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  bf16_t* sK = (bf16_t*)smem;                              // [MAPS][128][D]
-  bf16_t* sV = sK + MAPS * KT;                             // [128][DV]
-  bf16_t* sQ = sK + HALFSTAGE;                             // [MAPS][128][D]
-  bf16_t* sO = sQ + MAPS * KT;                             // [128][DV]
-  float* sR = (float*)(sK + 2 * HALFSTAGE);                // [2 halves][MAPS][128] row sums
-  float* sRow = sR + 2 * MAPS * 128;                       // [8 waves][256] bias gradient by position
-  float* sB = sRow + (BIAS ? 8 * 256 : 0);                 // [256] bias by position
-  float* extra = sB + (BIAS ? 256 : 0);
-  float* sDiag = DIAG_IN_V ? (float*)sV : extra;           // [8 waves][16 keys][48], as in the key kernel
-  bf16_t* sOut = ROOM ? sK : (bf16_t*)extra;               // exchange, then the waves' store slabs: in the place of k and v where that is large enough
+  // queries of a round of dS and of P, and dS's place: 128 channels: that of v; 64: its own; 32: that of the diagonals, so that two workgroups fit a CU
+  constexpr int RS = DV == 32 || D < DV && DV == 128 ? 64 : 128, RP = DV == 32 ? 64 : 128;
+  bf16_t* sK = (bf16_t*)smem;                              // [MAPS][128][D], then (with v's place) P
+  bf16_t* sV = sK + VT;                                    // [128][DV]
+  bf16_t* sQ = sV + VT;                                    // [MAPS][128][D]
+  bf16_t* sO = sQ + VT;                                    // [128][DV]
+  float* sR = (float*)(sO + VT);                           // [2 halves][MAPS][128] row sums
+  float* sX = sR + 2 * MAPS * 128;                         // [8 waves][768]: skewed score gradients as in the key kernel, then store slabs
+  float* sRow = sX + 8 * 768;                              // [8 waves][96] bias gradient of the wave's 95 positions
+  float* sEnd = sRow + (BIAS ? 8 * 96 : 0);                // [8 waves][2] its sums at and behind -R, +R
+  float* sB = sEnd + (BIAS ? 64 : 0);                      // [256] bias by position
+  bf16_t* sS = DV == 128 ? sV : DV == 32 ? (bf16_t*)sX : (bf16_t*)(sB + (BIAS ? 256 : 0));           // [MAPS][RS][128]
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w4 = wave & 3, half = wave >> 2;
-  auto request_queries = [&](int b, int h, int lane) {
-    load_tile<DV, 128, 8>(a.dO + ((size_t)b * a.Sq * a.H + h) * DV, (long long)a.H * DV, 0, a.Sq - 1, sO, wave, lane);
+  auto request = [&](int b, int h, int lane) {
 #pragma unroll
-    for (int m = 0; m < MAPS; m++)
+    for (int m = 0; m < MAPS; m++) {
+      load_tile<D, 128, 8>(a.k + (long long)b * a.k_sb + (long long)h * a.k_sh + m * a.k_sm, a.k_ss, 0, a.Sk - 1, sK + m * KT, wave, lane);
       load_tile<D, 128, 8>(a.q + (long long)b * a.q_sb + (long long)h * a.q_sh + m * a.q_sm, a.q_ss, 0, a.Sq - 1, sQ + m * KT, wave, lane);
+    }
+    load_tile<DV, 128, 8>(a.v + (long long)b * a.v_sb + (long long)h * a.v_sh, a.v_ss, 0, a.Sk - 1, sV, wave, lane);
+    load_tile<DV, 128, 8>(a.dO + ((size_t)b * a.Sq * a.H + h) * DV, (long long)a.H * DV, 0, a.Sq - 1, sO, wave, lane);
   };
-  int blk, b, h, b_next, h_next;
-  block_id(blockIdx.x, a.B * a.H, 1, a, a.H, blk, b, h);
-  request_queries(b, h, threadIdx.x & 63);
+  const int heads = a.B * a.H;
+  auto sample = [&](int id, int& b, int& h) {              // XCD x takes a contiguous range of the (head, sample) pairs
+    const int r = heads % 8, xcd = id % 8, v = heads / 8 * xcd + min(xcd, r) + id / 8;
+    h = v / a.B;
+    b = v - h * a.B;
+  };
+  int b, h, b_next, h_next, h_last = -1;
+  sample(blockIdx.x, b, h);
+  request(b, h, threadIdx.x & 63);
 #pragma unroll 1
-  for (int id = blockIdx.x; id < a.B * a.H; id += gridDim.x, b = b_next, h = h_next) {
+  for (int id = blockIdx.x; id < heads; id += gridDim.x, b = b_next, h = h_next) {
   const int tid = opaque(threadIdx.x), lane = tid & 63, g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;     // (opaque: nothing is kept ready over the loop)
-  load_tile<DV, 128, 8>(a.v + (long long)b * a.v_sb + (long long)h * a.v_sh, a.v_ss, 0, a.Sk - 1, sV, wave, lane);
-#pragma unroll
-  for (int m = 0; m < MAPS; m++) load_tile<D, 128, 8>(a.k + (long long)b * a.k_sb + (long long)h * a.k_sh + m * a.k_sm, a.k_ss, 0, a.Sk - 1, sK + m * KT, wave, lane);
   const int q0 = w4 * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1), key0 = half * 64;
   const bool live = q0 < a.Sq;
   float L[MAPS];
@@ -1269,10 +1276,10 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
     mask[i] = __builtin_amdgcn_ballot_w64(key < a.Sk && (!kv || kv[min(key, a.Sk - 1)] != 0));
   }
   const int rlo = -(a.Sq - 1) - a.off, rhi = 127 - a.off;  // positions of the workgroup
+  float* row = sRow + wave * 96;
   if constexpr (BIAS) {
-    load_bias(a, h, rlo, rhi, sB, tid, 512);
-#pragma unroll
-    for (int i = 0; i < 4; i++) sRow[wave * 256 + i * 64 + lane] = 0.f;
+    if (h != h_last) load_bias(a, h, rlo, rhi, sB, tid, 512);
+    h_last = h;
   }
   dma_wait();
   __syncthreads();
@@ -1285,6 +1292,19 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
         clear_rows<DV>(sV + i * 64 * DV, mask[i], 64, tid, 512);
       }
     __syncthreads();
+  }
+  // One workgroup per CU, all at the same place: the memory would idle under the products.  The next head's operands come to L2 meanwhile, a lane
+  // touching a line of 128 bytes (144 -> 126 us for 256 x 107, 8 heads of 128; two workgroups per CU overlap by themselves, 106 us against 108).
+  const bool more = id + (int)gridDim.x < heads;
+  sample(more ? id + gridDim.x : id, b_next, h_next);
+  int touched[2] = {0, 0};
+  if constexpr (DV > 32) {
+    constexpr int LK = MAPS * (D > 64 ? D / 64 : 1), LV = DV / 64;
+    const int t = tid & 255, S = (half ? a.Sq : a.Sk) - 1, lk = t % LK, lv = t % LV;
+    const bf16_t* x = half ? a.q + (long long)b_next * a.q_sb + (long long)h_next * a.q_sh : a.k + (long long)b_next * a.k_sb + (long long)h_next * a.k_sh;
+    const bf16_t* y = half ? a.dO + ((size_t)b_next * a.Sq * a.H + h_next) * DV : a.v + (long long)b_next * a.v_sb + (long long)h_next * a.v_sh;
+    touched[0] = *(const int*)(x + (long long)min(t / LK, S) * (half ? a.q_ss : a.k_ss) + (MAPS == 2 ? lk * (half ? a.q_sm : a.k_sm) : lk * 64));
+    touched[1] = *(const int*)(y + (long long)min(t / LV, S) * (half ? (long long)a.H * DV : a.v_ss) + lv * 64);
   }
   const int koff = 2 * Tile<D>::off(l31, 8 * g), voff = 2 * Tile<DV>::off(l31, 8 * g);                // bytes
   const int toff0 = 2 * Tile<D>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), toff1 = 2 * Tile<D>::rows8(toff0 / 2);
@@ -1353,10 +1373,12 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
   }
   // ---- P and dS, packed as operands
   unsigned pp[2][8], pd[MAPS][2][8];
-  float* diag = sDiag + wave * 768;
+  float* diag = sX + wave * 768;
   if constexpr (BIAS) {
 #pragma unroll
     for (int i = 0; i < 12; i++) diag[i * 64 + lane] = 0.f;
+    row[lane] = 0.f;
+    if (lane < 32) row[64 + lane] = 0.f;
   }
   float fl = 0.f, fr = 0.f;
 #pragma unroll
@@ -1375,9 +1397,9 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
         }
         if constexpr (BIAS) dp[kb][r + u] = d[0][u];
       }
-      pp[kb][r / 2] = pack2<HALF>(x[0], x[1]);
+      pp[kb][r / 2] = opaque(pack2<HALF>(x[0], x[1]));     // (opaque: formed here, by all waves at once, not in the rounds below)
 #pragma unroll
-      for (int m = 0; m < MAPS; m++) pd[m][kb][r / 2] = pack2<HALF>(d[m][0], d[m][1]);
+      for (int m = 0; m < MAPS; m++) pd[m][kb][r / 2] = opaque(pack2<HALF>(d[m][0], d[m][1]));
     }
     if constexpr (BIAS) {
       if (on[kb]) {
@@ -1401,7 +1423,7 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
         if (lane < 63) {
           if (rel >= a.R) fr += v;
           else if (rel <= -a.R) fl += v;
-          else if (rel >= a.glo && rel < a.glo + a.gw) sRow[wave * 256 + rel - a.glo] += v;
+          else row[32 * kb + lane] += v;
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -1410,132 +1432,126 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
   }
   if constexpr (BIAS) {
     fl = wave_sum_dpp(fl); fr = wave_sum_dpp(fr);
-    if (lane == 0) {
-      if (-a.R >= a.glo && -a.R < a.glo + a.gw) sRow[wave * 256 - a.R - a.glo] = fl;
-      if (a.R >= a.glo && a.R < a.glo + a.gw) sRow[wave * 256 + a.R - a.glo] = fr;
-    }
+    if (lane == 0) { sEnd[wave * 2] = fl; sEnd[wave * 2 + 1] = fr; }
   }
-  // ---- dq of this half's keys
-  f32x16 dq[NDV];
+  // tiles of the wave: queries 32 qb, channels 32 qc of dq; keys 32 kb .. 32 + channels 32 kc .. of dk and dv
+  auto qb = [&](int j) { return MAPS == 2 && NT == 2 ? 2 * j + half : NC == 1 ? wave : wave >> 1; };
+  auto qc = [&](int j) { return MAPS == 2 && NT == 2 ? w4 : NC == 1 ? 0 : NT * (wave & 1) + j; };
+  const int kblk = NC == 1 ? wave : wave >> 1, kc = NC == 1 ? 0 : NT * (wave & 1);
+  const bool keys = 32 * kblk < a.Sk && kblk < 4;
+  f32x16 dq[NT], dk[NT], dv[NT];
 #pragma unroll
-  for (int i = 0; i < NDV; i++) zero(dq[i]);
+  for (int j = 0; j < NT; j++) { zero(dq[j]); zero(dk[j]); zero(dv[j]); }
+  // products over `n` queries: the left operand's channels `c`, the right one's keys, both transposed; chunks of 16, the next one's fragments on their
+  // way under the MFMAs of the current one
+  auto products = [&](f32x16 (&acc)[NT], unsigned l0, unsigned l1, int lrow, int c, unsigned r0, unsigned r1, int n) {
+    const int n16 = (n + 15) / 16;
+    auto load = [&](int i, s16x8& fb, s16x8 (&fa)[NT]) {
+      fb = col_frag(r0 + i * 4096, r1 + i * 4096, kblk, 0);
 #pragma unroll
-  for (int kb = 0; kb < 2; kb++) {
-    if (!on[kb]) continue;
-    const unsigned ta0 = opaque(lds_at(sK + (key0 + 32 * kb) * D) + toff0), ta1 = opaque(lds_at(sK + (key0 + 32 * kb) * D) + toff1);
-    auto kcol = [&](int i) { return col_frag(ta0, ta1, i % ND, (i / (2 * ND) * KT + i / ND % 2 * 16 * D) * 2); };
-    s16x8 fa[RA];
-    fill<2 * MAPS * ND>(fa, kcol);
-    fence();
-    run<2 * MAPS * ND>(fa, kcol, [&](int i, s16x8 x) {
-      const int m = i / (2 * ND);
-      dq[m * ND + i % ND] = mma<HALF>(x, frag(pd[m][kb] + 4 * (i / ND % 2)), dq[m * ND + i % ND]);
-    });
-  }
-  // ---- dv (waves 0 - 3) and dk (waves 4 - 7) of 32 keys
-  f32x16 acc[NDV];
+      for (int j = 0; j < NT; j++) fa[j] = col_frag(l0 + i * lrow, l1 + i * lrow, c + j, 0);
+    };
+    auto mul = [&](const s16x8& fb, const s16x8 (&fa)[NT]) {
 #pragma unroll
-  for (int i = 0; i < NDV; i++) zero(acc[i]);
+      for (int j = 0; j < NT; j++) acc[j] = mma<HALF>(fa[j], fb, acc[j]);
+    };
+    s16x8 fb0, fb1, fa0[NT], fa1[NT];
+    load(0, fb0, fa0);
 #pragma unroll 1
-  for (int qr = 0; qr < a.Sq; qr += RQ) {
-    __syncthreads();                                       // k, v and the diagonals (or the last round's P and dS) are read
-    if (live && q0 >= qr && q0 < qr + RQ) {
-      const int row = q0 - qr + l31;
+    for (int i = 0; i < n16; i += 2) {
+      load(min(i + 1, n16 - 1), fb1, fa1);
+      fence();
+      mul(fb0, fa0);
+      fence();
+      load(min(i + 2, n16 - 1), fb0, fa0);
+      fence();
+      if (i + 1 < n16) mul(fb1, fa1);
+    }
+  };
+  auto put = [&](bf16_t* tile, const unsigned (&x)[2][8], int row) {
 #pragma unroll
-      for (int x = 0; x < NX; x++)
+    for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-        for (int kb = 0; kb < 2; kb++)
+      for (int j = 0; j < 4; j++) *(u32x2*)(tile + Tile<128>::off(row, key0 + 32 * kb + 8 * j + 4 * g)) = (u32x2){x[kb][2 * j], x[kb][2 * j + 1]};
+  };
+  // ---- dq and dk: dS of RS queries at a time
+#pragma unroll 1
+  for (int qr = 0; qr < a.Sq; qr += RS) {
+    if (qr || DV == 32) __syncthreads();                   // the last round's dS, or the diagonals, are read (v: all waves have met in the row sums since)
+    if (live && q0 >= qr && q0 < qr + RS) {
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const unsigned* s = (x ? pd[x - 1][kb] : pp[kb]) + 2 * j;
-            *(u32x2*)(sK + x * RQ * 128 + Tile<128>::off(row, key0 + 32 * kb + 8 * j + 4 * g)) = (u32x2){s[0], s[1]};
-          }
+      for (int m = 0; m < MAPS; m++) put(sS + m * RS * 128, pd[m], q0 - qr + l31);
     }
     __syncthreads();
-    if (32 * w4 < a.Sk) {
-      // chunks of 16 queries, the next one's fragments on their way under the MFMAs of the current one.  dv: P and dO's channels; dk: the maps' dS
-      // and q's channels of the map; the same code with other addresses
-      const int n16 = (min(RQ, a.Sq - qr) + 15) / 16, arow = half ? 32 * D : 32 * DV;                      // bytes of 16 rows
-      const unsigned a0 = opaque(half ? lds_at(sQ + qr * D) + toff0 : lds_at(sO + qr * DV) + ooff0), a1 = opaque(half ? lds_at(sQ + qr * D) + toff1 : lds_at(sO + qr * DV) + ooff1);
-      const unsigned x0 = opaque(lds_at(sK) + half * RQ * 256 + xoff0), x1 = opaque(lds_at(sK) + half * RQ * 256 + xoff1);
-      auto load = [&](int c, s16x8 (&fb)[MAPS], s16x8 (&fa)[NDV]) {
 #pragma unroll
-        for (int m = 0; m < MAPS; m++) fb[m] = col_frag(x0 + c * 4096 + (half ? m * RQ * 256 : 0), x1 + c * 4096 + (half ? m * RQ * 256 : 0), w4, 0);
+    for (int j = 0; j < NT; j++) {
+      if (32 * qb(j) < qr || 32 * qb(j) >= min(qr + RS, a.Sq)) continue;
+      const int m = qc(j) / ND;
+      const unsigned ra = opaque(lds_at(sS) + m * RS * 256 + (32 * qb(j) - qr) * 256 + 2 * Tile<128>::off(l31, 4 * g));
+      const unsigned ta0 = opaque(lds_at(sK) + m * KT * 2 + toff0), ta1 = opaque(lds_at(sK) + m * KT * 2 + toff1);
+      const int c = qc(j) % ND;
+      // 16 keys a step, in the order in which a transposing read of k delivers them
+      auto kcol = [&](int i) { return col_frag(ta0, ta1, c, i * 32 * D); };
+      typedef const __attribute__((address_space(3))) s16x4* rptr;
+      auto dsrow = [&](int i) { return cat4(*(rptr)(uintptr_t)(ra ^ (32 * i)), *(rptr)(uintptr_t)(ra ^ (32 * i) ^ 16)); };
+      s16x8 fa[RA], fb[RA];
+      fill<8>(fa, kcol);
+      fill<8>(fb, dsrow);
+      fence();
 #pragma unroll
-        for (int i = 0; i < NDV; i++) {
-          const int col = half ? i % ND : i, tile = half ? i / ND * KT * 2 : 0;
-          fa[i] = col_frag(a0 + c * arow, a1 + c * arow, col, tile);
-        }
-      };
-      auto mul = [&](const s16x8 (&fb)[MAPS], const s16x8 (&fa)[NDV]) {
-#pragma unroll
-        for (int i = 0; i < NDV; i++) acc[i] = mma<HALF>(fa[i], fb[i / ND], acc[i]);
-      };
-      s16x8 fb0[MAPS], fa0[NDV], fb1[MAPS], fa1[NDV];
-      load(0, fb0, fa0);
-#pragma unroll 1
-      for (int c = 0; c < n16; c += 2) {
-        load(min(c + 1, n16 - 1), fb1, fa1);
+      for (int i = 0; i < 8; i++) {
+        dq[j] = mma<HALF>(fa[i % RA], fb[i % RA], dq[j]);
+        if (i + RA < 8) { fa[i % RA] = kcol(i + RA); fb[i % RA] = dsrow(i + RA); }
         fence();
-        mul(fb0, fa0);
-        fence();
-        load(min(c + 2, n16 - 1), fb0, fa0);
-        fence();
-        if (c + 1 < n16) mul(fb1, fa1);
       }
     }
-  }
-  // ---- the halves of dq meet: the lower wave finishes the first HB channel blocks, the upper one the others
-  constexpr int HB = (NDV + 1) / 2, HO = NDV - HB;
-  __syncthreads();
-  if (id + (int)gridDim.x < a.B * a.H) {                   // q and dO are read: the next head's arrive under the exchange and the stores
-    block_id(id + gridDim.x, a.B * a.H, 1, a, a.H, blk, b_next, h_next);
-    request_queries(b_next, h_next, opaque(lane));
-  }
-  float* ex = (float*)sOut + wave * HB * 1024 + lane;
-  const float* ox = (const float*)sOut + (wave ^ 4) * HB * 1024 + lane;
-  static_assert(ROOM ? 8 * HB * 4096 <= HALFSTAGE * 2 : 8 * HB * 4096 <= 8 * SLAB * 2, "the exchange fits its place");
-#pragma unroll
-  for (int i = 0; i < HB; i++) {
-    if (half || i < HO) {
-#pragma unroll
-      for (int r = 0; r < 16; r++) ex[i * 1024 + r * 64] = half ? dq[i][r] : dq[i < HO ? HB + i : 0][r];
+    if (keys) {
+      const int m = kc / ND;
+      const unsigned qa = lds_at(sQ) + m * KT * 2 + qr * D * 2;
+      products(dk, opaque(qa + toff0), opaque(qa + toff1), 32 * D, kc % ND, opaque(lds_at(sS) + xoff0 + m * RS * 256), opaque(lds_at(sS) + xoff1 + m * RS * 256), min(RS, a.Sq - qr));
     }
   }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < HB; i++) {
-    if (!half) {
-#pragma unroll
-      for (int r = 0; r < 16; r++) dq[i][r] += ox[i * 1024 + r * 64];
-    } else if (i < HO) {
-#pragma unroll
-      for (int r = 0; r < 16; r++) dq[i][r] = dq[i < HO ? HB + i : 0][r] + ox[i * 1024 + r * 64];
+  // ---- dv: P of RP queries at a time
+#pragma unroll 1
+  for (int qr = 0; qr < a.Sq; qr += RP) {
+    __syncthreads();                                       // k, or the last round's P, is read
+    if (live && q0 >= qr && q0 < qr + RP) put(sK, pp, q0 - qr + l31);
+    __syncthreads();
+    if (keys) {
+      const unsigned oa = lds_at(sO) + qr * DV * 2;
+      products(dv, opaque(oa + ooff0), opaque(oa + ooff1), 32 * DV, kc, opaque(lds_at(sK) + xoff0), opaque(lds_at(sK) + xoff1), min(RP, a.Sq - qr));
     }
   }
-  if constexpr (BIAS) {                                    // the waves' sums by position, in wave order (their last writes are two barriers old)
-    if (tid < a.gw) {
+  __syncthreads();                                         // every tile is read: the next head's arrive under the stores
+  asm volatile("" ::"v"(touched[0]), "v"(touched[1]));
+  if (more) request(b_next, h_next, opaque(lane));
+  if constexpr (BIAS) {
+    if (tid < a.gw) {                                      // bias gradient: the waves' sums by position, in wave order
+      const int rel = a.glo + tid;
+      const int far = rel == a.R ? 1 : rel == -a.R ? 0 : -1;
       float x = 0.f;
 #pragma unroll
-      for (int w = 0; w < 8; w++) x += sRow[w * 256 + tid];
+      for (int w = 0; w < 8; w++) {                        // (column 95 of a wave's positions stays 0)
+        const int at = rel - (64 * (w >> 2) - 32 * (w & 3) - a.off - 31);
+        x += far >= 0 ? sEnd[w * 2 + far] : sRow[w * 96 + ((unsigned)at < 95u ? at : 95)];
+      }
       a.part[((size_t)h * a.B + b) * a.gw + tid] = x;
     }
   }
-  __syncthreads();
-  bf16_t* slab = sOut + wave * SLAB;
-  if (live) {
-    auto row = [=](int c) {
-      return [=](int r) -> bf16_t* { return q0 + r < a.Sq ? a.dq + (((size_t)b * a.Sq + q0 + r) * a.H + h) * DV + c : nullptr; };
-    };
-    if (!half) store_rows<HALF, 32 * HB>(dq, a.scale, slab, lane, row(0));
-    else if constexpr (HO > 0) store_rows<HALF, 32 * (HO > 0 ? HO : 1)>(dq, a.scale, slab, lane, row(32 * HB));
+  bf16_t* slab = (bf16_t*)(sX + wave * 768);
+#pragma unroll
+  for (int j = 0; j < NT; j++) {
+    if (32 * qb(j) < a.Sq)
+      store_rows<HALF, 32>(&dq[j], a.scale, slab, lane, [=](int r) -> bf16_t* {
+        return 32 * qb(j) + r < a.Sq ? a.dq + (((size_t)b * a.Sq + 32 * qb(j) + r) * a.H + h) * DV + 32 * qc(j) : nullptr; });
+    if (keys) {
+      auto rows = [=](bf16_t* base) {
+        return [=](int r) -> bf16_t* { return 32 * kblk + r < a.Sk ? base + (((size_t)b * a.Sk + 32 * kblk + r) * a.H + h) * DV + 32 * (kc + j) : nullptr; };
+      };
+      store_rows<HALF, 32>(&dk[j], a.scale, slab, lane, rows(a.dk));
+      store_rows<HALF, 32>(&dv[j], 1.f, slab, lane, rows(a.dv));
+    }
   }
-  if (32 * w4 < a.Sk) {
-    bf16_t* out = half ? a.dk : a.dv;
-    store_rows<HALF, DV>(acc, half ? a.scale : 1.f, slab, lane, [=](int r) -> bf16_t* {
-      return 32 * w4 + r < a.Sk ? out + (((size_t)b * a.Sk + 32 * w4 + r) * a.H + h) * DV : nullptr; });
-  }
-  __syncthreads();                                         // the slabs are read
   }
 }
 
@@ -1652,7 +1668,7 @@ void reachable(const uvtg_attn_dims* d, int& glo, int& gw) {
   gw = cl((long long)d->Sk - 1 - d->q_offset) - glo + 1;
 }
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
-// whole rows in one workgroup: one pass over the operands (256 x 107, 8 heads of 128: 145 us against 221 us of the two passes)
+// whole rows in one workgroup: one pass over the operands (256 x 107, 8 heads of 128: 125 us against 221 us of the two passes)
 bool short_rows(const uvtg_attn_dims* d) { return d->Sq <= 128 && d->Sk <= 128 && d->H == d->Hkv; }
 struct BwdWs { size_t rvec, part, sums, total; long long rows; int chunk, chunks; };
 BwdWs bwd_ws(const uvtg_attn_dims* d, int maps) {
@@ -1729,8 +1745,7 @@ template <bool HALF, int D, int MAPS> int run_bwd(const uvtg_attn_dims* d, MapAr
   a.part = (float*)(ws + w.part);
   if (MAPS == 1) reachable(d, a.glo, a.gw);
   if (short_rows(d)) {
-    constexpr size_t slabs = 8 * SLAB * 2, diag = MAPS == 1 && 128 * DV * 2 < DIAG_BYTES ? DIAG_BYTES : 0, extra = SHORT_ROOM<DV> ? diag : slabs > diag ? slabs : diag;
-    constexpr size_t lds = 4 * 128 * DV * 2 + 2 * MAPS * 512 + (MAPS == 1 ? 8 * 1024 + 1024 : 0) + extra;
+    constexpr size_t lds = 4 * 128 * DV * 2 + 2 * MAPS * 512 + DIAG_BYTES + (MAPS == 1 ? 8 * 96 * 4 + 256 + 1024 : 0) + (DV == 64 ? MAPS * 128 * 256 : 0);
     // workgroups that stay: one per CU, two where registers allow
     const int wgs = DV == 32 ? 512 : 256;
     hipLaunchKernelGGL((maps_bwd_short_kernel<HALF, D, MAPS>), dim3(d->H * d->B < wgs ? d->H * d->B : wgs), dim3(512), lds, s, a);
