@@ -258,18 +258,18 @@ def test_capture_is_refused_while_a_foreign_graph_of_a_leaf_lives():
 
     x, y = torch.zeros(3, requires_grad=True), torch.zeros(3)
     alive = attention._apply(Twice, (x, y), x, y)            # noted on x for stream 0
-    attention._refuse_foreign([x], 0)
+    attention._check_capture([x], 0)
     with pytest.raises(RuntimeError, match="still holds a leaf"):
-        attention._refuse_foreign([x], 2)
+        attention._check_capture([x], 2)
     kept = alive * 3                                         # the graph lives on behind a result
     for _ in range(3):
         attention._apply(Twice, (x, y), x, y)
     assert len(x._attention_graphs) == 2                     # the graphs that died are forgotten
     del alive
     with pytest.raises(RuntimeError, match="still holds a leaf"):
-        attention._refuse_foreign([x], 2)
+        attention._check_capture([x], 2)
     del kept
-    attention._refuse_foreign([x], 2)
+    attention._check_capture([x], 2)
     assert not hasattr(y, "_attention_graphs")
 
 
@@ -297,7 +297,7 @@ def test_leaves_are_copied_and_saved_as_before():
         y = torch.load(f, weights_only=True)
     assert torch.equal(x, y) and torch.equal(x, copy.deepcopy(x)) and y.requires_grad
     del alive
-    attention._refuse_foreign([x, y], 5)
+    attention._check_capture([x, y], 5)
 
 
 def test_reference_against_differences():
@@ -663,7 +663,7 @@ def test_captured_training_step():
     for x in (own, leaves):
         if x is leaves:
             with pytest.raises(RuntimeError, match="still holds a leaf"):
-                attention._refuse_foreign(leaves, torch.cuda.Stream().cuda_stream)
+                attention._check_capture(leaves, torch.cuda.Stream().cuda_stream)
             refused += 1
             assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(alive, leaves, do), want))
             del alive                                        # the last eager graph of these leaves: now they may be captured

@@ -59,7 +59,7 @@ def _apply(function, leaves, *args):
     stream = ops._stream_of(leaves[0]) if on_gpu else 0
     leaves = [t for t in leaves if t.requires_grad and t.is_leaf]
     if on_gpu and leaves and torch.cuda.is_current_stream_capturing():
-        _refuse_foreign(leaves, stream)
+        _check_capture(leaves, stream)
     o = function.apply(*args)
     if leaves:
         n = next(_numbers)
@@ -69,7 +69,7 @@ def _apply(function, leaves, *args):
     return o
 
 
-def _refuse_foreign(leaves, stream):
+def _check_capture(leaves, stream):
     if any(n in _nodes and s != stream for t in leaves for n, s in getattr(t, "_attention_graphs", ())):
         raise RuntimeError("attention: an autograd graph made outside this capture still holds a leaf of the captured call; release its outputs "
                            "before the capture, or pass the captured call leaves of its own")
