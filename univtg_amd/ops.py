@@ -243,14 +243,11 @@ def _attn_operand(t):
     2^26 elements apart (else a contiguous copy); the stride of an axis of one entry is never used."""
     st = t.stride()
     if st[-1] == 1 and t.data_ptr() % 16 == 0:
-        if 1 in t.shape:
-            st = [s if n > 1 else 0 for n, s in zip(t.shape[:-1], st)] + [1]
-        for s in st[:-1]:
-            if s % 8:
-                break
-        else:
-            if st[1] <= 1 << 26:
-                return t, st
+        if (st[0] | st[1] | st[2] | (st[3] if len(st) == 5 else 0)) & 7 == 0 and st[1] <= 1 << 26:
+            return t, st
+        st = [s if n > 1 else 0 for n, s in zip(t.shape[:-1], st)]
+        if all(s % 8 == 0 for s in st) and st[1] <= 1 << 26:
+            return t, st
     t = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
     return t, t.stride()
 
@@ -284,9 +281,9 @@ def _attn_call(name, maps, q, k, v, kvalid, q_offset, causal, scale):
     return d, q, k, v, kvalid
 
 
-def _attn_ws(lib, d, maps, backward, device):
+def _attn_ws(lib, d, maps, backward, like):
     n = lib.uvtg_attn_ws_bytes(d, maps, backward)
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    return like.new_empty(n, dtype=torch.uint8) if n else None
 
 
 def _elsewhere(t):
@@ -324,10 +321,9 @@ def _relpos_fwd(q, k, v, table, buckets, kvalid, q_offset, causal, scale):
     lib = _lib.load()
     d, q, k, v, kvalid = _attn_call("relpos_attention", 1, q, k, v, kvalid, q_offset, causal, scale)
     table, buckets = _relpos_operands(d, q, table, buckets)
-    dev = q.device
-    o = torch.empty((d.B, d.Sq, d.H, d.D), dtype=q.dtype, device=dev)
-    lse = torch.empty((d.B, d.H, d.Sq), dtype=torch.float32, device=dev)
-    ws = _attn_ws(lib, d, 1, 0, dev)
+    o = q.new_empty((d.B, d.Sq, d.H, d.D))
+    lse = q.new_empty((d.B, d.H, d.Sq), dtype=torch.float32)
+    ws = _attn_ws(lib, d, 1, 0, q)
     _lib.check(lib.uvtg_relpos_attention_fwd(d, _at(q), _at(k), _at(v), _at(table), _at(buckets), _at(kvalid), _at(o), _at(lse), _at(ws), _stream_of(q)),
                "uvtg_relpos_attention_fwd")
     return o, lse, (d, q, k, v, table, buckets, kvalid)
@@ -336,10 +332,9 @@ def _relpos_fwd(q, k, v, table, buckets, kvalid, q_offset, causal, scale):
 def _relpos_bwd(do, d, q, k, v, table, buckets, kvalid, o, lse, need_dtable):
     lib = _lib.load()
     do = _attn_saved("relpos_attention_bwd", do, q, "do")
-    dev, t = q.device, q.dtype
-    dq, dk, dv = torch.empty(q.shape, dtype=t, device=dev), torch.empty(k.shape, dtype=t, device=dev), torch.empty(v.shape, dtype=t, device=dev)
-    dtable = torch.empty(table.shape, dtype=torch.float32, device=dev) if need_dtable else None
-    ws = _attn_ws(lib, d, 1, 1, dev)
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    dtable = table.new_empty(table.shape) if need_dtable else None
+    ws = _attn_ws(lib, d, 1, 1, q)
     _lib.check(lib.uvtg_relpos_attention_bwd(d, _at(q), _at(k), _at(v), _at(table), _at(buckets), _at(kvalid), _at(o), _at(lse), _at(do), _at(dq), _at(dk),
                                              _at(dv), _at(dtable), _at(ws), _stream_of(q)), "uvtg_relpos_attention_bwd")
     return dq, dk, dv, dtable
@@ -378,11 +373,10 @@ def _diff_fwd(q, k, v, lam, kvalid, q_offset, causal, scale, need_o2):
     lib = _lib.load()
     d, q, k, v, kvalid = _attn_call("diff_attention", 2, q, k, v, kvalid, q_offset, causal, scale)
     lam = _lam_operand(d, q, lam)
-    dev = q.device
-    o = torch.empty((d.B, d.Sq, d.H, 2 * d.D), dtype=q.dtype, device=dev)
+    o = q.new_empty((d.B, d.Sq, d.H, 2 * d.D))
     o2 = torch.empty_like(o) if need_o2 else None
-    lse = torch.empty((d.B, d.H, 2, d.Sq), dtype=torch.float32, device=dev)
-    ws = _attn_ws(lib, d, 2, 0, dev)
+    lse = q.new_empty((d.B, d.H, 2, d.Sq), dtype=torch.float32)
+    ws = _attn_ws(lib, d, 2, 0, q)
     _lib.check(lib.uvtg_diff_attention_fwd(d, _at(q), _at(k), _at(v), _at(lam), _at(kvalid), _at(o), _at(o2), _at(lse), _at(ws), _stream_of(q)),
                "uvtg_diff_attention_fwd")
     return o, lse, o2, (d, q, k, v, lam, kvalid)
@@ -391,10 +385,9 @@ def _diff_fwd(q, k, v, lam, kvalid, q_offset, causal, scale, need_o2):
 def _diff_bwd(do, d, q, k, v, lam, kvalid, o, o2, lse, need_dlam):
     lib = _lib.load()
     do = _attn_saved("diff_attention_bwd", do, q, "do")
-    dev, t = q.device, q.dtype
-    dq, dk, dv = torch.empty(q.shape, dtype=t, device=dev), torch.empty(k.shape, dtype=t, device=dev), torch.empty(v.shape, dtype=t, device=dev)
-    dlam = torch.empty(d.H, dtype=torch.float32, device=dev) if need_dlam else None
-    ws = _attn_ws(lib, d, 2, 1, dev)
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    dlam = lam.new_empty(d.H) if need_dlam else None
+    ws = _attn_ws(lib, d, 2, 1, q)
     _lib.check(lib.uvtg_diff_attention_bwd(d, _at(q), _at(k), _at(v), _at(lam), _at(kvalid), _at(o), _at(o2), _at(lse), _at(do), _at(dq), _at(dk), _at(dv),
                                            _at(dlam), _at(ws), _stream_of(q)), "uvtg_diff_attention_bwd")
     return dq, dk, dv, dlam
