@@ -297,6 +297,11 @@ __device__ __forceinline__ void mask_scores(f32x16& s, unsigned mask32, int lim,
 // ------------------------------------------------------------------------------------------------
 // forward: one workgroup = 128 queries of one head, a wave of 32 each, 64-key tiles in two LDS stages.  The first two tiles are requested before
 // anything else is known; from then on the requests of the next tile go out between the MFMAs of the current one.
+//   one pass over the keys: m the running maximum of a row's scores, l = sum exp(x - m), o = sum exp(x - m) v, both times exp(m - m') when m rises
+// Bound by the matrix and the vector pipe by turns: a 64-key tile costs a wave 32 MFMAs of 32 cycles (128 channels) and about as many cycles of vector
+// work, half of it exponentials, and two waves per SIMD (registers) overlap the two in part.  MFMA 35 % and vector 43 % of the busy cycles at 128 channels,
+// 40 % and 71 % with three waves at 64.  Measured: 32 x 1232 (half of the keys valid), 8 heads of 128: 220 us, 680 TF/s; causal 2 x 8191, 16 heads of 64:
+// 395 us, 696 TF/s; two maps of 64, 2 x 6007, 8 heads: 546 us, 515 TF/s.  Row blocks of 256 (8 waves) were 5 - 20 % slower.
 // ------------------------------------------------------------------------------------------------
 template <bool HALF, int D, int MAPS>
 __global__ __launch_bounds__(256, 2) void maps_fwd_kernel(const MapArgs a) {
@@ -484,7 +489,9 @@ __global__ __launch_bounds__(256, 2) void maps_fwd_kernel(const MapArgs a) {
 
 // ------------------------------------------------------------------------------------------------
 // forward of few rows: one workgroup = up to 32 rows (queries of the heads that share a key head) x one range of keys; its 4 waves take 32-key
-// tiles in turn and never wait for each other before the end.  Bound by the bytes of k and v: every key row is read once per row block.
+// tiles in turn and never wait for each other before the end.  Bound by the bytes of k and v: every key row is read once per row block.  A single query
+// over 16 x 32765 keys (16 heads, 4 of keys, 128 channels): 188 us, 4.9 TB/s; 5 over 16 x 20011, two maps of 64: 126 us, 4.4 TB/s.  One query over 257
+// keys: 11 us, the chain of dependent memory accesses (bias, tile, tile, join).
 // ------------------------------------------------------------------------------------------------
 template <bool HALF, int D, int MAPS>
 __global__ __launch_bounds__(256, 2) void maps_fwd_split_kernel(const MapArgs a) {
@@ -694,7 +701,7 @@ __global__ __launch_bounds__(256, 2) void maps_fwd_split_kernel(const MapArgs a)
   }
 }
 
-// joins the key ranges of maps_fwd_split_kernel: one wave per row, ranges in order
+// joins the key ranges of maps_fwd_split_kernel: one wave per row, ranges in order (5 - 7 us for 256 - 1280 rows of 8 ranges: latency)
 template <bool HALF, int D, int MAPS>
 __global__ __launch_bounds__(256) void maps_join_kernel(const MapArgs a) {
   constexpr int DV = MAPS * D, CPL = (DV + 63) / 64, W = MAPS * (DV + 2);
@@ -746,6 +753,8 @@ __global__ __launch_bounds__(256) void maps_join_kernel(const MapArgs a) {
 // ds = p (dp - r) needs r before the first key: rowsum(dO o) gives it up to the rounding of o, which is enough for dq (16 bits), and the exact
 // fp32 sum falls out of the same registers (one FMA per element): the key kernel forms ds, the bias table's and lam's gradients from that.
 // Row statistics leave as [B][H][64-query tile][MAPS][2][64] floats: log2 of the row sum (ROW_OFF for a row without one), r.
+// Bound as the forward: three products per pair of positions instead of two.  32 x 1232, 8 heads of 128: 312 us, 717 TF/s; causal 4 x 4096, 16 heads of
+// two maps of 64: 690 us, 598 TF/s.  (Exponentials placed under the MFMAs of dP by hand were 13 % slower.)
 // ------------------------------------------------------------------------------------------------
 template <bool HALF, int D, int MAPS>
 __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
@@ -927,6 +936,8 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
 // every head of the group in tiles of 64, so that the shared heads' gradients are summed in registers, in a fixed order.  8 waves: wave w has keys
 // 32 (w & 3) .. and of each tile the queries 32 (w >> 2) .., and the two waves of a key block add up at the end: two waves per SIMD, whose LDS round
 // trips, exponentials and MFMAs overlap (one wave of 4 per SIMD, with everything in 420 registers, spent two thirds of its time waiting).
+// Bound by the pipes and by LDS, of which a block near the diagonal uses twice as much (its score gradients are summed along the diagonals): 32 x 1232,
+// 8 heads of 128: 485 us, 615 TF/s over four products; causal 4 x 4096, 16 heads of two maps of 64: 680 us, 808 TF/s.
 // ------------------------------------------------------------------------------------------------
 template <bool HALF, int D, int MAPS>
 __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
@@ -1216,7 +1227,7 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
 // that ds is formed from the exact row sums without a second pass.  dS and then P go through LDS in 16 bits to the products, whose 32 x 32 tiles of
 // dq, dk and dv the waves share evenly.  Workgroups stay and fetch their next head under the stores.
 // Bound by memory and by the phases' latency: q, k, v, dO in, dq, dk, dv out, 392 MB for 256 x 107 positions and 8 heads of 128: 77 us at the rate of a
-// copy, 125 us measured (220 us by the two passes of longer rows).
+// copy, 117 us measured (221 us by the two passes of longer rows).
 // ------------------------------------------------------------------------------------------------
 template <bool HALF, int D, int MAPS>
 __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_kernel(const MapArgs a) {
@@ -1557,6 +1568,7 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
 
 // ------------------------------------------------------------------------------------------------
 // bias table's gradient: part [H][B x 32-key blocks x 2][gw] -> sums over a chunk of rows -> sums over the positions of a bucket.  Fixed order.
+// 6 - 9 us and 5 - 6 us: 35 MB of parts for 24 x 601 keys, 12 heads, 801 positions.
 // ------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void diag_sum_kernel(const float* part, long long rows, int gw, int chunk, float* out) {
   __shared__ float red[4][64];
@@ -1638,15 +1650,16 @@ int check_attn(const uvtg_attn_dims* d, int maps) {
 }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-// Few rows or few workgroups: the split kernel (a row block of 32 instead of 128, the keys cut into ranges).  heads packed per row block, row
-// blocks per key head, key ranges
-struct SplitPlan { int use, hb, blocks, nsplit; };
+// Few rows: the split kernel, row blocks of 32 instead of 128 and the keys cut into ranges.  A row block of 128 takes about 5 + c Sk us on its own,
+// c = 0.022 (one map of 128 channels) or 0.044 (two of 64), as long as there are workgroups for every CU; the split kernel with the join takes about
+// 11 us + 0.08 us per 1000 keys of each of its row blocks.  Measured, row blocks against split, us (8 heads of 128; of two maps of 64):
+//   1 x 128 queries: 300 keys 14, 11; 20, 14   2048 keys 52, 17; 95, 21   4 x 256: 512 keys 19, 24; 29, 30   4096 keys 98, 93; 185, 99
+//   7 x 256, 1024 keys: 31, 54; 52, 63   32 x 128, 2048 keys: 63, 158; 101, 163   64 x 32, 1024 keys: 47, 48; 59, 52   64 x 32, 107 keys: 11, 11; 14, 16
+// Up to 32 queries the two differ little and the heads of a group share a row block, so that their keys are read once.
+struct SplitPlan { int use, hb, blocks, nsplit; };         // heads packed per row block, row blocks per key head, key ranges
 SplitPlan plan_split(const uvtg_attn_dims* d, int maps) {
   SplitPlan p = {0, 1, 0, 1};
   const int G = d->H / d->Hkv;
-  const long long wg = (long long)((d->Sq + 127) / 128) * d->H * d->B;
-  p.use = d->Sq <= 32 || (wg < 128 && d->Sk >= 512);
-  if (!p.use) return p;
   if (d->Sq < 32) {
     p.hb = 32 / d->Sq < G ? 32 / d->Sq : G;
     const int win = maps == 1 ? (2 * d->reach + 1 < d->Sk + d->Sq ? 2 * d->reach + 1 : d->Sk + d->Sq) : 0;
@@ -1654,6 +1667,10 @@ SplitPlan plan_split(const uvtg_attn_dims* d, int maps) {
   }
   p.blocks = ((G + p.hb - 1) / p.hb) * ((p.hb * d->Sq + 31) / 32);
   const long long base = (long long)p.blocks * d->B * d->Hkv;
+  p.use = d->Sq <= 32 || (base <= 128 * maps && d->Sk >= 128 + 3 * base / maps);
+  if (!p.use) return p;
+  // about two workgroups per CU, of at least 256 keys (8 heads of 128, ranges of at least 512, 256, 128 keys: 128 queries over 2048 18, 17, 20 us; one
+  // query over 2048 15, 12, 11 us, over 8192 17, 15, 17 us)
   const long long want = (512 + base - 1) / base, most = d->Sk / 256;
   p.nsplit = (int)(want < most ? want : most);
   if (p.nsplit > 128) p.nsplit = 128;
@@ -1668,7 +1685,7 @@ void reachable(const uvtg_attn_dims* d, int& glo, int& gw) {
   gw = cl((long long)d->Sk - 1 - d->q_offset) - glo + 1;
 }
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
-// whole rows in one workgroup: one pass over the operands (256 x 107, 8 heads of 128: 125 us against 221 us of the two passes)
+// whole rows in one workgroup: one pass over the operands (256 x 107, 8 heads of 128: 117 us against 221 us of the two passes)
 bool short_rows(const uvtg_attn_dims* d) { return d->Sq <= 128 && d->Sk <= 128 && d->H == d->Hkv; }
 struct BwdWs { size_t rvec, part, sums, total; long long rows; int chunk, chunks; };
 BwdWs bwd_ws(const uvtg_attn_dims* d, int maps) {
