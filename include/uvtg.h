@@ -262,7 +262,7 @@ int uvtg_sine_position(const float* vid_mask, const float* txt_mask, const float
  * A row that sees no key: o = 0, lse = -inf, no gradient.
  * Scores, statistics and sums are fp32; probabilities and score gradients are rounded to the operands' type for the products with v, k, q, dO.
  * The backward pass forms the probabilities from lse: their relative error grows with a row's largest score, 2^-23 of it, and none exceeds 1.
- * Results are bit-reproducible (no floating-point atomics on memory, fixed orders of summation).
+ * Results are bit-reproducible for a given set of dims (no floating-point atomics on memory, fixed orders of summation).
  * D: 32, 64, or 128 (relpos only).  ws: uvtg_attn_ws_bytes(dims, maps, backward) bytes, 16-byte aligned, no initial value, may be NULL if 0;
  * maps = 1 relpos, 2 diff.  Calls in flight at the same time need a ws each. */
 typedef struct uvtg_attn_dims {

@@ -1653,8 +1653,9 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // Few rows: the split kernel, row blocks of 32 instead of 128 and the keys cut into ranges.  A row block of 128 takes about 5 + c Sk us on its own,
 // c = 0.022 (one map of 128 channels) or 0.044 (two of 64), as long as there are workgroups for every CU; the split kernel with the join takes about
 // 11 us + 0.08 us per 1000 keys of each of its row blocks.  Measured, row blocks against split, us (8 heads of 128; of two maps of 64):
-//   1 x 128 queries: 300 keys 14, 11; 20, 14   2048 keys 52, 17; 95, 21   4 x 256: 512 keys 19, 24; 29, 30   4096 keys 98, 93; 185, 99
+//   1 x 128 queries: 512 keys 18, 13; 28, 16   2048 keys 52, 17; 95, 21   4 x 256: 512 keys 19, 24; 29, 30   4096 keys 98, 93; 185, 99
 //   7 x 256, 1024 keys: 31, 54; 52, 63   32 x 128, 2048 keys: 63, 158; 101, 163   64 x 32, 1024 keys: 47, 48; 59, 52   64 x 32, 107 keys: 11, 11; 14, 16
+// (Under 512 keys the gain is 3 - 6 us at most, and a sample's result does not depend on how many others there are.)
 // Up to 32 queries the two differ little and the heads of a group share a row block, so that their keys are read once.
 struct SplitPlan { int use, hb, blocks, nsplit; };         // heads packed per row block, row blocks per key head, key ranges
 SplitPlan plan_split(const uvtg_attn_dims* d, int maps) {
@@ -1667,7 +1668,7 @@ SplitPlan plan_split(const uvtg_attn_dims* d, int maps) {
   }
   p.blocks = ((G + p.hb - 1) / p.hb) * ((p.hb * d->Sq + 31) / 32);
   const long long base = (long long)p.blocks * d->B * d->Hkv;
-  p.use = d->Sq <= 32 || (base <= 128 * maps && d->Sk >= 128 + 3 * base / maps);
+  p.use = d->Sq <= 32 || (base <= 128 * maps && d->Sk >= 512);
   if (!p.use) return p;
   // about two workgroups per CU, of at least 256 keys (8 heads of 128, ranges of at least 512, 256, 128 keys: 128 queries over 2048 18, 17, 20 us; one
   // query over 2048 15, 12, 11 us, over 8192 17, 15, 17 us)
