@@ -264,7 +264,7 @@ int uvtg_sine_position(const float* vid_mask, const float* txt_mask, const float
  * The backward pass forms the probabilities from lse: their relative error grows with a row's largest score, 2^-23 of it, and none exceeds 1.
  * Results are bit-reproducible for a given set of dims (no floating-point atomics on memory, fixed orders of summation).
  * D: 32, 64, or 128 (relpos only).  ws: uvtg_attn_ws_bytes(dims, maps, backward) bytes, 16-byte aligned, no initial value, may be NULL if 0;
- * maps = 1 relpos, 2 diff.  Calls in flight at the same time need a ws each. */
+ * maps = 1 relpos, 2 diff.  Calls in flight at the same time need a ws each.  No output may overlap an input. */
 typedef struct uvtg_attn_dims {
   int struct_size;             /* = sizeof(uvtg_attn_dims)                                    */
   int dtype;                   /* 0 bf16, 1 fp16                                              */

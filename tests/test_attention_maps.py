@@ -702,6 +702,10 @@ def test_refusals_name_the_argument():
         (RuntimeError, "reach", lambda: ops.relpos_attention_fwd(q, k, v, w, bk[:1])),
         (ValueError, "do and o", lambda: ops.relpos_attention_bwd(do[:, :2], q, k, v, w, bk, o, lse)),
         (ValueError, "do must be", lambda: ops.relpos_attention_bwd(do.float(), q, k, v, w, bk, o, lse)),
+        (ValueError, "do must be", lambda: ops.relpos_attention_bwd(do.cpu(), q, k, v, w, bk, o, lse)),
+        (ValueError, "o must be", lambda: ops.relpos_attention_bwd(do, q, k, v, w, bk, o.cpu(), lse)),
+        (ValueError, "lse must be", lambda: ops.relpos_attention_bwd(do, q, k, v, w, bk, o, lse.cpu())),
+        (ValueError, "lse must be", lambda: ops.relpos_attention_bwd(do, q, k, v, w, bk, o, lse.double())),
     ]
     q2, k2, v2, lam, _, do2 = make("diff", torch.float16, 1, 2, 2, 64, 4, 6)
     od, lse2, o2 = ops.diff_attention_fwd(q2, k2, v2, lam, need_o2=True)
@@ -711,6 +715,8 @@ def test_refusals_name_the_argument():
         (ValueError, "lam", lambda: ops.diff_attention_fwd(q2, k2, v2, lam[:1])),
         (RuntimeError, "32 or 64", lambda: ops.diff_attention_fwd(torch.cat([q2, q2], -1), torch.cat([k2, k2], -1), torch.cat([v2, v2], -1), lam)),
         (ValueError, "do, o and o2", lambda: ops.diff_attention_bwd(do2, q2, k2, v2, lam, od, o2[:, :2], lse2)),
+        (ValueError, "o2 must be", lambda: ops.diff_attention_bwd(do2, q2, k2, v2, lam, od, o2.cpu(), lse2)),
+        (ValueError, "lse must be", lambda: ops.diff_attention_bwd(do2, q2, k2, v2, lam, od, o2, lse2.cpu())),
     ]
     for kind, text, call in cases:
         with pytest.raises(kind, match=text):

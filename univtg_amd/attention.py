@@ -7,7 +7,10 @@
     o = diff_attention(q, k, v, lam, kvalid=kvalid)                        # lam: [H], e.g. exp(a1 . b1) - exp(a2 . b2) + lam0 of four parameters
 
 Under `torch.no_grad()`, or when nothing requires a gradient, they are the forward calls alone: a few new tokens against a cache of keys and
-values (`q_offset` = how many came before) run the kernel that splits the keys."""
+values (`q_offset` = how many came before) run the kernel that splits the keys.
+
+A step that is captured into a graph is captured whole, forward and backward, on one stream, with no autograd graph of another stream alive that
+holds the same leaves (such a call is refused)."""
 from __future__ import annotations
 
 import itertools

@@ -305,9 +305,9 @@ def _relpos_operands(d, q, table, buckets):
     return _f32c(table), buckets.contiguous()
 
 
-def _attn_saved(name, t, like, what):
-    if t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{name}: {what} must be {like.dtype} on {like.device}")
+def _attn_saved(name, t, like, what, dtype=None):
+    if t.dtype != (dtype or like.dtype) or t.device != like.device:
+        raise ValueError(f"{name}: {what} must be {dtype or like.dtype} on {like.device}")
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
@@ -360,7 +360,8 @@ def relpos_attention_bwd(do, q, k, v, table, buckets, o, lse, kvalid=None, q_off
     table, buckets = _relpos_operands(d, q, table, buckets)
     if do.shape != (d.B, d.Sq, d.H, d.D) or o.shape != do.shape or lse.shape != (d.B, d.H, d.Sq):
         raise ValueError("relpos_attention_bwd: do and o must be [B, Sq, H, D], lse [B, H, Sq]")
-    return _relpos_bwd(do, d, q, k, v, table, buckets, kvalid, _attn_saved("relpos_attention_bwd", o, q, "o"), _f32c(lse), need_dtable)
+    return _relpos_bwd(do, d, q, k, v, table, buckets, kvalid, _attn_saved("relpos_attention_bwd", o, q, "o"),
+                       _attn_saved("relpos_attention_bwd", lse, q, "lse", torch.float32), need_dtable)
 
 
 def _lam_operand(d, q, lam):
@@ -414,4 +415,4 @@ def diff_attention_bwd(do, q, k, v, lam, o, o2, lse, kvalid=None, q_offset=0, ca
     if do.shape != (d.B, d.Sq, d.H, 2 * d.D) or o.shape != do.shape or o2.shape != do.shape or lse.shape != (d.B, d.H, 2, d.Sq):
         raise ValueError("diff_attention_bwd: do, o and o2 must be [B, Sq, H, 2 D], lse [B, H, 2, Sq]")
     o, o2 = (_attn_saved("diff_attention_bwd", t, q, w) for t, w in ((o, "o"), (o2, "o2")))
-    return _diff_bwd(do, d, q, k, v, lam, kvalid, o, o2, _f32c(lse), need_dlam)
+    return _diff_bwd(do, d, q, k, v, lam, kvalid, o, o2, _attn_saved("diff_attention_bwd", lse, q, "lse", torch.float32), need_dlam)
