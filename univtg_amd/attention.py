@@ -28,6 +28,12 @@ _nodes = {}
 _numbers = itertools.count(random.getrandbits(62))
 
 
+def _once(backward):
+    """torch's once_differentiable, whose wrapping costs 5 us: only where a second derivative could be asked for (create_graph)."""
+    guarded = once_differentiable(backward)
+    return lambda ctx, do: guarded(ctx, do) if torch.is_grad_enabled() else backward(ctx, do)
+
+
 class _RelposAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, buckets, kvalid, opts):
@@ -36,7 +42,7 @@ class _RelposAttention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, do):
         return *ops._relpos_bwd(do, ctx.dims, *ctx.saved_tensors, ctx.needs_input_grad[3]), None, None, None
 
@@ -49,7 +55,7 @@ class _DiffAttention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, do):
         return *ops._diff_bwd(do, ctx.dims, *ctx.saved_tensors, ctx.needs_input_grad[3]), None, None
 

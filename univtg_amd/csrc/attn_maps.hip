@@ -115,7 +115,8 @@ __device__ __forceinline__ s16x8 row_frag(unsigned at, int i, int bytes) {
 }
 __device__ __forceinline__ s16x8 col_frag(unsigned at0, unsigned at1, int i, int bytes) {
   typedef __attribute__((address_space(3))) s16x4* lptr;
-  return cat4(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(uintptr_t)((at0 ^ (64 * i)) + bytes)), __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(uintptr_t)((at1 ^ (64 * i)) + bytes)));
+  return cat4(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(uintptr_t)((at0 ^ (64 * i)) + bytes)),
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(uintptr_t)((at1 ^ (64 * i)) + bytes)));
 }
 __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
 
@@ -175,7 +176,8 @@ template <int W, int ROWS, int NW> struct Loader {
     for (int i = 0; i < PIECES; i++) {
       const int n = i * NW + wave, r0 = min(row0 + n * RPI, last);
       if (NI % NW == 0 || n < NI)
-        dma16(base + disp + (unsigned long long)(unsigned)r0 * stride, (unsigned)min((int)opaque(row), last - r0) * stride + (chunk ^ (16 * Tile<W>::f(NW == 1 ? i % PERIOD * RPI : 0))), lds + n * 1024);   // (opaque: not kept ready)
+        dma16(base + disp + (unsigned long long)(unsigned)r0 * stride,                                 // (opaque: not kept ready)
+              (unsigned)min((int)opaque(row), last - r0) * stride + (chunk ^ (16 * Tile<W>::f(NW == 1 ? i % PERIOD * RPI : 0))), lds + n * 1024);
     }
   }
 };
@@ -1065,7 +1067,8 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
           fence();
         }
         if (req) request(qt + 1, buf ^ 1);                 // (while the score MFMAs run)
-        const unsigned qt0 = opaque(lds_at(sQ) + tq0), qt1 = opaque(lds_at(sQ) + tq1), ot0 = DV == D ? qt0 : opaque(lds_at(sO) + to0), ot1 = DV == D ? qt1 : opaque(lds_at(sO) + to1);
+        const unsigned qt0 = opaque(lds_at(sQ) + tq0), qt1 = opaque(lds_at(sQ) + tq1);
+        const unsigned ot0 = DV == D ? qt0 : opaque(lds_at(sO) + to0), ot1 = DV == D ? qt1 : opaque(lds_at(sO) + to1);
         // transposed fragments, 16 queries (hf) x 32 channels: dO's NDV blocks, then q's ND blocks of each map
         auto tcol = [&](int i) {
           const int hf = i / NP, c = i % NP;
@@ -1268,301 +1271,302 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
   request(b, h, threadIdx.x & 63);
 #pragma unroll 1
   for (int id = blockIdx.x; id < heads; id += gridDim.x, b = b_next, h = h_next) {
-  const int tid = opaque(threadIdx.x), lane = tid & 63, g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;     // (opaque: nothing is kept ready over the loop)
-  const int q0 = w4 * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1), key0 = half * 64;
-  const bool live = q0 < a.Sq;
-  float L[MAPS];
+    // (opaque: nothing is kept ready over the loop)
+    const int tid = opaque(threadIdx.x), lane = tid & 63, g = lane >> 5, l31 = lane & 31, i16 = lane & 15, qd = (lane >> 4) & 1;
+    const int q0 = w4 * 32, q_raw = q0 + l31, qrow = min(q_raw, a.Sq - 1), key0 = half * 64;
+    const bool live = q0 < a.Sq;
+    float L[MAPS];
 #pragma unroll
-  for (int m = 0; m < MAPS; m++) {
-    const float l = a.lse_in[(((size_t)b * a.H + h) * MAPS + m) * a.Sq + qrow];
-    L[m] = q_raw >= a.Sq || l == -INFINITY ? ROW_OFF : l * LOG2E;
-  }
-  const float lam = MAPS == 2 ? a.lam[h] : 0.f;
-  // masks of both halves of the keys
-  const unsigned char* kv = a.kvalid ? a.kvalid + (size_t)b * a.mask_sb : nullptr;
-  unsigned long long mask[2];
+    for (int m = 0; m < MAPS; m++) {
+      const float l = a.lse_in[(((size_t)b * a.H + h) * MAPS + m) * a.Sq + qrow];
+      L[m] = q_raw >= a.Sq || l == -INFINITY ? ROW_OFF : l * LOG2E;
+    }
+    const float lam = MAPS == 2 ? a.lam[h] : 0.f;
+    // masks of both halves of the keys
+    const unsigned char* kv = a.kvalid ? a.kvalid + (size_t)b * a.mask_sb : nullptr;
+    unsigned long long mask[2];
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int key = 64 * i + lane;
-    mask[i] = __builtin_amdgcn_ballot_w64(key < a.Sk && (!kv || kv[min(key, a.Sk - 1)] != 0));
-  }
-  const int rlo = -(a.Sq - 1) - a.off, rhi = 127 - a.off;  // positions of the workgroup
-  float* row = sRow + wave * 96;
-  if constexpr (BIAS) {
-    if (h != h_last) load_bias(a, h, rlo, rhi, sB, tid, 512);
-    h_last = h;
-  }
-  dma_wait();
-  __syncthreads();
-  if ((mask[0] & mask[1]) != ~0ull) {                      // masked rows, and the repeated ones behind the last
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-      if (mask[i] != ~0ull) {
-#pragma unroll
-        for (int m = 0; m < MAPS; m++) clear_rows<D>(sK + m * KT + i * 64 * D, mask[i], 64, tid, 512);
-        clear_rows<DV>(sV + i * 64 * DV, mask[i], 64, tid, 512);
-      }
+    for (int i = 0; i < 2; i++) {
+      const int key = 64 * i + lane;
+      mask[i] = __builtin_amdgcn_ballot_w64(key < a.Sk && (!kv || kv[min(key, a.Sk - 1)] != 0));
+    }
+    const int rlo = -(a.Sq - 1) - a.off, rhi = 127 - a.off;  // positions of the workgroup
+    float* row = sRow + wave * 96;
+    if constexpr (BIAS) {
+      if (h != h_last) load_bias(a, h, rlo, rhi, sB, tid, 512);
+      h_last = h;
+    }
+    dma_wait();
     __syncthreads();
-  }
-  // One workgroup per CU, all at the same place: the memory would idle under the products.  The next head's operands come to L2 meanwhile, a lane
-  // touching a line of 128 bytes (144 -> 126 us for 256 x 107, 8 heads of 128; two workgroups per CU overlap by themselves, 106 us against 108).
-  const bool more = id + (int)gridDim.x < heads;
-  sample(more ? id + gridDim.x : id, b_next, h_next);
-  int touched[2] = {0, 0};
-  if constexpr (DV > 32) {
-    constexpr int LK = MAPS * (D > 64 ? D / 64 : 1), LV = DV / 64;
-    const int t = tid & 255, S = (half ? a.Sq : a.Sk) - 1, lk = t % LK, lv = t % LV;
-    const bf16_t* x = half ? a.q + (long long)b_next * a.q_sb + (long long)h_next * a.q_sh : a.k + (long long)b_next * a.k_sb + (long long)h_next * a.k_sh;
-    const bf16_t* y = half ? a.dO + ((size_t)b_next * a.Sq * a.H + h_next) * DV : a.v + (long long)b_next * a.v_sb + (long long)h_next * a.v_sh;
-    touched[0] = *(const int*)(x + (long long)min(t / LK, S) * (half ? a.q_ss : a.k_ss) + (MAPS == 2 ? lk * (half ? a.q_sm : a.k_sm) : lk * 64));
-    touched[1] = *(const int*)(y + (long long)min(t / LV, S) * (half ? (long long)a.H * DV : a.v_ss) + lv * 64);
-  }
-  const int koff = 2 * Tile<D>::off(l31, 8 * g), voff = 2 * Tile<DV>::off(l31, 8 * g);                // bytes
-  const int toff0 = 2 * Tile<D>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), toff1 = 2 * Tile<D>::rows8(toff0 / 2);
-  const int ooff0 = 2 * Tile<DV>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), ooff1 = 2 * Tile<DV>::rows8(ooff0 / 2);
-  const int xoff0 = 2 * Tile<128>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), xoff1 = 2 * Tile<128>::rows8(xoff0 / 2);
-  // ---- scores of 32 queries x 2 blocks of 32 keys: p of every map, dP, and this half's row sums
-  f32x16 p[MAPS][2], dp[2];
-  float rs[MAPS];
+    if ((mask[0] & mask[1]) != ~0ull) {                      // masked rows, and the repeated ones behind the last
 #pragma unroll
-  for (int m = 0; m < MAPS; m++) { rs[m] = 0.f; zero(p[m][0]); zero(p[m][1]); }
-  zero(dp[0]); zero(dp[1]);
-  bool on[2];                                              // the block has a (query, key) pair
+      for (int i = 0; i < 2; i++)
+        if (mask[i] != ~0ull) {
 #pragma unroll
-  for (int kb = 0; kb < 2; kb++) on[kb] = live && (unsigned)(mask[half] >> (32 * kb)) != 0 && (!a.causal || min(q0 + 31, a.Sq - 1) + a.off >= key0 + 32 * kb);
-  if (on[0] || on[1]) {
-    s16x8 qf[MAPS][NK], of[NV];
+          for (int m = 0; m < MAPS; m++) clear_rows<D>(sK + m * KT + i * 64 * D, mask[i], 64, tid, 512);
+          clear_rows<DV>(sV + i * 64 * DV, mask[i], 64, tid, 512);
+        }
+      __syncthreads();
+    }
+    // One workgroup per CU, all at the same place: the memory would idle under the products.  The next head's operands come to L2 meanwhile, a lane
+    // touching a line of 128 bytes (144 -> 126 us for 256 x 107, 8 heads of 128; two workgroups per CU overlap by themselves, 106 us against 108).
+    const bool more = id + (int)gridDim.x < heads;
+    sample(more ? id + gridDim.x : id, b_next, h_next);
+    int touched[2] = {0, 0};
+    if constexpr (DV > 32) {
+      constexpr int LK = MAPS * (D > 64 ? D / 64 : 1), LV = DV / 64;
+      const int t = tid & 255, S = (half ? a.Sq : a.Sk) - 1, lk = t % LK, lv = t % LV;
+      const bf16_t* x = half ? a.q + (long long)b_next * a.q_sb + (long long)h_next * a.q_sh : a.k + (long long)b_next * a.k_sb + (long long)h_next * a.k_sh;
+      const bf16_t* y = half ? a.dO + ((size_t)b_next * a.Sq * a.H + h_next) * DV : a.v + (long long)b_next * a.v_sb + (long long)h_next * a.v_sh;
+      touched[0] = *(const int*)(x + (long long)min(t / LK, S) * (half ? a.q_ss : a.k_ss) + (MAPS == 2 ? lk * (half ? a.q_sm : a.k_sm) : lk * 64));
+      touched[1] = *(const int*)(y + (long long)min(t / LV, S) * (half ? (long long)a.H * DV : a.v_ss) + lv * 64);
+    }
+    const int koff = 2 * Tile<D>::off(l31, 8 * g), voff = 2 * Tile<DV>::off(l31, 8 * g);                // bytes
+    const int toff0 = 2 * Tile<D>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), toff1 = 2 * Tile<D>::rows8(toff0 / 2);
+    const int ooff0 = 2 * Tile<DV>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), ooff1 = 2 * Tile<DV>::rows8(ooff0 / 2);
+    const int xoff0 = 2 * Tile<128>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), xoff1 = 2 * Tile<128>::rows8(xoff0 / 2);
+    // ---- scores of 32 queries x 2 blocks of 32 keys: p of every map, dP, and this half's row sums
+    f32x16 p[MAPS][2], dp[2];
+    float rs[MAPS];
 #pragma unroll
-    for (int m = 0; m < MAPS; m++)
+    for (int m = 0; m < MAPS; m++) { rs[m] = 0.f; zero(p[m][0]); zero(p[m][1]); }
+    zero(dp[0]); zero(dp[1]);
+    bool on[2];                                              // the block has a (query, key) pair
 #pragma unroll
-      for (int ks = 0; ks < NK; ks++) qf[m][ks] = row_frag(lds_at(sQ + m * KT + q0 * D) + koff, ks, 0);
+    for (int kb = 0; kb < 2; kb++) on[kb] = live && (unsigned)(mask[half] >> (32 * kb)) != 0 && (!a.causal || min(q0 + 31, a.Sq - 1) + a.off >= key0 + 32 * kb);
+    if (on[0] || on[1]) {
+      s16x8 qf[MAPS][NK], of[NV];
 #pragma unroll
-    for (int ks = 0; ks < NV; ks++) of[ks] = row_frag(lds_at(sO + q0 * DV) + voff, ks, 0);
+      for (int m = 0; m < MAPS; m++)
+#pragma unroll
+        for (int ks = 0; ks < NK; ks++) qf[m][ks] = row_frag(lds_at(sQ + m * KT + q0 * D) + koff, ks, 0);
+#pragma unroll
+      for (int ks = 0; ks < NV; ks++) of[ks] = row_frag(lds_at(sO + q0 * DV) + voff, ks, 0);
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++) {
+        if (!on[kb]) continue;
+        const unsigned ka = opaque(lds_at(sK + (key0 + 32 * kb) * D) + koff), va = opaque(lds_at(sV + (key0 + 32 * kb) * DV) + voff);
+        auto kvrow = [&](int i) { return i < NV ? row_frag(va, i, 0) : row_frag(ka, (i - NV) % NK, (i - NV) / NK * KT * 2); };
+        s16x8 fa[RA];
+        fill<NV + MAPS * NK>(fa, kvrow);
+        fence();
+        run<NV + MAPS * NK>(fa, kvrow, [&](int i, s16x8 x) {
+          const int j = i < NV ? 0 : i - NV;
+          if (i < NV) dp[kb] = mma<HALF>(x, of[i < NV ? i : 0], dp[kb]); else p[j / NK][kb] = mma<HALF>(x, qf[j / NK][j % NK], p[j / NK][kb]);
+        });
+        const unsigned mk = (unsigned)(mask[half] >> (32 * kb));
+        const bool part = mk != ~0u || (a.causal && q0 + a.off < key0 + 32 * kb + 31);
+#pragma unroll
+        for (int m = 0; m < MAPS; m++) {
+          float cc = a.c;
+          if constexpr (BIAS) {
+            const float* bp = sB + (key0 + 32 * kb - qrow - a.off + 4 * g - rlo);
+#pragma unroll
+            for (int r = 0; r < 16; r++) p[m][kb][r] = fmaf(p[m][kb][r], a.c, bp[(r & 3) + 8 * (r >> 2)]);
+            cc = 1.f;
+          }
+          if (part) mask_scores(p[m][kb], mk, a.causal ? q_raw + a.off - key0 - 32 * kb : 32, g, -INFINITY);
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            p[m][kb][r] = prob(fmaf(p[m][kb][r], cc, -L[m]));
+            rs[m] = fmaf(p[m][kb][r], dp[kb][r], rs[m]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MAPS; m++) {
+      rs[m] = half_sum(rs[m]);
+      if (g == 0) sR[(half * MAPS + m) * 128 + q_raw] = rs[m];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < MAPS; m++) rs[m] = sR[m * 128 + q_raw] + sR[(MAPS + m) * 128 + q_raw];
+    if (MAPS == 2 && half == 0 && live) {                    // lam's gradient: the wave's 32 rows, [H][B][32-row block]
+      const float w = wave_sum_dpp(g == 0 && q_raw < a.Sq ? rs[MAPS - 1] : 0.f);
+      if (lane == 0) a.part[((size_t)h * a.B + b) * ((a.Sq + 31) / 32) + w4] = w;
+    }
+    // ---- P and dS, packed as operands
+    unsigned pp[2][8], pd[MAPS][2][8];
+    float* diag = sX + wave * 768;
+    if constexpr (BIAS) {
+#pragma unroll
+      for (int i = 0; i < 12; i++) diag[i * 64 + lane] = 0.f;
+      row[lane] = 0.f;
+      if (lane < 32) row[64 + lane] = 0.f;
+    }
+    float fl = 0.f, fr = 0.f;
 #pragma unroll
     for (int kb = 0; kb < 2; kb++) {
-      if (!on[kb]) continue;
-      const unsigned ka = opaque(lds_at(sK + (key0 + 32 * kb) * D) + koff), va = opaque(lds_at(sV + (key0 + 32 * kb) * DV) + voff);
-      auto kvrow = [&](int i) { return i < NV ? row_frag(va, i, 0) : row_frag(ka, (i - NV) % NK, (i - NV) / NK * KT * 2); };
-      s16x8 fa[RA];
-      fill<NV + MAPS * NK>(fa, kvrow);
-      fence();
-      run<NV + MAPS * NK>(fa, kvrow, [&](int i, s16x8 x) {
-        const int j = i < NV ? 0 : i - NV;
-        if (i < NV) dp[kb] = mma<HALF>(x, of[i < NV ? i : 0], dp[kb]); else p[j / NK][kb] = mma<HALF>(x, qf[j / NK][j % NK], p[j / NK][kb]);
-      });
-      const unsigned mk = (unsigned)(mask[half] >> (32 * kb));
-      const bool part = mk != ~0u || (a.causal && q0 + a.off < key0 + 32 * kb + 31);
 #pragma unroll
-      for (int m = 0; m < MAPS; m++) {
-        float cc = a.c;
-        if constexpr (BIAS) {
-          const float* bp = sB + (key0 + 32 * kb - qrow - a.off + 4 * g - rlo);
+      for (int r = 0; r < 16; r += 2) {
+        float x[2], d[MAPS][2];
 #pragma unroll
-          for (int r = 0; r < 16; r++) p[m][kb][r] = fmaf(p[m][kb][r], a.c, bp[(r & 3) + 8 * (r >> 2)]);
-          cc = 1.f;
+        for (int u = 0; u < 2; u++) {
+          x[u] = p[0][kb][r + u];
+          d[0][u] = x[u] * (dp[kb][r + u] - rs[0]);
+          if constexpr (MAPS == 2) {
+            const float y = -lam * p[MAPS - 1][kb][r + u];
+            d[MAPS - 1][u] = y * (dp[kb][r + u] - rs[MAPS - 1]);
+            x[u] += y;
+          }
+          if constexpr (BIAS) dp[kb][r + u] = d[0][u];
         }
-        if (part) mask_scores(p[m][kb], mk, a.causal ? q_raw + a.off - key0 - 32 * kb : 32, g, -INFINITY);
+        pp[kb][r / 2] = opaque(pack2<HALF>(x[0], x[1]));     // (opaque: formed here, by all waves at once, not in the rounds below)
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-          p[m][kb][r] = prob(fmaf(p[m][kb][r], cc, -L[m]));
-          rs[m] = fmaf(p[m][kb][r], dp[kb][r], rs[m]);
+        for (int m = 0; m < MAPS; m++) pd[m][kb][r / 2] = opaque(pack2<HALF>(d[m][0], d[m][1]));
+      }
+      if constexpr (BIAS) {
+        if (on[kb]) {
+          // sums along the block's diagonals as in the key kernel, keys and queries exchanged: lane l collects position l - 31 of the block
+          float v = 0.f;
+#pragma unroll
+          for (int ps = 0; ps < 2; ps++) {                   // 16 keys
+#pragma unroll
+            for (int r = 0; r < 8; r++) diag[(4 * g + (r & 3) + 8 * (r >> 2)) * 49 + 31 - l31] = dp[kb][8 * ps + r];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const float* col = diag + (ps ? (lane >= 16 && lane < 63 ? lane - 16 : 47) : (lane < 47 ? lane : 47));
+            float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 16; i++) t[i & 3] += col[i * 48];
+            v += (t[0] + t[1]) + (t[2] + t[3]);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+          }
+          const int rel = key0 + 32 * kb - q0 - a.off + lane - 31;
+          if (lane < 63) {
+            if (rel >= a.R) fr += v;
+            else if (rel <= -a.R) fl += v;
+            else row[32 * kb + lane] += v;
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
         }
       }
-    }
-  }
-#pragma unroll
-  for (int m = 0; m < MAPS; m++) {
-    rs[m] = half_sum(rs[m]);
-    if (g == 0) sR[(half * MAPS + m) * 128 + q_raw] = rs[m];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int m = 0; m < MAPS; m++) rs[m] = sR[m * 128 + q_raw] + sR[(MAPS + m) * 128 + q_raw];
-  if (MAPS == 2 && half == 0 && live) {                    // lam's gradient: the wave's 32 rows, [H][B][32-row block]
-    const float w = wave_sum_dpp(g == 0 && q_raw < a.Sq ? rs[MAPS - 1] : 0.f);
-    if (lane == 0) a.part[((size_t)h * a.B + b) * ((a.Sq + 31) / 32) + w4] = w;
-  }
-  // ---- P and dS, packed as operands
-  unsigned pp[2][8], pd[MAPS][2][8];
-  float* diag = sX + wave * 768;
-  if constexpr (BIAS) {
-#pragma unroll
-    for (int i = 0; i < 12; i++) diag[i * 64 + lane] = 0.f;
-    row[lane] = 0.f;
-    if (lane < 32) row[64 + lane] = 0.f;
-  }
-  float fl = 0.f, fr = 0.f;
-#pragma unroll
-  for (int kb = 0; kb < 2; kb++) {
-#pragma unroll
-    for (int r = 0; r < 16; r += 2) {
-      float x[2], d[MAPS][2];
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-        x[u] = p[0][kb][r + u];
-        d[0][u] = x[u] * (dp[kb][r + u] - rs[0]);
-        if constexpr (MAPS == 2) {
-          const float y = -lam * p[MAPS - 1][kb][r + u];
-          d[MAPS - 1][u] = y * (dp[kb][r + u] - rs[MAPS - 1]);
-          x[u] += y;
-        }
-        if constexpr (BIAS) dp[kb][r + u] = d[0][u];
-      }
-      pp[kb][r / 2] = opaque(pack2<HALF>(x[0], x[1]));     // (opaque: formed here, by all waves at once, not in the rounds below)
-#pragma unroll
-      for (int m = 0; m < MAPS; m++) pd[m][kb][r / 2] = opaque(pack2<HALF>(d[m][0], d[m][1]));
     }
     if constexpr (BIAS) {
-      if (on[kb]) {
-        // sums along the block's diagonals as in the key kernel, keys and queries exchanged: lane l collects position l - 31 of the block
-        float v = 0.f;
+      fl = wave_sum_dpp(fl); fr = wave_sum_dpp(fr);
+      if (lane == 0) { sEnd[wave * 2] = fl; sEnd[wave * 2 + 1] = fr; }
+    }
+    // tiles of the wave: queries 32 qb, channels 32 qc of dq; keys 32 kb .. 32 + channels 32 kc .. of dk and dv
+    auto qb = [&](int j) { return MAPS == 2 && NT == 2 ? 2 * j + half : NC == 1 ? wave : wave >> 1; };
+    auto qc = [&](int j) { return MAPS == 2 && NT == 2 ? w4 : NC == 1 ? 0 : NT * (wave & 1) + j; };
+    const int kblk = NC == 1 ? wave : wave >> 1, kc = NC == 1 ? 0 : NT * (wave & 1);
+    const bool keys = 32 * kblk < a.Sk && kblk < 4;
+    f32x16 dq[NT], dk[NT], dv[NT];
 #pragma unroll
-        for (int ps = 0; ps < 2; ps++) {                   // 16 keys
+    for (int j = 0; j < NT; j++) { zero(dq[j]); zero(dk[j]); zero(dv[j]); }
+    // products over `n` queries: the left operand's channels `c`, the right one's keys, both transposed; chunks of 16, the next one's fragments on their
+    // way under the MFMAs of the current one
+    auto products = [&](f32x16 (&acc)[NT], unsigned l0, unsigned l1, int lrow, int c, unsigned r0, unsigned r1, int n) {
+      const int n16 = (n + 15) / 16;
+      auto load = [&](int i, s16x8& fb, s16x8 (&fa)[NT]) {
+        fb = col_frag(r0 + i * 4096, r1 + i * 4096, kblk, 0);
 #pragma unroll
-          for (int r = 0; r < 8; r++) diag[(4 * g + (r & 3) + 8 * (r >> 2)) * 49 + 31 - l31] = dp[kb][8 * ps + r];
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          __builtin_amdgcn_wave_barrier();
-          const float* col = diag + (ps ? (lane >= 16 && lane < 63 ? lane - 16 : 47) : (lane < 47 ? lane : 47));
-          float t[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < NT; j++) fa[j] = col_frag(l0 + i * lrow, l1 + i * lrow, c + j, 0);
+      };
+      auto mul = [&](const s16x8& fb, const s16x8 (&fa)[NT]) {
 #pragma unroll
-          for (int i = 0; i < 16; i++) t[i & 3] += col[i * 48];
-          v += (t[0] + t[1]) + (t[2] + t[3]);
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          __builtin_amdgcn_wave_barrier();
+        for (int j = 0; j < NT; j++) acc[j] = mma<HALF>(fa[j], fb, acc[j]);
+      };
+      s16x8 fb0, fb1, fa0[NT], fa1[NT];
+      load(0, fb0, fa0);
+#pragma unroll 1
+      for (int i = 0; i < n16; i += 2) {
+        load(min(i + 1, n16 - 1), fb1, fa1);
+        fence();
+        mul(fb0, fa0);
+        fence();
+        load(min(i + 2, n16 - 1), fb0, fa0);
+        fence();
+        if (i + 1 < n16) mul(fb1, fa1);
+      }
+    };
+    auto put = [&](bf16_t* tile, const unsigned (&x)[2][8], int row) {
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) *(u32x2*)(tile + Tile<128>::off(row, key0 + 32 * kb + 8 * j + 4 * g)) = (u32x2){x[kb][2 * j], x[kb][2 * j + 1]};
+    };
+    // ---- dq and dk: dS of RS queries at a time
+#pragma unroll 1
+    for (int qr = 0; qr < a.Sq; qr += RS) {
+      if (qr || DV == 32) __syncthreads();                   // the last round's dS, or the diagonals, are read (v: all waves have met in the row sums since)
+      if (live && q0 >= qr && q0 < qr + RS) {
+#pragma unroll
+        for (int m = 0; m < MAPS; m++) put(sS + m * RS * 128, pd[m], q0 - qr + l31);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < NT; j++) {
+        if (32 * qb(j) < qr || 32 * qb(j) >= min(qr + RS, a.Sq)) continue;
+        const int m = qc(j) / ND;
+        const unsigned ra = opaque(lds_at(sS) + m * RS * 256 + (32 * qb(j) - qr) * 256 + 2 * Tile<128>::off(l31, 4 * g));
+        const unsigned ta0 = opaque(lds_at(sK) + m * KT * 2 + toff0), ta1 = opaque(lds_at(sK) + m * KT * 2 + toff1);
+        const int c = qc(j) % ND;
+        // 16 keys a step, in the order in which a transposing read of k delivers them
+        auto kcol = [&](int i) { return col_frag(ta0, ta1, c, i * 32 * D); };
+        typedef const __attribute__((address_space(3))) s16x4* rptr;
+        auto dsrow = [&](int i) { return cat4(*(rptr)(uintptr_t)(ra ^ (32 * i)), *(rptr)(uintptr_t)(ra ^ (32 * i) ^ 16)); };
+        s16x8 fa[RA], fb[RA];
+        fill<8>(fa, kcol);
+        fill<8>(fb, dsrow);
+        fence();
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          dq[j] = mma<HALF>(fa[i % RA], fb[i % RA], dq[j]);
+          if (i + RA < 8) { fa[i % RA] = kcol(i + RA); fb[i % RA] = dsrow(i + RA); }
+          fence();
         }
-        const int rel = key0 + 32 * kb - q0 - a.off + lane - 31;
-        if (lane < 63) {
-          if (rel >= a.R) fr += v;
-          else if (rel <= -a.R) fl += v;
-          else row[32 * kb + lane] += v;
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+      }
+      if (keys) {
+        const int m = kc / ND;
+        const unsigned qa = lds_at(sQ) + m * KT * 2 + qr * D * 2, sa = lds_at(sS) + m * RS * 256;
+        products(dk, opaque(qa + toff0), opaque(qa + toff1), 32 * D, kc % ND, opaque(sa + xoff0), opaque(sa + xoff1), min(RS, a.Sq - qr));
       }
     }
-  }
-  if constexpr (BIAS) {
-    fl = wave_sum_dpp(fl); fr = wave_sum_dpp(fr);
-    if (lane == 0) { sEnd[wave * 2] = fl; sEnd[wave * 2 + 1] = fr; }
-  }
-  // tiles of the wave: queries 32 qb, channels 32 qc of dq; keys 32 kb .. 32 + channels 32 kc .. of dk and dv
-  auto qb = [&](int j) { return MAPS == 2 && NT == 2 ? 2 * j + half : NC == 1 ? wave : wave >> 1; };
-  auto qc = [&](int j) { return MAPS == 2 && NT == 2 ? w4 : NC == 1 ? 0 : NT * (wave & 1) + j; };
-  const int kblk = NC == 1 ? wave : wave >> 1, kc = NC == 1 ? 0 : NT * (wave & 1);
-  const bool keys = 32 * kblk < a.Sk && kblk < 4;
-  f32x16 dq[NT], dk[NT], dv[NT];
-#pragma unroll
-  for (int j = 0; j < NT; j++) { zero(dq[j]); zero(dk[j]); zero(dv[j]); }
-  // products over `n` queries: the left operand's channels `c`, the right one's keys, both transposed; chunks of 16, the next one's fragments on their
-  // way under the MFMAs of the current one
-  auto products = [&](f32x16 (&acc)[NT], unsigned l0, unsigned l1, int lrow, int c, unsigned r0, unsigned r1, int n) {
-    const int n16 = (n + 15) / 16;
-    auto load = [&](int i, s16x8& fb, s16x8 (&fa)[NT]) {
-      fb = col_frag(r0 + i * 4096, r1 + i * 4096, kblk, 0);
-#pragma unroll
-      for (int j = 0; j < NT; j++) fa[j] = col_frag(l0 + i * lrow, l1 + i * lrow, c + j, 0);
-    };
-    auto mul = [&](const s16x8& fb, const s16x8 (&fa)[NT]) {
-#pragma unroll
-      for (int j = 0; j < NT; j++) acc[j] = mma<HALF>(fa[j], fb, acc[j]);
-    };
-    s16x8 fb0, fb1, fa0[NT], fa1[NT];
-    load(0, fb0, fa0);
+    // ---- dv: P of RP queries at a time
 #pragma unroll 1
-    for (int i = 0; i < n16; i += 2) {
-      load(min(i + 1, n16 - 1), fb1, fa1);
-      fence();
-      mul(fb0, fa0);
-      fence();
-      load(min(i + 2, n16 - 1), fb0, fa0);
-      fence();
-      if (i + 1 < n16) mul(fb1, fa1);
+    for (int qr = 0; qr < a.Sq; qr += RP) {
+      __syncthreads();                                       // k, or the last round's P, is read
+      if (live && q0 >= qr && q0 < qr + RP) put(sK, pp, q0 - qr + l31);
+      __syncthreads();
+      if (keys) {
+        const unsigned oa = lds_at(sO) + qr * DV * 2;
+        products(dv, opaque(oa + ooff0), opaque(oa + ooff1), 32 * DV, kc, opaque(lds_at(sK) + xoff0), opaque(lds_at(sK) + xoff1), min(RP, a.Sq - qr));
+      }
     }
-  };
-  auto put = [&](bf16_t* tile, const unsigned (&x)[2][8], int row) {
+    __syncthreads();                                         // every tile is read: the next head's arrive under the stores
+    asm volatile("" ::"v"(touched[0]), "v"(touched[1]));
+    if (more) request(b_next, h_next, opaque(lane));
+    if constexpr (BIAS) {
+      if (tid < a.gw) {                                      // bias gradient: the waves' sums by position, in wave order
+        const int rel = a.glo + tid;
+        const int far = rel == a.R ? 1 : rel == -a.R ? 0 : -1;
+        float x = 0.f;
 #pragma unroll
-    for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-      for (int j = 0; j < 4; j++) *(u32x2*)(tile + Tile<128>::off(row, key0 + 32 * kb + 8 * j + 4 * g)) = (u32x2){x[kb][2 * j], x[kb][2 * j + 1]};
-  };
-  // ---- dq and dk: dS of RS queries at a time
-#pragma unroll 1
-  for (int qr = 0; qr < a.Sq; qr += RS) {
-    if (qr || DV == 32) __syncthreads();                   // the last round's dS, or the diagonals, are read (v: all waves have met in the row sums since)
-    if (live && q0 >= qr && q0 < qr + RS) {
-#pragma unroll
-      for (int m = 0; m < MAPS; m++) put(sS + m * RS * 128, pd[m], q0 - qr + l31);
+        for (int w = 0; w < 8; w++) {                        // (column 95 of a wave's positions stays 0)
+          const int at = rel - (64 * (w >> 2) - 32 * (w & 3) - a.off - 31);
+          x += far >= 0 ? sEnd[w * 2 + far] : sRow[w * 96 + ((unsigned)at < 95u ? at : 95)];
+        }
+        a.part[((size_t)h * a.B + b) * a.gw + tid] = x;
+      }
     }
-    __syncthreads();
+    bf16_t* slab = (bf16_t*)(sX + wave * 768);
 #pragma unroll
     for (int j = 0; j < NT; j++) {
-      if (32 * qb(j) < qr || 32 * qb(j) >= min(qr + RS, a.Sq)) continue;
-      const int m = qc(j) / ND;
-      const unsigned ra = opaque(lds_at(sS) + m * RS * 256 + (32 * qb(j) - qr) * 256 + 2 * Tile<128>::off(l31, 4 * g));
-      const unsigned ta0 = opaque(lds_at(sK) + m * KT * 2 + toff0), ta1 = opaque(lds_at(sK) + m * KT * 2 + toff1);
-      const int c = qc(j) % ND;
-      // 16 keys a step, in the order in which a transposing read of k delivers them
-      auto kcol = [&](int i) { return col_frag(ta0, ta1, c, i * 32 * D); };
-      typedef const __attribute__((address_space(3))) s16x4* rptr;
-      auto dsrow = [&](int i) { return cat4(*(rptr)(uintptr_t)(ra ^ (32 * i)), *(rptr)(uintptr_t)(ra ^ (32 * i) ^ 16)); };
-      s16x8 fa[RA], fb[RA];
-      fill<8>(fa, kcol);
-      fill<8>(fb, dsrow);
-      fence();
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        dq[j] = mma<HALF>(fa[i % RA], fb[i % RA], dq[j]);
-        if (i + RA < 8) { fa[i % RA] = kcol(i + RA); fb[i % RA] = dsrow(i + RA); }
-        fence();
+      if (32 * qb(j) < a.Sq)
+        store_rows<HALF, 32>(&dq[j], a.scale, slab, lane, [=](int r) -> bf16_t* {
+          return 32 * qb(j) + r < a.Sq ? a.dq + (((size_t)b * a.Sq + 32 * qb(j) + r) * a.H + h) * DV + 32 * qc(j) : nullptr; });
+      if (keys) {
+        auto rows = [=](bf16_t* base) {
+          return [=](int r) -> bf16_t* { return 32 * kblk + r < a.Sk ? base + (((size_t)b * a.Sk + 32 * kblk + r) * a.H + h) * DV + 32 * (kc + j) : nullptr; };
+        };
+        store_rows<HALF, 32>(&dk[j], a.scale, slab, lane, rows(a.dk));
+        store_rows<HALF, 32>(&dv[j], 1.f, slab, lane, rows(a.dv));
       }
     }
-    if (keys) {
-      const int m = kc / ND;
-      const unsigned qa = lds_at(sQ) + m * KT * 2 + qr * D * 2;
-      products(dk, opaque(qa + toff0), opaque(qa + toff1), 32 * D, kc % ND, opaque(lds_at(sS) + xoff0 + m * RS * 256), opaque(lds_at(sS) + xoff1 + m * RS * 256), min(RS, a.Sq - qr));
-    }
-  }
-  // ---- dv: P of RP queries at a time
-#pragma unroll 1
-  for (int qr = 0; qr < a.Sq; qr += RP) {
-    __syncthreads();                                       // k, or the last round's P, is read
-    if (live && q0 >= qr && q0 < qr + RP) put(sK, pp, q0 - qr + l31);
-    __syncthreads();
-    if (keys) {
-      const unsigned oa = lds_at(sO) + qr * DV * 2;
-      products(dv, opaque(oa + ooff0), opaque(oa + ooff1), 32 * DV, kc, opaque(lds_at(sK) + xoff0), opaque(lds_at(sK) + xoff1), min(RP, a.Sq - qr));
-    }
-  }
-  __syncthreads();                                         // every tile is read: the next head's arrive under the stores
-  asm volatile("" ::"v"(touched[0]), "v"(touched[1]));
-  if (more) request(b_next, h_next, opaque(lane));
-  if constexpr (BIAS) {
-    if (tid < a.gw) {                                      // bias gradient: the waves' sums by position, in wave order
-      const int rel = a.glo + tid;
-      const int far = rel == a.R ? 1 : rel == -a.R ? 0 : -1;
-      float x = 0.f;
-#pragma unroll
-      for (int w = 0; w < 8; w++) {                        // (column 95 of a wave's positions stays 0)
-        const int at = rel - (64 * (w >> 2) - 32 * (w & 3) - a.off - 31);
-        x += far >= 0 ? sEnd[w * 2 + far] : sRow[w * 96 + ((unsigned)at < 95u ? at : 95)];
-      }
-      a.part[((size_t)h * a.B + b) * a.gw + tid] = x;
-    }
-  }
-  bf16_t* slab = (bf16_t*)(sX + wave * 768);
-#pragma unroll
-  for (int j = 0; j < NT; j++) {
-    if (32 * qb(j) < a.Sq)
-      store_rows<HALF, 32>(&dq[j], a.scale, slab, lane, [=](int r) -> bf16_t* {
-        return 32 * qb(j) + r < a.Sq ? a.dq + (((size_t)b * a.Sq + 32 * qb(j) + r) * a.H + h) * DV + 32 * qc(j) : nullptr; });
-    if (keys) {
-      auto rows = [=](bf16_t* base) {
-        return [=](int r) -> bf16_t* { return 32 * kblk + r < a.Sk ? base + (((size_t)b * a.Sk + 32 * kblk + r) * a.H + h) * DV + 32 * (kc + j) : nullptr; };
-      };
-      store_rows<HALF, 32>(&dk[j], a.scale, slab, lane, rows(a.dk));
-      store_rows<HALF, 32>(&dv[j], 1.f, slab, lane, rows(a.dv));
-    }
-  }
   }
 }
 
@@ -1583,18 +1587,36 @@ __global__ __launch_bounds__(256) void diag_sum_kernel(const float* part, long l
   __syncthreads();
   if (w == 0 && col < gw) out[((size_t)h * gridDim.y + blockIdx.y) * gw + col] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
 }
-// one workgroup per head: position sums in 64 bits and the positions' buckets to LDS, then a wave per bucket
-__global__ __launch_bounds__(1024) void bucket_sum_kernel(const float* sums, int chunks, int gw, int glo, const int* buckets, int R, int NB, int H, float* dtable) {
+// one workgroup per head: position sums in 64 bits (a position's rows shared by as many threads as the workgroup has to spare) and the positions' buckets
+// to LDS, then a wave per bucket
+__global__ __launch_bounds__(1024) void bucket_sum_kernel(const float* sums, int rows, int gw, int glo, const int* buckets, int R, int NB, int H, float* dtable) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem2[];
   double* sS = (double*)smem2;
-  int* sM = (int*)(sS + gw);
-  const int h = blockIdx.x, lane = threadIdx.x & 63;
-  for (int i = threadIdx.x; i < gw; i += 1024) {
+  double* sG = sS + gw;
+  int* sM = (int*)(sG + 1024);
+  const int h = blockIdx.x, lane = threadIdx.x & 63, wide = (gw + 63) & ~63, groups = wide < 1024 ? 1024 / wide : 1, grp = threadIdx.x / wide;
+  for (int i = threadIdx.x; i < gw; i += 1024) sM[i] = min(max(buckets[min(max(glo + i, -R), R) + R], 0), NB - 1);
+  if (groups > 1) {
+    const int i = threadIdx.x - grp * wide;
     double x = 0.;
+    if (grp < groups && i < gw) {
+#pragma unroll 16
+      for (int c = grp; c < rows; c += groups) x += (double)sums[((size_t)h * rows + c) * gw + i];
+    }
+    sG[threadIdx.x] = x;
+    __syncthreads();
+    if (threadIdx.x < gw) {
+      x = 0.;
+      for (int n = 0; n < groups; n++) x += sG[n * wide + threadIdx.x];
+      sS[threadIdx.x] = x;
+    }
+  } else {
+    for (int i = threadIdx.x; i < gw; i += 1024) {
+      double x = 0.;
 #pragma unroll 8
-    for (int c = 0; c < chunks; c++) x += (double)sums[((size_t)h * chunks + c) * gw + i];
-    sS[i] = x;
-    sM[i] = min(max(buckets[min(max(glo + i, -R), R) + R], 0), NB - 1);
+      for (int c = 0; c < rows; c++) x += (double)sums[((size_t)h * rows + c) * gw + i];
+      sS[i] = x;
+    }
   }
   __syncthreads();
   for (int bk = threadIdx.x >> 6; bk < NB; bk += 16) {
@@ -1688,7 +1710,7 @@ void reachable(const uvtg_attn_dims* d, int& glo, int& gw) {
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 // whole rows in one workgroup: one pass over the operands (256 x 107, 8 heads of 128: 117 us against 221 us of the two passes)
 bool short_rows(const uvtg_attn_dims* d) { return d->Sq <= 128 && d->Sk <= 128 && d->H == d->Hkv; }
-struct BwdWs { size_t rvec, part, sums, total; long long rows; int chunk, chunks; };
+struct BwdWs { size_t rvec, part, sums, total; long long rows; int chunk, chunks, direct; };
 BwdWs bwd_ws(const uvtg_attn_dims* d, int maps) {
   BwdWs w;
   w.rvec = 0;
@@ -1700,12 +1722,14 @@ BwdWs bwd_ws(const uvtg_attn_dims* d, int maps) {
     w.rows = short_rows(d) ? d->B : (long long)d->B * ((d->Sk + 31) / 32) * 2;
     w.chunk = w.rows > 64 * 128 ? (int)((w.rows + 63) / 64) : 128;
     w.chunks = (int)((w.rows + w.chunk - 1) / w.chunk);
+    // few parts (at most 64 per thread of the second kernel): without the first one
+    w.direct = w.rows * ((gw + 63) & ~63) <= 64 * 1024;
     at += align256((size_t)d->H * w.rows * gw * 4);
     w.sums = at;
-    at += align256((size_t)d->H * w.chunks * gw * 4);
+    if (!w.direct) at += align256((size_t)d->H * w.chunks * gw * 4);
   } else {
     w.rows = (long long)d->B * ((d->Sq + 31) / 32);
-    w.chunk = w.chunks = 0;
+    w.chunk = w.chunks = w.direct = 0;
     at += align256((size_t)d->H * w.rows * 4);
     w.sums = at;
   }
@@ -1779,9 +1803,12 @@ template <bool HALF, int D, int MAPS> int run_bwd(const uvtg_attn_dims* d, MapAr
   if (!dsum) return 0;
   if (MAPS == 1) {
     float* sums = (float*)(ws + w.sums);
-    hipLaunchKernelGGL(diag_sum_kernel, dim3((a.gw + 63) / 64, w.chunks, d->H), dim3(256), 0, s, a.part, w.rows, a.gw, w.chunk, sums);
-    UVTG_CHECK_LAUNCH();
-    hipLaunchKernelGGL(bucket_sum_kernel, dim3(d->H), dim3(1024), (size_t)a.gw * 12, s, sums, w.chunks, a.gw, a.glo, a.buckets, a.R, a.NB, a.H, dsum);
+    if (!w.direct) {
+      hipLaunchKernelGGL(diag_sum_kernel, dim3((a.gw + 63) / 64, w.chunks, d->H), dim3(256), 0, s, a.part, w.rows, a.gw, w.chunk, sums);
+      UVTG_CHECK_LAUNCH();
+    }
+    hipLaunchKernelGGL(bucket_sum_kernel, dim3(d->H), dim3(1024), (size_t)a.gw * 12 + 1024 * 8, s, w.direct ? a.part : sums, w.direct ? (int)w.rows : w.chunks, a.gw, a.glo,
+                       a.buckets, a.R, a.NB, a.H, dsum);
   } else hipLaunchKernelGGL(lam_sum_kernel, dim3(d->H), dim3(256), 0, s, a.part, w.rows, dsum);
   UVTG_CHECK_LAUNCH();
   return 0;
