@@ -1572,7 +1572,7 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
 
 // ------------------------------------------------------------------------------------------------
 // bias table's gradient: part [H][B x 32-key blocks x 2][gw] -> sums over a chunk of rows -> sums over the positions of a bucket.  Fixed order.
-// 6 - 9 us and 5 - 6 us: 35 MB of parts for 24 x 601 keys, 12 heads, 801 positions.
+// 7 - 9 us and 6 us (9 us alone for 256 parts of 213 positions): 35 MB of parts for 24 x 601 keys, 12 heads, 801 positions.
 // ------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void diag_sum_kernel(const float* part, long long rows, int gw, int chunk, float* out) {
   __shared__ float red[4][64];
