@@ -72,7 +72,7 @@ def _apply(function, leaves, *args):
     o = function.apply(*args)
     if leaves:
         n = next(_numbers)
-        _nodes[n] = weakref.ref(o.grad_fn, lambda _: _nodes.pop(n, None))
+        _nodes[n] = weakref.ref(o.grad_fn, lambda _, nodes=_nodes: nodes.pop(n, None))
         for t in leaves:
             t._attention_graphs = [p for p in getattr(t, "_attention_graphs", ()) if p[0] in _nodes] + [(n, stream)]
     return o
