@@ -66,6 +66,11 @@ __device__ __forceinline__ float half_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
   return fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
 }
+// log2 of a number that is 1 but for roundings (or, for coarse statistics, is not)
+__device__ __forceinline__ float log2_near_1(float s) {
+  const float d = s - 1.f;
+  return fabsf(d) < 1e-3f ? d * LOG2E * fmaf(-0.5f, d, 1.f) : __builtin_amdgcn_logf(s);
+}
 __device__ __forceinline__ void zero(f32x16& x) {
 #pragma unroll
   for (int r = 0; r < 16; r++) x[r] = 0.f;
@@ -753,7 +758,9 @@ __global__ __launch_bounds__(256) void maps_join_kernel(const MapArgs a) {
 // ------------------------------------------------------------------------------------------------
 // backward, queries: dq and the row sums r_i = sum_j p_ij dp_ij.  One workgroup = 128 queries of one head, tiles as in the forward.
 // ds = p (dp - r) needs r before the first key: rowsum(dO o) gives it up to the rounding of o, which is enough for dq (16 bits), and the exact
-// fp32 sum falls out of the same registers (one FMA per element): the key kernel forms ds, the bias table's and lam's gradients from that.
+// fp32 sum falls out of the same registers (one FMA per element): the key kernel forms ds, the bias table's and lam's gradients from that.  Both are
+// divided by the row's sum of p, which is 1 up to the rounding of lse (1e-6): the ds of a row then add up to 0, where a bucket that holds nearly all of
+// a row would keep the difference and nothing else.
 // Row statistics leave as [B][H][64-query tile][MAPS][2][64] floats: log2 of the row sum (ROW_OFF for a row without one), r.
 // Bound as the forward: three products per pair of positions instead of two.  32 x 1232, 8 heads of 128: 312 us, 717 TF/s; causal 4 x 4096, 16 heads of
 // two maps of 64: 690 us, 598 TF/s.  (Exponentials placed under the MFMAs of dP by hand were 13 % slower.)
@@ -789,7 +796,7 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
   if (ntiles > 0) request(0, 0);
   if (ntiles > 1) request(1, 1);
   s16x8 qf[MAPS][NK], of[NV];
-  float L[MAPS], del[MAPS], racc[MAPS];
+  float L[MAPS], del[MAPS], racc[MAPS], psum[MAPS];
   const float lam = MAPS == 2 ? a.lam[h] : 0.f;
   {
     const size_t ro = (((size_t)b * a.Sq + qrow) * a.H + h) * DV + 8 * g;
@@ -800,7 +807,7 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
         qf[m][ks] = *(const s16x8*)(a.q + (long long)b * a.q_sb + (long long)qrow * a.q_ss + (long long)h * a.q_sh + m * a.q_sm + 16 * ks + 8 * g);
       const float l = a.lse_in[(((size_t)b * a.H + h) * MAPS + m) * a.Sq + qrow];
       L[m] = l == -INFINITY ? ROW_OFF : l * LOG2E;
-      del[m] = 0.f; racc[m] = 0.f;
+      del[m] = 0.f; racc[m] = 0.f; psum[m] = 0.f;
     }
 #pragma unroll
     for (int ks = 0; ks < NV; ks++) of[ks] = *(const s16x8*)(a.dO + ro + 16 * ks);
@@ -896,12 +903,15 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
           if (part) mask_scores(s[m], (unsigned)(mask >> (32 * kb)), (a.causal ? q_raw + a.off - key0 : 64) - 32 * kb, g, -INFINITY);
           const float e0 = cb - L[m];
           const float f = m == 0 ? 1.f : -lam;
+          float rb = 0.f, pb = 0.f;                        // (sums of a block, then of blocks: a long row's last terms meet no long sum)
 #pragma unroll
           for (int r = 0; r < 16; r += 2) {
             const float p0 = prob(fmaf(s[m][r], cc, e0)), p1 = prob(fmaf(s[m][r + 1], cc, e0));
-            racc[m] = fmaf(p0, dp[r], racc[m]); racc[m] = fmaf(p1, dp[r + 1], racc[m]);
+            rb = fmaf(p0, dp[r], rb); rb = fmaf(p1, dp[r + 1], rb);
+            pb += p0 + p1;
             pk[m][r / 2] = pack2<HALF>((m ? f * p0 : p0) * (dp[r] - del[m]), (m ? f * p1 : p1) * (dp[r + 1] - del[m]));
           }
+          racc[m] += rb; psum[m] += pb;
         }
         fence();
         run<NP>(fa, kcol, [&](int i, s16x8 x) {
@@ -917,9 +927,9 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
   if (!live) return;
 #pragma unroll
   for (int m = 0; m < MAPS; m++) {
-    const float r = half_sum(racc[m]);
+    const float s = half_sum(psum[m]), r = s > 0.f ? half_sum(racc[m]) / s : 0.f;
     float* st = a.rvec + ((((size_t)b * a.H + h) * ((a.Sq + 63) / 64) + q0 / 64) * MAPS + m) * 128 + (q0 & 32) + l31;
-    st[g * 64] = g ? r : q_raw < a.Sq ? L[m] : ROW_OFF;
+    st[g * 64] = g ? r : q_raw < a.Sq && s > 0.f ? L[m] + log2_near_1(s) : ROW_OFF;
     if (MAPS == 2 && m == MAPS - 1) {                      // lam's gradient: the wave's 32 rows, [H][B][32-row block]
       const float w = wave_sum_dpp(g == 0 && q_raw < a.Sq ? r : 0.f);
       const int n32 = (a.Sq + 31) / 32;
@@ -1244,8 +1254,8 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
   bf16_t* sV = sK + VT;                                    // [128][DV]
   bf16_t* sQ = sV + VT;                                    // [MAPS][128][D]
   bf16_t* sO = sQ + VT;                                    // [128][DV]
-  float* sR = (float*)(sO + VT);                           // [2 halves][MAPS][128] row sums
-  float* sX = sR + 2 * MAPS * 128;                         // [8 waves][768]: skewed score gradients as in the key kernel, then store slabs
+  float* sR = (float*)(sO + VT);                           // [2 halves][MAPS][2][128] row sums of p dp and of p
+  float* sX = sR + 4 * MAPS * 128;                         // [8 waves][768]: skewed score gradients as in the key kernel, then store slabs
   float* sRow = sX + 8 * 768;                              // [8 waves][96] bias gradient of the wave's 95 positions
   float* sEnd = sRow + (BIAS ? 8 * 96 : 0);                // [8 waves][2] its sums at and behind -R, +R
   float* sB = sEnd + (BIAS ? 64 : 0);                      // [256] bias by position
@@ -1327,9 +1337,9 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
     const int xoff0 = 2 * Tile<128>::off(4 * g + (i16 >> 2), 16 * qd + 4 * (i16 & 3)), xoff1 = 2 * Tile<128>::rows8(xoff0 / 2);
     // ---- scores of 32 queries x 2 blocks of 32 keys: p of every map, dP, and this half's row sums
     f32x16 p[MAPS][2], dp[2];
-    float rs[MAPS];
+    float rs[MAPS], ps[MAPS];
 #pragma unroll
-    for (int m = 0; m < MAPS; m++) { rs[m] = 0.f; zero(p[m][0]); zero(p[m][1]); }
+    for (int m = 0; m < MAPS; m++) { rs[m] = ps[m] = 0.f; zero(p[m][0]); zero(p[m][1]); }
     zero(dp[0]); zero(dp[1]);
     bool on[2];                                              // the block has a (query, key) pair
 #pragma unroll
@@ -1370,18 +1380,24 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
           for (int r = 0; r < 16; r++) {
             p[m][kb][r] = prob(fmaf(p[m][kb][r], cc, -L[m]));
             rs[m] = fmaf(p[m][kb][r], dp[kb][r], rs[m]);
+            ps[m] += p[m][kb][r];
           }
         }
       }
     }
 #pragma unroll
     for (int m = 0; m < MAPS; m++) {
-      rs[m] = half_sum(rs[m]);
-      if (g == 0) sR[(half * MAPS + m) * 128 + q_raw] = rs[m];
+      rs[m] = half_sum(rs[m]); ps[m] = half_sum(ps[m]);
+      sR[((half * MAPS + m) * 2 + g) * 128 + q_raw] = g ? ps[m] : rs[m];
     }
     __syncthreads();
 #pragma unroll
-    for (int m = 0; m < MAPS; m++) rs[m] = sR[m * 128 + q_raw] + sR[(MAPS + m) * 128 + q_raw];
+    for (int m = 0; m < MAPS; m++) {                         // (divided by the row's sum of p, as in the query kernel)
+      const float x = sR[(2 * m + 1) * 128 + q_raw] + sR[(2 * (MAPS + m) + 1) * 128 + q_raw];
+      ps[m] = x > 0.f ? 1.f / x : 0.f;
+      rs[m] = (sR[2 * m * 128 + q_raw] + sR[2 * (MAPS + m) * 128 + q_raw]) * ps[m];
+      if (m) ps[m] *= -lam;
+    }
     if (MAPS == 2 && half == 0 && live) {                    // lam's gradient: the wave's 32 rows, [H][B][32-row block]
       const float w = wave_sum_dpp(g == 0 && q_raw < a.Sq ? rs[MAPS - 1] : 0.f);
       if (lane == 0) a.part[((size_t)h * a.B + b) * ((a.Sq + 31) / 32) + w4] = w;
@@ -1403,10 +1419,10 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
         float x[2], d[MAPS][2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-          x[u] = p[0][kb][r + u];
+          x[u] = p[0][kb][r + u] * ps[0];
           d[0][u] = x[u] * (dp[kb][r + u] - rs[0]);
           if constexpr (MAPS == 2) {
-            const float y = -lam * p[MAPS - 1][kb][r + u];
+            const float y = ps[MAPS - 1] * p[MAPS - 1][kb][r + u];
             d[MAPS - 1][u] = y * (dp[kb][r + u] - rs[MAPS - 1]);
             x[u] += y;
           }
@@ -1787,7 +1803,7 @@ template <bool HALF, int D, int MAPS> int run_bwd(const uvtg_attn_dims* d, MapAr
   a.part = (float*)(ws + w.part);
   if (MAPS == 1) reachable(d, a.glo, a.gw);
   if (short_rows(d)) {
-    constexpr size_t lds = 4 * 128 * DV * 2 + 2 * MAPS * 512 + DIAG_BYTES + (MAPS == 1 ? 8 * 96 * 4 + 256 + 1024 : 0) + (DV == 64 ? MAPS * 128 * 256 : 0);
+    constexpr size_t lds = 4 * 128 * DV * 2 + 4 * MAPS * 512 + DIAG_BYTES + (MAPS == 1 ? 8 * 96 * 4 + 256 + 1024 : 0) + (DV == 64 ? MAPS * 128 * 256 : 0);
     // workgroups that stay: one per CU, two where registers allow
     const int wgs = DV == 32 ? 512 : 256;
     hipLaunchKernelGGL((maps_bwd_short_kernel<HALF, D, MAPS>), dim3(d->H * d->B < wgs ? d->H * d->B : wgs), dim3(512), lds, s, a);
