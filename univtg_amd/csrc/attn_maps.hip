@@ -71,6 +71,10 @@ __device__ __forceinline__ float log2_near_1(float s) {
   const float d = s - 1.f;
   return fabsf(d) < 1e-3f ? d * LOG2E * fmaf(-0.5f, d, 1.f) : __builtin_amdgcn_logf(s);
 }
+// The matrix pipe's sums are off by a little to one side (measured: dP about 1e-8 of its terms low).  lam's gradient adds one such sum per row of all
+// queries, which cancel, and so would keep it: half of dP's products are formed with the other sign, where the error has it too (two maps of 32,
+// 4 x 3869 queries over 2657 keys, fp16: 1.1e-5 of dlam before, under 1e-6 with it).  ds does not feel a constant in dP.
+__device__ __forceinline__ s16x8 negated(s16x8 x) { return x ^ (short)0x8000; }
 __device__ __forceinline__ void zero(f32x16& x) {
 #pragma unroll
   for (int r = 0; r < 16; r++) x[r] = 0.f;
@@ -828,6 +832,10 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
     }
 #pragma unroll
     for (int m = 0; m < MAPS; m++) del[m] = half_sum(del[m]);
+    if constexpr (MAPS == 2) {
+#pragma unroll
+      for (int ks = NV / 4; ks < 3 * NV / 4; ks++) of[ks] = negated(of[ks]);
+    }
   }
   Masks masks(a, b, ntiles, sMask, wave, lane);
   masks.load();
@@ -880,6 +888,7 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
         fence();
         run<NS>(fa, kvrow, [&](int i, s16x8 x) {
           const int j = i < NV ? 0 : i - NV;
+          if (MAPS == 2 && (i == NV / 4 || i == 3 * NV / 4)) dp = -dp;
           if (i < NV) dp = mma<HALF>(x, of[i < NV ? i : 0], dp); else s[j / NK] = mma<HALF>(x, qf[j / NK][j % NK], s[j / NK]);
         });
         if (req && kb == 0) request(tn, buf ^ 1);
@@ -1352,6 +1361,10 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
         for (int ks = 0; ks < NK; ks++) qf[m][ks] = row_frag(lds_at(sQ + m * KT + q0 * D) + koff, ks, 0);
 #pragma unroll
       for (int ks = 0; ks < NV; ks++) of[ks] = row_frag(lds_at(sO + q0 * DV) + voff, ks, 0);
+      if constexpr (MAPS == 2) {
+#pragma unroll
+        for (int ks = NV / 4; ks < 3 * NV / 4; ks++) of[ks] = negated(of[ks]);
+      }
 #pragma unroll
       for (int kb = 0; kb < 2; kb++) {
         if (!on[kb]) continue;
@@ -1362,6 +1375,7 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
         fence();
         run<NV + MAPS * NK>(fa, kvrow, [&](int i, s16x8 x) {
           const int j = i < NV ? 0 : i - NV;
+          if (MAPS == 2 && (i == NV / 4 || i == 3 * NV / 4)) dp[kb] = -dp[kb];
           if (i < NV) dp[kb] = mma<HALF>(x, of[i < NV ? i : 0], dp[kb]); else p[j / NK][kb] = mma<HALF>(x, qf[j / NK][j % NK], p[j / NK][kb]);
         });
         const unsigned mk = (unsigned)(mask[half] >> (32 * kb));
