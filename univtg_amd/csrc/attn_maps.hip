@@ -766,8 +766,8 @@ __global__ __launch_bounds__(256) void maps_join_kernel(const MapArgs a) {
 // divided by the row's sum of p, which is 1 up to the rounding of lse (1e-6): the ds of a row then add up to 0, where a bucket that holds nearly all of
 // a row would keep the difference and nothing else.
 // Row statistics leave as [B][H][64-query tile][MAPS][2][64] floats: log2 of the row sum (ROW_OFF for a row without one), r.
-// Bound as the forward: three products per pair of positions instead of two.  32 x 1232, 8 heads of 128: 312 us, 717 TF/s; causal 4 x 4096, 16 heads of
-// two maps of 64: 690 us, 598 TF/s.  (Exponentials placed under the MFMAs of dP by hand were 13 % slower.)
+// Bound as the forward: three products per pair of positions instead of two.  32 x 1232, 8 heads of 128: 320 us, 700 TF/s; causal 4 x 4096, 16 heads of
+// two maps of 64: 720 us, 572 TF/s (of which the sums of p and dP's signs, for the precision of r: 3 - 5 %).  (Exponentials placed under the MFMAs of dP by hand were 13 % slower.)
 // ------------------------------------------------------------------------------------------------
 template <bool HALF, int D, int MAPS>
 __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
@@ -1249,7 +1249,7 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
 // that ds is formed from the exact row sums without a second pass.  dS and then P go through LDS in 16 bits to the products, whose 32 x 32 tiles of
 // dq, dk and dv the waves share evenly.  Workgroups stay and fetch their next head under the stores.
 // Bound by memory and by the phases' latency: q, k, v, dO in, dq, dk, dv out, 392 MB for 256 x 107 positions and 8 heads of 128: 77 us at the rate of a
-// copy, 117 us measured (221 us by the two passes of longer rows).
+// copy, 120 us measured (221 us by the two passes of longer rows).
 // ------------------------------------------------------------------------------------------------
 template <bool HALF, int D, int MAPS>
 __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_kernel(const MapArgs a) {
@@ -1738,7 +1738,7 @@ void reachable(const uvtg_attn_dims* d, int& glo, int& gw) {
   gw = cl((long long)d->Sk - 1 - d->q_offset) - glo + 1;
 }
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
-// whole rows in one workgroup: one pass over the operands (256 x 107, 8 heads of 128: 117 us against 221 us of the two passes)
+// whole rows in one workgroup: one pass over the operands (256 x 107, 8 heads of 128: 120 us against 221 us of the two passes)
 bool short_rows(const uvtg_attn_dims* d) { return d->Sq <= 128 && d->Sk <= 128 && d->H == d->Hkv; }
 struct BwdWs { size_t rvec, part, sums, total; long long rows; int chunk, chunks, direct; };
 BwdWs bwd_ws(const uvtg_attn_dims* d, int maps) {
