@@ -1,0 +1,108 @@
+"""What the attention cores' autograd layer relies on between a forward and a backward call.  Saved-tensor hooks (activation offloading, compression) may
+hand the backward call equal values in another layout than the forward call laid out.  On the CPU the library is a stand-in that notes its arguments."""
+import pytest
+import torch
+
+
+class Library:
+    """Takes every call, computes nothing, keeps the descriptor and the tensors behind the addresses."""
+    def __init__(self, monkeypatch):
+        from univtg_amd import _lib, ops
+        self.calls, self.tensors, at = [], {}, ops._at
+        monkeypatch.setattr(_lib, "load", lambda: self)
+        monkeypatch.setattr(ops, "_elsewhere", lambda t: False)
+        monkeypatch.setattr(ops, "_stream_of", lambda t: 0)
+        monkeypatch.setattr(ops, "_at", lambda t: None if t is None else self.tensors.setdefault(at(t), t).data_ptr())
+
+    def uvtg_attn_ws_bytes(self, d, maps, backward):
+        return 0
+
+    def __getattr__(self, name):
+        if not name.startswith("uvtg_"):
+            raise AttributeError(name)
+
+        def call(d, *args):
+            self.calls.append((name, {n: getattr(d, n) for n, _ in d._fields_}, [self.tensors.get(a) for a in args]))
+            return 0
+        return call
+
+
+@pytest.fixture
+def library(monkeypatch):
+    return Library(monkeypatch)
+
+
+def packed(op, B, S, H, D, dev, t=torch.bfloat16):
+    """q, k, v as views of one projection, which is how an encoder layer has them."""
+    g = torch.Generator(device=dev).manual_seed(4)
+    if op == "relpos":
+        return torch.randn(B, S, 3, H, D, generator=g, device=dev).to(t).unbind(2)
+    x = torch.randn(B, S, 3, 2 * H * D, generator=g, device=dev).to(t)
+    return [x[:, :, 0].unflatten(2, (H, 2, D)), x[:, :, 1].unflatten(2, (H, 2, D)), x[:, :, 2].unflatten(2, (H, 2 * D))]
+
+
+def weights(op, H, dev):
+    from univtg_amd import ops
+    if op == "relpos":
+        return torch.linspace(-1, 1, 8 * H, device=dev).view(8, H), ops.relpos_buckets(8, 20, device=dev)
+    return torch.linspace(0.1, 0.8, H, device=dev), None
+
+
+def attend(op, q, k, v, w, buckets, **opts):
+    from univtg_amd import attention
+    return attention.relpos_attention(q, k, v, w, buckets, **opts) if op == "relpos" else attention.diff_attention(q, k, v, w, **opts)
+
+
+RELAYOUTS = {
+    "dense": lambda t: t.clone(memory_format=torch.contiguous_format),                                   # what torch.autograd.graph.save_on_cpu returns
+    "unaligned": lambda t: torch.cat([t.reshape(-1)[:1], t.reshape(-1)])[1:].view(t.shape),
+    "axes": lambda t: t.permute(*range(t.dim())[::-1]).contiguous().permute(*range(t.dim())[::-1]),
+    "halves": lambda t: torch.stack([t, t], 0)[0] if t.dim() < 2 else torch.stack([t, t], 1)[:, 0],      # samples twice as far apart
+    "strided": lambda t: torch.stack([t, t], -1)[..., 0],
+}
+
+
+@pytest.mark.parametrize("how", RELAYOUTS)
+@pytest.mark.parametrize("op", ["relpos", "diff"])
+def test_backward_describes_the_operands_it_is_given(library, op, how):
+    B, S, H, D = 2, 10, 4, 32
+    q, k, v = packed(op, B, S, H, D, "cpu")
+    w, bk = weights(op, H, "cpu")
+    kvalid = (torch.arange(S) < 7).to(torch.uint8).expand(B, S)
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v, w)]
+    assert leaves[0].stride(1) == 3 * H * D * (2 if op == "diff" else 1)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: RELAYOUTS[how](t.detach())):
+        o = attend(op, *leaves, bk, kvalid=kvalid)
+        o.backward(torch.ones_like(o))
+    (_, _, fwd), (name, d, bwd) = library.calls
+    assert name.endswith("attention_bwd")
+    n = 6 if op == "relpos" else 5                           # q, k, v, table and buckets or lam, kvalid
+    for a, b in zip(fwd[:n], bwd[:n]):
+        assert torch.equal(a, b)
+    for x, prefix, axes in ((bwd[0], "q", "bshm"), (bwd[1], "k", "bshm"), (bwd[2], "v", "bsh")):
+        assert x.data_ptr() % 16 == 0 and x.stride(-1) == 1
+        for axis, stride in zip(axes, x.stride()[:-1]):
+            assert d[f"{prefix}_s{axis}"] == stride and stride % 8 == 0, (prefix, axis)
+    assert bwd[n - 1].stride() == (d["kvalid_sb"], 1)
+    saved = bwd[3: n - 1] + bwd[n: n + (3 if op == "relpos" else 4)]                                     # weights; o, (o2,) lse, dO
+    assert all(x.is_contiguous() and x.data_ptr() % 4 == 0 for x in saved) and all(x.data_ptr() % 16 == 0 for x in saved if x.dim() == 4 and x.dtype == q.dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", RELAYOUTS)
+@pytest.mark.parametrize("op", ["relpos", "diff"])
+def test_gradients_do_not_depend_on_saved_tensor_hooks(op, how):
+    """Short rows and longer ones (one kernel, two passes), packed views, a mask shared over the batch."""
+    for S, H, D in ((70, 4, 32), (150, 2, 64)):
+        q, k, v = packed(op, 2, S, H, D, "cuda")
+        w, bk = weights(op, H, "cuda")
+        kvalid = (torch.arange(S, device="cuda") < S - 9).to(torch.uint8).expand(2, S)
+        leaves = [x.detach().requires_grad_(True) for x in (q, k, v, w)]
+        do = torch.randn(2, S, H, v.shape[-1], device="cuda").to(q.dtype)
+        want = torch.autograd.grad(attend(op, *leaves, bk, kvalid=kvalid), leaves, do)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: RELAYOUTS[how](t.detach())):
+            got = torch.autograd.grad(attend(op, *leaves, bk, kvalid=kvalid), leaves, do)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        with torch.autograd.graph.save_on_cpu():
+            got = torch.autograd.grad(attend(op, *leaves, bk, kvalid=kvalid), leaves, do)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

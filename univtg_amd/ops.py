@@ -278,7 +278,17 @@ def _attn_call(name, maps, q, k, v, kvalid, q_offset, causal, scale):
         raise ValueError(f"{name}: q_offset must lie within +-2^28, got {q_offset}")
     d = _lib.AttnDims(0, _ATTN_TYPES[dtype], B, H, Hkv, D, Sq, Sk, 1 if causal else 0, int(q_offset), D ** -0.5 if scale is None else float(scale), 0, 0,
                       qs[0], qs[1], qs[2], qs[3] if maps == 2 else 0, ks[0], ks[1], ks[2], ks[3] if maps == 2 else 0, vs[0], vs[1], vs[2], mask_sb)
+    d.layout = (dev, qs, ks, vs, None if kvalid is None else kvalid.stride())
     return d, q, k, v, kvalid
+
+
+def _attn_saved_operands(name, maps, d, q, k, v, kvalid):
+    """What _attn_call returned, for operands that went through autograd's hands since: saved-tensor hooks (offloading, compression) return equal values
+    in whatever layout, which is then checked, laid out and described anew."""
+    if (q.device, q.stride(), k.stride(), v.stride(), None if kvalid is None else kvalid.stride()) == d.layout and k.device == v.device == q.device and \
+            (kvalid is None or kvalid.device == q.device) and not (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        return d, q, k, v, kvalid
+    return _attn_call(name, maps, q, k, v, kvalid, d.q_offset, d.causal, d.scale)
 
 
 def _attn_ws(lib, d, maps, backward, like):
@@ -331,7 +341,10 @@ def _relpos_fwd(q, k, v, table, buckets, kvalid, q_offset, causal, scale):
 
 def _relpos_bwd(do, d, q, k, v, table, buckets, kvalid, o, lse, need_dtable):
     lib = _lib.load()
-    do = _attn_saved("relpos_attention_bwd", do, q, "do")
+    d, q, k, v, kvalid = _attn_saved_operands("relpos_attention_bwd", 1, d, q, k, v, kvalid)
+    table, buckets = _relpos_operands(d, q, table, buckets)
+    do, o = (_attn_saved("relpos_attention_bwd", t, q, w) for t, w in ((do, "do"), (o, "o")))
+    lse = _attn_saved("relpos_attention_bwd", lse, q, "lse", torch.float32)
     dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     dtable = table.new_empty(table.shape) if need_dtable else None
     ws = _attn_ws(lib, d, 1, 1, q)
@@ -357,11 +370,9 @@ def relpos_attention_bwd(do, q, k, v, table, buckets, o, lse, kvalid=None, q_off
         with torch.cuda.device(q.device):
             return relpos_attention_bwd(do, q, k, v, table, buckets, o, lse, kvalid, q_offset, causal, scale, need_dtable)
     d, q, k, v, kvalid = _attn_call("relpos_attention", 1, q, k, v, kvalid, q_offset, causal, scale)
-    table, buckets = _relpos_operands(d, q, table, buckets)
     if do.shape != (d.B, d.Sq, d.H, d.D) or o.shape != do.shape or lse.shape != (d.B, d.H, d.Sq):
         raise ValueError("relpos_attention_bwd: do and o must be [B, Sq, H, D], lse [B, H, Sq]")
-    return _relpos_bwd(do, d, q, k, v, table, buckets, kvalid, _attn_saved("relpos_attention_bwd", o, q, "o"),
-                       _attn_saved("relpos_attention_bwd", lse, q, "lse", torch.float32), need_dtable)
+    return _relpos_bwd(do, d, q, k, v, table, buckets, kvalid, o, lse, need_dtable)
 
 
 def _lam_operand(d, q, lam):
@@ -385,7 +396,10 @@ def _diff_fwd(q, k, v, lam, kvalid, q_offset, causal, scale, need_o2):
 
 def _diff_bwd(do, d, q, k, v, lam, kvalid, o, o2, lse, need_dlam):
     lib = _lib.load()
-    do = _attn_saved("diff_attention_bwd", do, q, "do")
+    d, q, k, v, kvalid = _attn_saved_operands("diff_attention_bwd", 2, d, q, k, v, kvalid)
+    lam = _lam_operand(d, q, lam)
+    do, o, o2 = (_attn_saved("diff_attention_bwd", t, q, w) for t, w in ((do, "do"), (o, "o"), (o2, "o2")))
+    lse = _attn_saved("diff_attention_bwd", lse, q, "lse", torch.float32)
     dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     dlam = lam.new_empty(d.H) if need_dlam else None
     ws = _attn_ws(lib, d, 2, 1, q)
@@ -411,8 +425,6 @@ def diff_attention_bwd(do, q, k, v, lam, o, o2, lse, kvalid=None, q_offset=0, ca
         with torch.cuda.device(q.device):
             return diff_attention_bwd(do, q, k, v, lam, o, o2, lse, kvalid, q_offset, causal, scale, need_dlam)
     d, q, k, v, kvalid = _attn_call("diff_attention", 2, q, k, v, kvalid, q_offset, causal, scale)
-    lam = _lam_operand(d, q, lam)
     if do.shape != (d.B, d.Sq, d.H, 2 * d.D) or o.shape != do.shape or o2.shape != do.shape or lse.shape != (d.B, d.H, 2, d.Sq):
         raise ValueError("diff_attention_bwd: do, o and o2 must be [B, Sq, H, 2 D], lse [B, H, 2, Sq]")
-    o, o2 = (_attn_saved("diff_attention_bwd", t, q, w) for t, w in ((o, "o"), (o2, "o2")))
-    return _diff_bwd(do, d, q, k, v, lam, kvalid, o, o2, _attn_saved("diff_attention_bwd", lse, q, "lse", torch.float32), need_dlam)
+    return _diff_bwd(do, d, q, k, v, lam, kvalid, o, o2, lse, need_dlam)
