@@ -258,7 +258,8 @@ int uvtg_sine_position(const float* vid_mask, const float* txt_mask, const float
  * o, o2, dO, dq, dk, dv are contiguous [B, S, heads, (2,) channels] of the same type; lse [B, H, (2,) Sq] fp32 is the natural logarithm of the
  * row sums.  table [n_buckets, H], lam [H], dtable and dlam are fp32; buckets [2 reach + 1] int32 (entries outside 0 .. n_buckets - 1 are
  * read as the nearest one inside).  kvalid [B, Sk] uint8, rows kvalid_sb bytes apart, 0 = the key is masked (its k / v rows may hold anything);
- * NULL = no mask.  causal: query i sees keys j <= i + q_offset.  A table entry of -inf, or below -2.3e38, takes its positions out of the row.
+ * NULL = no mask.  causal: query i sees keys j <= i + q_offset, and rows of keys that no query sees may hold anything, too (a cache with room
+ * behind its newest position).  A table entry of -inf, or below -2.3e38, takes its positions out of the row.
  * A row that sees no key: o = 0, lse = -inf, no gradient.
  * Scores, statistics and sums are fp32; probabilities and score gradients are rounded to the operands' type for the products with v, k, q, dO.
  * The backward pass forms the probabilities from lse: their relative error grows with a row's largest score, 2^-23 of it, and none exceeds 1.

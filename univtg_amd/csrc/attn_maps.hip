@@ -32,6 +32,7 @@ struct MapArgs {
   const float* lse_in;
   long long q_sb, q_ss, q_sh, q_sm, k_sb, k_ss, k_sh, k_sm, v_sb, v_ss, v_sh, mask_sb;     // element strides
   int B, H, Hkv, G, Sq, Sk, NB, R, off, causal;
+  int seen;                                     // keys from here on are seen by no query (causal), so that their rows may hold anything: masked, as by kvalid
   float scale, c;                               // c = scale log2(e)
   int hb, nsplit;                               // split kernel: heads packed into a row block, key ranges
   int glo, gw;                                  // bias gradient: first reachable relative position, number of them
@@ -203,7 +204,7 @@ struct Masks {
   unsigned long long* words;
   int w0, Sk, ntiles, wave, lane;
   __device__ __forceinline__ Masks(const MapArgs& a, int b, int ntiles_, unsigned long long* words_, int wave_, int lane_)
-      : kv(a.kvalid ? a.kvalid + (size_t)b * a.mask_sb : nullptr), words(words_), w0(0), Sk(a.Sk), ntiles(ntiles_), wave(wave_), lane(lane_) {}
+      : kv(a.kvalid ? a.kvalid + (size_t)b * a.mask_sb : nullptr), words(words_), w0(0), Sk(a.seen), ntiles(ntiles_), wave(wave_), lane(lane_) {}
   __device__ __forceinline__ void load() {       // (a barrier before and behind)
     if (!kv) return;
     const int n = min(WIN, ntiles - w0);
@@ -567,7 +568,7 @@ __global__ __launch_bounds__(256, 2) void maps_fwd_split_kernel(const MapArgs a)
 #pragma unroll 4
     for (int t = 2 * wave; t < wn; t += 8) {               // two 32-key masks per ballot
       const int key = (w0 + t) * 32 + lane;
-      const unsigned long long m = __builtin_amdgcn_ballot_w64(key < a.Sk && (!kv || kv[key] != 0));
+      const unsigned long long m = __builtin_amdgcn_ballot_w64(key < a.seen && (!kv || kv[key] != 0));
       if (lane == 0) { sMask[t] = (unsigned)m; sMask[t + 1] = (unsigned)(m >> 32); }
     }
     __syncthreads();
@@ -997,7 +998,7 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
   };
   request_two();
   // lane = key in every product: whatever a masked key's row holds reaches only its own gradient rows, which are zeroed before the store
-  const bool kok = key < a.Sk && (!a.kvalid || a.kvalid[(size_t)b * a.mask_sb + krow] != 0);
+  const bool kok = key < a.seen && (!a.kvalid || a.kvalid[(size_t)b * a.mask_sb + krow] != 0);
   const bf16_t* vb_ = a.v + (long long)b * a.v_sb + (long long)kh * a.v_sh;
   s16x8 kf[MAPS][NK], vf[VLDS ? 1 : NV];
 #pragma unroll
@@ -1307,7 +1308,7 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       const int key = 64 * i + lane;
-      mask[i] = __builtin_amdgcn_ballot_w64(key < a.Sk && (!kv || kv[min(key, a.Sk - 1)] != 0));
+      mask[i] = __builtin_amdgcn_ballot_w64(key < a.seen && (!kv || kv[min(key, a.Sk - 1)] != 0));
     }
     const int rlo = -(a.Sq - 1) - a.off, rhi = 127 - a.off;  // positions of the workgroup
     float* row = sRow + wave * 96;
@@ -1774,7 +1775,7 @@ MapArgs map_args(const uvtg_attn_dims* d) {
   a.k_sb = d->k_sb; a.k_ss = d->k_ss; a.k_sh = d->k_sh; a.k_sm = d->k_sm;
   a.v_sb = d->v_sb; a.v_ss = d->v_ss; a.v_sh = d->v_sh; a.mask_sb = d->kvalid_sb;
   a.B = d->B; a.H = d->H; a.Hkv = d->Hkv; a.G = d->H / d->Hkv; a.Sq = d->Sq; a.Sk = d->Sk; a.NB = d->n_buckets; a.R = d->reach;
-  a.off = d->q_offset; a.causal = d->causal != 0; a.scale = d->scale; a.c = d->scale * LOG2E;
+  a.off = d->q_offset; a.causal = d->causal != 0; a.seen = a.causal ? max(0, min(d->Sk, d->Sq + d->q_offset)) : d->Sk; a.scale = d->scale; a.c = d->scale * LOG2E;
   return a;
 }
 

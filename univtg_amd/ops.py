@@ -356,7 +356,7 @@ def _relpos_bwd(do, d, q, k, v, table, buckets, kvalid, o, lse, need_dtable):
 def relpos_attention_fwd(q, k, v, table, buckets, kvalid=None, q_offset=0, causal=False, scale=None):
     """softmax(scale q k^T + table[buckets[clamp(j - i - q_offset)], h]) v: q [B, Sq, H, D], k and v [B, Sk, Hkv, D] (bf16 or fp16, D 32 / 64 / 128,
     any strides), table [n_buckets, H] fp32, buckets int32 [2 reach + 1] (relpos_buckets), kvalid [B, Sk] uint8 / bool (0 = masked key).  causal:
-    query i sees keys up to i + q_offset.  A table entry of -inf takes its positions out of the row.  scale defaults to D ** -0.5.  Returns o
+    query i sees keys up to i + q_offset; k and v rows that are masked, or behind what any query sees, may hold anything.  A table entry of -inf takes its positions out of the row.  scale defaults to D ** -0.5.  Returns o
     [B, Sq, H, D] and lse [B, H, Sq] (fp32); a row that sees no key is 0 with lse -inf."""
     if _elsewhere(q):
         with torch.cuda.device(q.device):
