@@ -261,6 +261,7 @@ int uvtg_sine_position(const float* vid_mask, const float* txt_mask, const float
  * NULL = no mask.  causal: query i sees keys j <= i + q_offset, and rows of keys that no query sees may hold anything, too (a cache with room
  * behind its newest position).  A table entry of -inf, or below -2.3e38, takes its positions out of the row.
  * A row that sees no key: o = 0, lse = -inf, no gradient.
+ * NaN stays visible: a row with a NaN score has it in o, lse, dq, the unmasked keys' dk and dv, dtable and dlam; masked keys' dk and dv are 0.
  * Scores, statistics and sums are fp32; probabilities and score gradients are rounded to the operands' type for the products with v, k, q, dO.
  * The backward pass forms the probabilities from lse: their relative error grows with a row's largest score, 2^-23 of it, and none exceeds 1.
  * Results are bit-reproducible for a given set of dims (no floating-point atomics on memory, fixed orders of summation).

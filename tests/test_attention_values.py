@@ -1,4 +1,4 @@
-"""Values that the attention cores meet at the edges: rows of a cache that no query sees.  The formulas in 64 bits and their tolerances are those of
+"""Values that the attention cores meet at the edges: NaN and infinities that are not masked, rows of a cache that no query sees.  The formulas in 64 bits and their tolerances are those of
 test_attention_maps."""
 import math
 
@@ -30,3 +30,52 @@ def test_keys_that_no_query_sees_may_hold_anything(op, D, Sq, Sk, seen):
                 got = run(op, q, k2, v2, w, bk, do, **opts)
                 assert all(torch.equal(got[n], want[n]) for n in got), x
                 assert not got["dk"][:, seen:].any() and not got["dv"][:, seen:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq, Sk, H, Hkv", [(70, 100, 2, 2), (70, 100, 4, 2), (150, 201, 2, 2), (5, 700, 4, 2)])
+@pytest.mark.parametrize("what", ["q", "k", "v", "do"])
+@pytest.mark.parametrize("op, D", OPS)
+def test_nan_and_infinity_reach_what_depends_on_them(op, D, what, Sq, Sk, H, Hkv):
+    """One in a query, an unmasked key, a value or an output gradient: none of what the formula makes of it comes out finite, in either backward form; masked
+    keys' gradients are zeros, and what does not depend on it keeps its bits."""
+    q, k, v, w, bk, do = make(op, torch.bfloat16, 2, H, Hkv, D, Sq, Sk, seed=31, buckets=8, reach=40)
+    kv = mask("holes", 2, Sk)
+    kv[:, 3] = 1
+    b, h, i, j, R = 1, 1, Sq // 2, 3, 40
+    kh = h * Hkv // H
+    valid = kv[b] != 0
+    heads = [h] if what in ("q", "do") else [x for x in range(H) if x * Hkv // H == kh]
+    want = run(op, q, k, v, w, bk, do, kvalid=kv)
+    for value in (math.nan, math.inf):
+        for m in (0, 1) if op == "diff" and what in ("q", "k") else (0,):
+            x = dict(q=q, k=k, v=v, do=do)
+            at = (b, i, h) if what in ("q", "do") else (b, j, kh)
+            x[what] = _spoil(x[what], at + ((m, 5) if x[what].dim() == 5 else (5,)), value)
+            got = run(op, x["q"], x["k"], x["v"], w, bk, x["do"], kvalid=kv)
+            bad = {n: ~y.isfinite() for n, y in got.items()}
+            rows = torch.ones(Sq, dtype=torch.bool, device="cuda") if what in ("k", "v") else torch.arange(Sq, device="cuda") == i
+            for hd in heads:
+                lost = rows                                  # rows without a finite score map: a key of +inf takes all of a row, one of -inf leaves it
+                if what == "k" and value == math.inf:
+                    lost = rows & ((q[b, :, hd, m, 5] if op == "diff" else q[b, :, hd, 5]) > 0)
+                assert bool(bad["dq"][b, :, hd].flatten(1).any(1)[lost].all()) and not bool(bad["dq"][b, :, hd][~rows].any())
+                if what != "do":
+                    assert bool(bad["o"][b, :, hd].any(1)[lost].all()) and not bool(bad["o"][b, :, hd][~rows].any())
+                if what in ("q", "k"):
+                    assert bool((got["lse"][b, hd, m] if op == "diff" else got["lse"][b, hd]).isnan()[lost].all())
+                if op == "relpos":
+                    rel = (torch.arange(Sk, device="cuda")[valid][None] - torch.arange(Sq, device="cuda")[lost][:, None]).clamp(-R, R) + R
+                    assert bool(bad["dw"][bk.long()[rel].unique(), hd].all())
+                elif m == 1 or what in ("v", "do"):          # (lam's gradient is the second map's)
+                    assert bool(bad["dw"][hd])
+            dk = bad["dk"][b, :, kh, m] if op == "diff" else bad["dk"][b, :, kh]
+            assert bool(dk.any(1)[valid].all())
+            if what == "v":
+                assert torch.equal(got["dv"], want["dv"])
+            else:
+                assert bool(bad["dv"][b, :, kh].any(1)[valid].all())
+            assert not got["dk"][b][~valid].any() and not got["dv"][b][~valid].any()
+            rest, rest_k = [y for y in range(H) if y not in heads], [y for y in range(Hkv) if y != kh]
+            for n, other in (("o", rest), ("dq", rest), ("dk", rest_k), ("dv", rest_k)):
+                assert torch.equal(got[n][0], want[n][0]) and torch.equal(got[n][:, :, other], want[n][:, :, other]), n

@@ -56,8 +56,10 @@ __device__ __forceinline__ s16x8 frag(const unsigned* p) { return __builtin_bit_
 __device__ __forceinline__ s16x8 cat4(s16x4 a, s16x4 b) { return (s16x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}; }
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 // a probability from its log2: the statistics of a row with scores of 1e9 are tens of units coarse, and no probability may exceed 1 for that (the
-// clamp is a modifier of the exponential itself)
+// clamp is a modifier of the exponential itself).  A NaN has to stay one: the modifier turns it into 0 unless the wave's DX10_CLAMP (bit 8 of the mode
+// register) is off, which costs nothing where an instruction per score would.
 __device__ __forceinline__ float prob(float x) { return __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(x), 0.f, 1.f); }
+__device__ __forceinline__ void clamp_keeps_nan() { __builtin_amdgcn_s_setreg(1 | 8 << 6, 0); }
 // the other half-wave's value, without LDS
 __device__ __forceinline__ float half_sum(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
@@ -772,6 +774,7 @@ __global__ __launch_bounds__(256) void maps_join_kernel(const MapArgs a) {
 // ------------------------------------------------------------------------------------------------
 template <bool HALF, int D, int MAPS>
 __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
+  clamp_keeps_nan();
   constexpr int DV = MAPS * D, KT = 64 * D, STAGE = MAPS * KT + 64 * DV, NK = D / 16, NV = DV / 16, ND = D / 32, RA = 4;
   constexpr bool BIAS = MAPS == 1;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -937,9 +940,9 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
   if (!live) return;
 #pragma unroll
   for (int m = 0; m < MAPS; m++) {
-    const float s = half_sum(psum[m]), r = s > 0.f ? half_sum(racc[m]) / s : 0.f;
+    const float s = half_sum(psum[m]), r = s == 0.f ? 0.f : half_sum(racc[m]) / s;          // (NaN stays NaN)
     float* st = a.rvec + ((((size_t)b * a.H + h) * ((a.Sq + 63) / 64) + q0 / 64) * MAPS + m) * 128 + (q0 & 32) + l31;
-    st[g * 64] = g ? r : q_raw < a.Sq && s > 0.f ? L[m] + log2_near_1(s) : ROW_OFF;
+    st[g * 64] = g ? r : q_raw < a.Sq && s != 0.f ? L[m] + log2_near_1(s) : ROW_OFF;
     if (MAPS == 2 && m == MAPS - 1) {                      // lam's gradient: the wave's 32 rows, [H][B][32-row block]
       const float w = wave_sum_dpp(g == 0 && q_raw < a.Sq ? r : 0.f);
       const int n32 = (a.Sq + 31) / 32;
@@ -963,6 +966,7 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
 // ------------------------------------------------------------------------------------------------
 template <bool HALF, int D, int MAPS>
 __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
+  clamp_keeps_nan();
   constexpr int DV = MAPS * D, QT = 64 * D, STAGE = MAPS * QT + 64 * DV, NK = D / 16, NV = DV / 16, ND = D / 32, NDV = DV / 32;
   constexpr bool BIAS = MAPS == 1, VLDS = DV == 128;       // 128 channels: v's fragments stay in LDS, beside the accumulators they would not fit
   constexpr int RA = VLDS ? 3 : 4, RV = 2;
@@ -1254,6 +1258,7 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
 // ------------------------------------------------------------------------------------------------
 template <bool HALF, int D, int MAPS>
 __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_kernel(const MapArgs a) {
+  clamp_keeps_nan();
   constexpr int DV = MAPS * D, KT = 128 * D, VT = 128 * DV, NK = D / 16, NV = DV / 16, NC = DV / 32, ND = D / 32, RA = DV == 32 ? 2 : 4;
   constexpr int NT = NC == 4 ? 2 : 1;                      // 32 x 32 tiles of dq, of dk and of dv per wave (DV = 32: of the first four waves)
   constexpr bool BIAS = MAPS == 1;
@@ -1409,7 +1414,7 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
 #pragma unroll
     for (int m = 0; m < MAPS; m++) {                         // (divided by the row's sum of p, as in the query kernel)
       const float x = sR[(2 * m + 1) * 128 + q_raw] + sR[(2 * (MAPS + m) + 1) * 128 + q_raw];
-      ps[m] = x > 0.f ? 1.f / x : 0.f;
+      ps[m] = x == 0.f ? 0.f : 1.f / x;
       rs[m] = (sR[2 * m * 128 + q_raw] + sR[2 * (MAPS + m) * 128 + q_raw]) * ps[m];
       if (m) ps[m] *= -lam;
     }
@@ -1584,6 +1589,8 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
         a.part[((size_t)h * a.B + b) * a.gw + tid] = x;
       }
     }
+    // a row with a NaN has one at every key: not in a masked key's gradients
+    const bool kok = (mask[kblk >> 1 & 1] >> (32 * (kblk & 1) + l31)) & 1;
     bf16_t* slab = (bf16_t*)(sX + wave * 768);
 #pragma unroll
     for (int j = 0; j < NT; j++) {
@@ -1591,6 +1598,7 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
         store_rows<HALF, 32>(&dq[j], a.scale, slab, lane, [=](int r) -> bf16_t* {
           return 32 * qb(j) + r < a.Sq ? a.dq + (((size_t)b * a.Sq + 32 * qb(j) + r) * a.H + h) * DV + 32 * qc(j) : nullptr; });
       if (keys) {
+        if (!kok) { zero(dk[j]); zero(dv[j]); }
         auto rows = [=](bf16_t* base) {
           return [=](int r) -> bf16_t* { return 32 * kblk + r < a.Sk ? base + (((size_t)b * a.Sk + 32 * kblk + r) * a.H + h) * DV + 32 * (kc + j) : nullptr; };
         };
