@@ -1,5 +1,6 @@
 """What the attention cores' autograd layer relies on between a forward and a backward call.  Saved-tensor hooks (activation offloading, compression) may
-hand the backward call equal values in another layout than the forward call laid out.  On the CPU the library is a stand-in that notes its arguments."""
+hand the backward call equal values in another layout than the forward call laid out; other derivatives than the first ones in reverse mode are refused.
+On the CPU the library is a stand-in that notes its arguments."""
 import pytest
 import torch
 
@@ -86,6 +87,26 @@ def test_backward_describes_the_operands_it_is_given(library, op, how):
     assert bwd[n - 1].stride() == (d["kvalid_sb"], 1)
     saved = bwd[3: n - 1] + bwd[n: n + (3 if op == "relpos" else 4)]                                     # weights; o, (o2,) lse, dO
     assert all(x.is_contiguous() and x.data_ptr() % 4 == 0 for x in saved) and all(x.data_ptr() % 16 == 0 for x in saved if x.dim() == 4 and x.dtype == q.dtype)
+
+
+@pytest.mark.parametrize("op", ["relpos", "diff"])
+def test_forward_mode_is_refused(library, op):
+    """A tangent of an operand, or of the gradient that comes in, would be lost."""
+    from torch.autograd import forward_ad
+    q, k, v = packed(op, 2, 10, 4, 32, "cpu")
+    w, bk = weights(op, 4, "cpu")
+    with forward_ad.dual_level():
+        for i in range(4):
+            x = [q, k, v, w]
+            x[i] = forward_ad.make_dual(x[i], torch.ones_like(x[i]))
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
+                    attend(op, *x, bk)
+        attend(op, q, k, v, w, bk)                           # (no tangent: as ever)
+        leaf = q.detach().requires_grad_(True)
+        o = attend(op, leaf, k, v, w, bk)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(o, leaf, forward_ad.make_dual(torch.ones_like(o), torch.ones_like(o)))
 
 
 @pytest.mark.gpu

@@ -9,6 +9,8 @@
 Under `torch.no_grad()`, or when nothing requires a gradient, they are the forward calls alone: a few new tokens against a cache of keys and
 values (`q_offset` = how many came before) run the kernel that splits the keys.
 
+Derivatives are first ones, in reverse mode; others are refused.
+
 A step that is captured into a graph is captured whole, forward and backward, on one stream, with no autograd graph of another stream alive that
 holds the same leaves (such a call is refused)."""
 from __future__ import annotations
@@ -18,6 +20,7 @@ import random
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops
@@ -31,7 +34,17 @@ _numbers = itertools.count(random.getrandbits(62))
 def _once(backward):
     """torch's once_differentiable, whose wrapping costs 5 us: only where a second derivative could be asked for (create_graph)."""
     guarded = once_differentiable(backward)
-    return lambda ctx, do: guarded(ctx, do) if torch.is_grad_enabled() else backward(ctx, do)
+
+    def once(ctx, do):
+        _refuse_tangents(do)
+        return guarded(ctx, do) if torch.is_grad_enabled() else backward(ctx, do)
+    return once
+
+
+def _refuse_tangents(*tensors):
+    """Forward-mode differentiation: the kernels would drop the tangents without a word."""
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("attention: forward-mode differentiation is not implemented")
 
 
 class _RelposAttention(torch.autograd.Function):
@@ -85,6 +98,7 @@ def _check_capture(leaves, stream):
 
 
 def _needs_grad(*tensors):
+    _refuse_tangents(*tensors)
     return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
