@@ -12,7 +12,8 @@ values (`q_offset` = how many came before) run the kernel that splits the keys.
 Derivatives are first ones, in reverse mode; others are refused.
 
 A step that is captured into a graph is captured whole, forward and backward, on one stream, with no autograd graph of another stream alive that
-holds the same leaves (such a call is refused)."""
+holds the same leaves.  Where such a graph was made by these functions, the call is refused; those of other operations on the same leaves (a weight whose
+loss of an eager step is still referenced) are not seen here and have to be released before the capture."""
 from __future__ import annotations
 
 import itertools
@@ -76,7 +77,8 @@ class _DiffAttention(torch.autograd.Function):
 def _apply(function, leaves, *args):
     """function.apply(*args), which differentiates `leaves`.  A gradient accumulator lives as long as some autograd graph of its leaf does, and autograd's
     engine makes the stream it was made on wait for a backward pass: during a capture that joins a stream outside it, which ends the process in
-    capture_end, not in an error.  So every graph made here is noted on its leaves, and a capture is refused while one of another stream is alive."""
+    capture_end, not in an error.  So every graph made here is noted on its leaves, and a capture is refused while one of another stream is alive.  (Whether a graph of another
+    operation holds a leaf cannot be asked of torch.)"""
     on_gpu = leaves[0].is_cuda
     stream = ops._stream_of(leaves[0]) if on_gpu else 0
     leaves = [t for t in leaves if t.requires_grad and t.is_leaf]
@@ -86,8 +88,9 @@ def _apply(function, leaves, *args):
     if leaves:
         n = next(_numbers)
         _nodes[n] = weakref.ref(o.grad_fn, lambda _, nodes=_nodes: nodes.pop(n, None))
-        for t in leaves:
-            t._attention_graphs = [p for p in getattr(t, "_attention_graphs", ()) if p[0] in _nodes] + [(n, stream)]
+        for t in leaves:                                     # (a graph beside others shares their accumulator, made on the first one's stream)
+            alive = [p for p in getattr(t, "_attention_graphs", ()) if p[0] in _nodes]
+            t._attention_graphs = alive + [(n, alive[0][1] if alive else stream)]
     return o
 
 
