@@ -1,6 +1,6 @@
 """What the attention cores' autograd layer relies on between a forward and a backward call.  Saved-tensor hooks (activation offloading, compression) may
 hand the backward call equal values in another layout than the forward call laid out; other derivatives than the first ones in reverse mode are refused.
-On the CPU the library is a stand-in that notes its arguments."""
+Workgroups that stay leave reserved compute units alone.  On the CPU the library is a stand-in that notes its arguments."""
 import pytest
 import torch
 
@@ -127,3 +127,37 @@ def test_gradients_do_not_depend_on_saved_tensor_hooks(op, how):
         with torch.autograd.graph.save_on_cpu():
             got = torch.autograd.grad(attend(op, *leaves, bk, kvalid=kvalid), leaves, do)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op, D", [("relpos", 128), ("diff", 32), ("relpos", 32)])
+def test_reserved_compute_units_stay_free(op, D):
+    """The backward of short rows keeps its workgroups: with all but 8 compute units reserved (of 256) it runs on those 8 alone, at least 4 times as long,
+    and gives the same bits."""
+    from test_attention_maps import make
+    from univtg_amd import _lib, ops
+    q, k, v, w, bk, do = make(op, torch.bfloat16, 128, 8, 8, D, 64, 64)
+    if op == "relpos":
+        o, lse = ops.relpos_attention_fwd(q, k, v, w, bk)
+        bwd = lambda: ops.relpos_attention_bwd(do, q, k, v, w, bk, o, lse)
+    else:
+        o, lse, o2 = ops.diff_attention_fwd(q, k, v, w, need_o2=True)
+        bwd = lambda: ops.diff_attention_bwd(do, q, k, v, w, o, o2, lse)
+
+    def timed():
+        ev = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        bwd()
+        ev[0].record()
+        for _ in range(5):
+            out = bwd()
+        ev[1].record()
+        torch.cuda.synchronize()
+        return ev[0].elapsed_time(ev[1]), out
+    lib = _lib.load()
+    whole, want = timed()
+    try:
+        assert lib.uvtg_set_reserved_cus(1 << 16) == 8
+        few, got = timed()
+    finally:
+        lib.uvtg_set_reserved_cus(0)
+    assert few > 4 * whole and all(torch.equal(a, b) for a, b in zip(got, want))

@@ -1828,7 +1828,7 @@ template <bool HALF, int D, int MAPS> int run_bwd(const uvtg_attn_dims* d, MapAr
   if (short_rows(d)) {
     constexpr size_t lds = 4 * 128 * DV * 2 + 4 * MAPS * 512 + DIAG_BYTES + (MAPS == 1 ? 8 * 96 * 4 + 256 + 1024 : 0) + (DV == 64 ? MAPS * 128 * 256 : 0);
     // workgroups that stay: one per CU, two where registers allow
-    const int wgs = DV == 32 ? 512 : 256;
+    const int wgs = (DV == 32 ? 2 : 1) * persistent_cus();
     hipLaunchKernelGGL((maps_bwd_short_kernel<HALF, D, MAPS>), dim3(d->H * d->B < wgs ? d->H * d->B : wgs), dim3(512), lds, s, a);
     UVTG_CHECK_LAUNCH();
   } else {

@@ -1794,6 +1794,7 @@ static bool nt256_ok(const GemmArgs& a) {
   const long long bmax = (long long)a.N * a.ldb + (long long)groups * a.gB;
   return amax * 2 < (1LL << 32) && bmax * 2 < (1LL << 32);
 }
+int persistent_cus() { return ensure_num_cu() ? 256 : eff_cus(); }
 extern "C" int uvtg_set_reserved_cus(int k) {
   g_cu_reserved = k > 0 ? k : 0;
   if (ensure_num_cu()) return -1;

@@ -70,6 +70,7 @@ bool gemm_nt_delta_ok(const GemmArgs& a);
 constexpr int UVTG_SK_UNITS = 256;                 // capacity the engine's workspace provides
 constexpr int UVTG_SK_TILE_FLOATS = 128 * 256;
 int launch_gemm_nt_bf16(const GemmArgs& a, hipStream_t s);
+int persistent_cus();            // CUs that a persistent grid may use: the device's, less those of uvtg_set_reserved_cus
 int launch_gemm_nt_split(const GemmArgs& a, hipStream_t s);
 
 // C[N,K] (+)= P[M,N]^T * Q[M,K]  (reduction over rows; fp32 atomic accumulation, split over M)
