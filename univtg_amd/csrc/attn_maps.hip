@@ -266,8 +266,9 @@ __device__ __forceinline__ void block_id(int nblk, const MapArgs& a, int heads, 
 }
 
 // [W / 32] accumulators (rows = channels, lane = row of the output) times a factor per lane -> 16-bit rows of W contiguous channels, through a
-// wave-private LDS slab: 16 bytes per lane, W / 8 lanes per row
-template <bool HALF, int W, typename F> __device__ __forceinline__ void store_rows(const f32x16* acc, float factor, bf16_t* slab, int lane, F&& row_ptr) {
+// wave-private LDS slab: 16 bytes per lane, W / 8 lanes per row.  keep: all ones, or 0 for a lane whose row is stored as zeros (NaN included)
+template <bool HALF, int W, typename F>
+__device__ __forceinline__ void store_rows(const f32x16* acc, float factor, bf16_t* slab, int lane, F&& row_ptr, unsigned keep = ~0u) {
   constexpr int PW = W < 64 ? W : 64, STR = PW + 8, CPR = PW / 8;
   const int l31 = lane & 31, g = lane >> 5;
 #pragma unroll
@@ -278,8 +279,8 @@ template <bool HALF, int W, typename F> __device__ __forceinline__ void store_ro
       for (int j = 0; j < 4; j++) {
         const f32x16& x = acc[pass * (PW / 32) + i];
         u32x2 t;
-        t[0] = pack2<HALF>(x[4 * j] * factor, x[4 * j + 1] * factor);
-        t[1] = pack2<HALF>(x[4 * j + 2] * factor, x[4 * j + 3] * factor);
+        t[0] = pack2<HALF>(x[4 * j] * factor, x[4 * j + 1] * factor) & keep;
+        t[1] = pack2<HALF>(x[4 * j + 2] * factor, x[4 * j + 3] * factor) & keep;
         *(u32x2*)(slab + l31 * STR + i * 32 + 8 * j + 4 * g) = t;
       }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -1590,7 +1591,7 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
       }
     }
     // a row with a NaN has one at every key: not in a masked key's gradients
-    const bool kok = (mask[kblk >> 1 & 1] >> (32 * (kblk & 1) + l31)) & 1;
+    const unsigned keep = -(unsigned)((mask[kblk >> 1 & 1] >> (32 * (kblk & 1) + l31)) & 1);
     bf16_t* slab = (bf16_t*)(sX + wave * 768);
 #pragma unroll
     for (int j = 0; j < NT; j++) {
@@ -1598,12 +1599,11 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
         store_rows<HALF, 32>(&dq[j], a.scale, slab, lane, [=](int r) -> bf16_t* {
           return 32 * qb(j) + r < a.Sq ? a.dq + (((size_t)b * a.Sq + 32 * qb(j) + r) * a.H + h) * DV + 32 * qc(j) : nullptr; });
       if (keys) {
-        if (!kok) { zero(dk[j]); zero(dv[j]); }
         auto rows = [=](bf16_t* base) {
           return [=](int r) -> bf16_t* { return 32 * kblk + r < a.Sk ? base + (((size_t)b * a.Sk + 32 * kblk + r) * a.H + h) * DV + 32 * (kc + j) : nullptr; };
         };
-        store_rows<HALF, 32>(&dk[j], a.scale, slab, lane, rows(a.dk));
-        store_rows<HALF, 32>(&dv[j], 1.f, slab, lane, rows(a.dv));
+        store_rows<HALF, 32>(&dk[j], a.scale, slab, lane, rows(a.dk), keep);
+        store_rows<HALF, 32>(&dv[j], 1.f, slab, lane, rows(a.dv), keep);
       }
     }
   }
