@@ -44,7 +44,7 @@ def _once(backward):
 
 def _refuse_tangents(*tensors):
     """Forward-mode differentiation: the kernels would drop the tangents without a word."""
-    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError("attention: forward-mode differentiation is not implemented")
 
 

@@ -278,17 +278,23 @@ def _attn_call(name, maps, q, k, v, kvalid, q_offset, causal, scale):
         raise ValueError(f"{name}: q_offset must lie within +-2^28, got {q_offset}")
     d = _lib.AttnDims(0, _ATTN_TYPES[dtype], B, H, Hkv, D, Sq, Sk, 1 if causal else 0, int(q_offset), D ** -0.5 if scale is None else float(scale), 0, 0,
                       qs[0], qs[1], qs[2], qs[3] if maps == 2 else 0, ks[0], ks[1], ks[2], ks[3] if maps == 2 else 0, vs[0], vs[1], vs[2], mask_sb)
-    d.layout = (dev, qs, ks, vs, None if kvalid is None else kvalid.stride())
+    d.layout = (qs, ks, vs)
     return d, q, k, v, kvalid
 
 
-def _attn_saved_operands(name, maps, d, q, k, v, kvalid):
-    """What _attn_call returned, for operands that went through autograd's hands since: saved-tensor hooks (offloading, compression) return equal values
-    in whatever layout, which is then checked, laid out and described anew."""
-    if (q.device, q.stride(), k.stride(), v.stride(), None if kvalid is None else kvalid.stride()) == d.layout and k.device == v.device == q.device and \
-            (kvalid is None or kvalid.device == q.device) and not (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
-        return d, q, k, v, kvalid
-    return _attn_call(name, maps, q, k, v, kvalid, d.q_offset, d.causal, d.scale)
+def _attn_unchanged(d, q, k, v, kvalid, dense):
+    """Whether operands that autograd kept since their call laid them out are still laid out that way (`dense`: those that are contiguous).  Saved-tensor
+    hooks (offloading, compression) return equal values in whatever layout."""
+    dev, address = q.get_device(), q.data_ptr() | k.data_ptr() | v.data_ptr()
+    if (q.stride(), k.stride(), v.stride()) != d.layout or k.get_device() != dev or v.get_device() != dev or not q.dtype == k.dtype == v.dtype:
+        return False
+    if kvalid is not None and (kvalid.stride() != (d.kvalid_sb, 1) or kvalid.get_device() != dev):
+        return False
+    for t in dense:
+        if not t.is_contiguous() or t.get_device() != dev:
+            return False
+        address |= t.data_ptr()
+    return not address & 15
 
 
 def _attn_ws(lib, d, maps, backward, like):
@@ -341,10 +347,11 @@ def _relpos_fwd(q, k, v, table, buckets, kvalid, q_offset, causal, scale):
 
 def _relpos_bwd(do, d, q, k, v, table, buckets, kvalid, o, lse, need_dtable):
     lib = _lib.load()
-    d, q, k, v, kvalid = _attn_saved_operands("relpos_attention_bwd", 1, d, q, k, v, kvalid)
-    table, buckets = _relpos_operands(d, q, table, buckets)
-    do, o = (_attn_saved("relpos_attention_bwd", t, q, w) for t, w in ((do, "do"), (o, "o")))
-    lse = _attn_saved("relpos_attention_bwd", lse, q, "lse", torch.float32)
+    if not _attn_unchanged(d, q, k, v, kvalid, (table, buckets, o, lse)):
+        d, q, k, v, kvalid = _attn_call("relpos_attention_bwd", 1, q, k, v, kvalid, d.q_offset, d.causal, d.scale)
+        table, buckets = _relpos_operands(d, q, table, buckets)
+        o, lse = _attn_saved("relpos_attention_bwd", o, q, "o"), _attn_saved("relpos_attention_bwd", lse, q, "lse", torch.float32)
+    do = _attn_saved("relpos_attention_bwd", do, q, "do")
     dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     dtable = table.new_empty(table.shape) if need_dtable else None
     ws = _attn_ws(lib, d, 1, 1, q)
@@ -356,8 +363,8 @@ def _relpos_bwd(do, d, q, k, v, table, buckets, kvalid, o, lse, need_dtable):
 def relpos_attention_fwd(q, k, v, table, buckets, kvalid=None, q_offset=0, causal=False, scale=None):
     """softmax(scale q k^T + table[buckets[clamp(j - i - q_offset)], h]) v: q [B, Sq, H, D], k and v [B, Sk, Hkv, D] (bf16 or fp16, D 32 / 64 / 128,
     any strides), table [n_buckets, H] fp32, buckets int32 [2 reach + 1] (relpos_buckets), kvalid [B, Sk] uint8 / bool (0 = masked key).  causal:
-    query i sees keys up to i + q_offset; k and v rows that are masked, or behind what any query sees, may hold anything.  A table entry of -inf takes its positions out of the row.  scale defaults to D ** -0.5.  Returns o
-    [B, Sq, H, D] and lse [B, H, Sq] (fp32); a row that sees no key is 0 with lse -inf."""
+    query i sees keys up to i + q_offset; k and v rows that are masked, or behind what any query sees, may hold anything.  A table entry of -inf takes its
+    positions out of the row.  scale defaults to D ** -0.5.  Returns o [B, Sq, H, D] and lse [B, H, Sq] (fp32); a row that sees no key is 0 with lse -inf."""
     if _elsewhere(q):
         with torch.cuda.device(q.device):
             return relpos_attention_fwd(q, k, v, table, buckets, kvalid, q_offset, causal, scale)
@@ -370,9 +377,11 @@ def relpos_attention_bwd(do, q, k, v, table, buckets, o, lse, kvalid=None, q_off
         with torch.cuda.device(q.device):
             return relpos_attention_bwd(do, q, k, v, table, buckets, o, lse, kvalid, q_offset, causal, scale, need_dtable)
     d, q, k, v, kvalid = _attn_call("relpos_attention", 1, q, k, v, kvalid, q_offset, causal, scale)
+    table, buckets = _relpos_operands(d, q, table, buckets)
     if do.shape != (d.B, d.Sq, d.H, d.D) or o.shape != do.shape or lse.shape != (d.B, d.H, d.Sq):
         raise ValueError("relpos_attention_bwd: do and o must be [B, Sq, H, D], lse [B, H, Sq]")
-    return _relpos_bwd(do, d, q, k, v, table, buckets, kvalid, o, lse, need_dtable)
+    return _relpos_bwd(do, d, q, k, v, table, buckets, kvalid, _attn_saved("relpos_attention_bwd", o, q, "o"),
+                       _attn_saved("relpos_attention_bwd", lse, q, "lse", torch.float32), need_dtable)
 
 
 def _lam_operand(d, q, lam):
@@ -396,10 +405,12 @@ def _diff_fwd(q, k, v, lam, kvalid, q_offset, causal, scale, need_o2):
 
 def _diff_bwd(do, d, q, k, v, lam, kvalid, o, o2, lse, need_dlam):
     lib = _lib.load()
-    d, q, k, v, kvalid = _attn_saved_operands("diff_attention_bwd", 2, d, q, k, v, kvalid)
-    lam = _lam_operand(d, q, lam)
-    do, o, o2 = (_attn_saved("diff_attention_bwd", t, q, w) for t, w in ((do, "do"), (o, "o"), (o2, "o2")))
-    lse = _attn_saved("diff_attention_bwd", lse, q, "lse", torch.float32)
+    if not _attn_unchanged(d, q, k, v, kvalid, (lam, o, o2, lse)):
+        d, q, k, v, kvalid = _attn_call("diff_attention_bwd", 2, q, k, v, kvalid, d.q_offset, d.causal, d.scale)
+        lam = _lam_operand(d, q, lam)
+        o, o2 = _attn_saved("diff_attention_bwd", o, q, "o"), _attn_saved("diff_attention_bwd", o2, q, "o2")
+        lse = _attn_saved("diff_attention_bwd", lse, q, "lse", torch.float32)
+    do = _attn_saved("diff_attention_bwd", do, q, "do")
     dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     dlam = lam.new_empty(d.H) if need_dlam else None
     ws = _attn_ws(lib, d, 2, 1, q)
@@ -425,6 +436,8 @@ def diff_attention_bwd(do, q, k, v, lam, o, o2, lse, kvalid=None, q_offset=0, ca
         with torch.cuda.device(q.device):
             return diff_attention_bwd(do, q, k, v, lam, o, o2, lse, kvalid, q_offset, causal, scale, need_dlam)
     d, q, k, v, kvalid = _attn_call("diff_attention", 2, q, k, v, kvalid, q_offset, causal, scale)
+    lam = _lam_operand(d, q, lam)
     if do.shape != (d.B, d.Sq, d.H, 2 * d.D) or o.shape != do.shape or o2.shape != do.shape or lse.shape != (d.B, d.H, 2, d.Sq):
         raise ValueError("diff_attention_bwd: do, o and o2 must be [B, Sq, H, 2 D], lse [B, H, 2, Sq]")
-    return _diff_bwd(do, d, q, k, v, lam, kvalid, o, o2, lse, need_dlam)
+    o, o2 = (_attn_saved("diff_attention_bwd", t, q, w) for t, w in ((o, "o"), (o2, "o2")))
+    return _diff_bwd(do, d, q, k, v, lam, kvalid, o, o2, _attn_saved("diff_attention_bwd", lse, q, "lse", torch.float32), need_dlam)
