@@ -1,4 +1,4 @@
-"""Values that the attention cores meet at the edges: NaN and infinities that are not masked, rows of a cache that no query sees.  The formulas in 64 bits and their tolerances are those of
+"""Values that the attention cores meet at the edges: NaN and infinities that are not masked, rows of a cache that no query sees, small gradients.  The formulas in 64 bits and their tolerances are those of
 test_attention_maps."""
 import math
 
@@ -79,3 +79,36 @@ def test_nan_and_infinity_reach_what_depends_on_them(op, D, what, Sq, Sk, H, Hkv
             rest, rest_k = [y for y in range(H) if y not in heads], [y for y in range(Hkv) if y != kh]
             for n, other in (("o", rest), ("dq", rest), ("dk", rest_k), ("dv", rest_k)):
                 assert torch.equal(got[n][0], want[n][0]) and torch.equal(got[n][:, :, other], want[n][:, :, other]), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq, Sk, H, Hkv", [(100, 100, 2, 2), (60, 128, 4, 2), (1000, 1000, 2, 1), (700, 4000, 2, 2)])
+@pytest.mark.parametrize("power", [-6, -10, -13])
+@pytest.mark.parametrize("op, D", OPS)
+def test_small_gradients_in_half_precision(op, D, power, Sq, Sk, H, Hkv):
+    """Output gradients of 2^power, as a mean over a batch leaves them without a loss scale: dq and dk are about as near to the formula as at 2^0, where the
+    score gradients lie in the type's normal range.  In the 2-norm an error of P, dS or the output itself is at most u sqrt(1 / 3) of its part, three of
+    them 2^-11, and a rounding of the output below the normal range adds 2^-25 sqrt(1 / 3) per entry; twice their sum is allowed."""
+    q, k, v, w, bk, do = make(op, torch.float16, 1, H, Hkv, D, Sq, Sk, seed=33)
+    rows = torch.rand(1, Sq, 1, 1, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") < 0.9
+    do = torch.where(rows, do, do * 2.0 ** -4) * 2.0 ** power                        # (some rows smaller still)
+    got, want = run(op, q, k, v, w, bk, do), reference(op, q, k, v, w, bk, do=do)
+    for n in ("dq", "dk"):
+        x = want[n][0]
+        bound = 2 * (2.0 ** -11 * x.norm() + 2.0 ** -25 * (x.numel() / 3) ** 0.5)
+        assert (got[n].double() - x).norm() < bound, (n, float((got[n].double() - x).norm() / bound))
+    check({n: got[n] for n in ("o", "lse", "dv", "dw")}, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq, Sk", [(90, 110), (200, 300)])
+@pytest.mark.parametrize("op, D", OPS)
+def test_powers_of_two_pass_through(op, D, Sq, Sk):
+    """Gradients are linear in dO: halving it halves the fp32 gradients exactly, and those in 16 bits as long as no entry leaves the normal range."""
+    q, k, v, w, bk, do = make(op, torch.float16, 2, 2, 2, D, Sq, Sk, seed=34)
+    do = (do.clamp(-3, 3) * 256).round() / 1024              # (whole multiples of 2^-10, at most 3 / 4: their halves are exact)
+    one, half = run(op, q, k, v, w, bk, do), run(op, q, k, v, w, bk, do * 0.5)
+    assert torch.equal(one["dw"], half["dw"] * 2)
+    for n in ("dq", "dk", "dv"):
+        big = one[n].abs() >= 2.0 ** -13
+        assert torch.equal(one[n][big], half[n][big] * 2), n

@@ -28,7 +28,7 @@ struct MapArgs {
   const int* buckets;
   const unsigned char* kvalid;
   bf16_t *out, *out2, *dq, *dk, *dv;
-  float *lse, *rvec, *part, *acc;
+  float *lse, *rvec, *part, *acc, *amax;
   const float* lse_in;
   long long q_sb, q_ss, q_sh, q_sm, k_sb, k_ss, k_sh, k_sm, v_sb, v_ss, v_sh, mask_sb;     // element strides
   int B, H, Hkv, G, Sq, Sk, NB, R, off, causal;
@@ -78,6 +78,34 @@ __device__ __forceinline__ float log2_near_1(float s) {
 // queries, which cancel, and so would keep it: half of dP's products are formed with the other sign, where the error has it too (two maps of 32,
 // 4 x 3869 queries over 2657 keys, fp16: 1.1e-5 of dlam before, under 1e-6 with it).  ds does not feel a constant in dP.
 __device__ __forceinline__ s16x8 negated(s16x8 x) { return x ^ (short)0x8000; }
+// fp16 score gradients: of a small dO (a mean over a batch, no loss scale) most would fall below the type's normal range (dO of 2^-10 over 4000 keys: dq and
+// dk off by 5e-3 instead of 3e-4).  They are formed from dO times the power of two that brings its largest entry to 1 .. 2, and dq and dk are divided by it
+// in the factor that they are stored with; an entry of 1 or more leaves everything as it is.  (Not further up: |dS| may reach |dO| |v| channels / 2.)
+__device__ __forceinline__ float lift_of(float amax) {                     // (NaN, infinity: 1)
+  const int e = (int)((__float_as_uint(amax) >> 23) & 255) - 127;
+  return __uint_as_float((unsigned)(127 + min(max(-e, 0), 15)) << 23);
+}
+__device__ __forceinline__ float inverse_of(float lift) { return __uint_as_float((254u << 23) - __float_as_uint(lift)); }
+template <int N> __device__ __forceinline__ float amax_half(const s16x8 (&x)[N]) {     // (as whole numbers, whose order is the values'; a NaN is the largest)
+  typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+  u16x2 m = 0;
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const u32x4 w = __builtin_bit_cast(u32x4, x[i]);
+#pragma unroll
+    for (int e = 0; e < 4; e++) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu));
+  }
+  return (float)__builtin_bit_cast(_Float16, (unsigned short)(m[0] > m[1] ? m[0] : m[1]));
+}
+__device__ __forceinline__ float top_of_wave(float x) {                    // (steps as in wave_sum_dpp)
+  x = fmaxf(x, dpp_mov<0xB1>(x));
+  x = fmaxf(x, dpp_mov<0x4E>(x));
+  x = fmaxf(x, dpp_mov<0x141>(x));
+  x = fmaxf(x, dpp_mov<0x140>(x));
+  const int b = __float_as_int(x);
+  return fmaxf(fmaxf(__int_as_float(__builtin_amdgcn_readlane(b, 0)), __int_as_float(__builtin_amdgcn_readlane(b, 16))),
+               fmaxf(__int_as_float(__builtin_amdgcn_readlane(b, 32)), __int_as_float(__builtin_amdgcn_readlane(b, 48))));
+}
 __device__ __forceinline__ void zero(f32x16& x) {
 #pragma unroll
   for (int r = 0; r < 16; r++) x[r] = 0.f;
@@ -805,7 +833,7 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
   if (ntiles > 0) request(0, 0);
   if (ntiles > 1) request(1, 1);
   s16x8 qf[MAPS][NK], of[NV];
-  float L[MAPS], del[MAPS], racc[MAPS], psum[MAPS];
+  float L[MAPS], del[MAPS], racc[MAPS], psum[MAPS], drop = 1.f;
   const float lam = MAPS == 2 ? a.lam[h] : 0.f;
   {
     const size_t ro = (((size_t)b * a.Sq + qrow) * a.H + h) * DV + 8 * g;
@@ -837,7 +865,16 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
     }
 #pragma unroll
     for (int m = 0; m < MAPS; m++) del[m] = half_sum(del[m]);
-    if constexpr (MAPS == 2) {
+    if constexpr (HALF) {                                  // every row by its own power of two; the key kernel takes one for all rows that it adds up
+      const float am = half_max(amax_half(of)), lift = lift_of(am), top = top_of_wave(am);
+      drop = inverse_of(lift);
+      if (live && lane == 0) a.amax[((size_t)b * a.H + h) * ((a.Sq + 31) / 32) + q0 / 32] = top;
+#pragma unroll
+      for (int m = 0; m < MAPS; m++) del[m] *= lift;
+#pragma unroll
+      for (int ks = 0; ks < NV; ks++)
+        of[ks] = __builtin_bit_cast(s16x8, __builtin_bit_cast(half8_t, of[ks]) * (_Float16)(MAPS == 2 && ks >= NV / 4 && ks < 3 * NV / 4 ? -lift : lift));
+    } else if constexpr (MAPS == 2) {
 #pragma unroll
       for (int ks = NV / 4; ks < 3 * NV / 4; ks++) of[ks] = negated(of[ks]);
     }
@@ -941,7 +978,7 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
   if (!live) return;
 #pragma unroll
   for (int m = 0; m < MAPS; m++) {
-    const float s = half_sum(psum[m]), r = s == 0.f ? 0.f : half_sum(racc[m]) / s;          // (NaN stays NaN)
+    const float s = half_sum(psum[m]), r = s == 0.f ? 0.f : half_sum(racc[m]) / s * drop;          // (NaN stays NaN)
     float* st = a.rvec + ((((size_t)b * a.H + h) * ((a.Sq + 63) / 64) + q0 / 64) * MAPS + m) * 128 + (q0 & 32) + l31;
     st[g * 64] = g ? r : q_raw < a.Sq && s != 0.f ? L[m] + log2_near_1(s) : ROW_OFF;
     if (MAPS == 2 && m == MAPS - 1) {                      // lam's gradient: the wave's 32 rows, [H][B][32-row block]
@@ -953,7 +990,7 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
   bf16_t* slab = stage + wave * SLAB;
 #pragma unroll
   for (int m = 0; m < MAPS; m++)
-    store_rows<HALF, D>(acc[m], a.scale, slab, lane, [=](int row) -> bf16_t* {
+    store_rows<HALF, D>(acc[m], a.scale * drop, slab, lane, [=](int row) -> bf16_t* {
       return q0 + row < a.Sq ? a.dq + ((((size_t)b * a.Sq + q0 + row) * a.H + h) * MAPS + m) * D : nullptr; });
 }
 
@@ -1036,6 +1073,7 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
 #pragma unroll
     for (int i = 0; i < 12; i++) diag[i * 64 + lane] = 0.f;
   }
+  float drop = 1.f;
   const bool live = __builtin_amdgcn_ballot_w64(kok) != 0;
   if (lane == 0) sAny[wave] = live ? 1.f : 0.f;
   int nqt = max(0, nq64 - first);
@@ -1044,6 +1082,11 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
     const float lam = MAPS == 2 ? a.lam[h] : 0.f;
     float fl = 0.f, fr = 0.f, bl = 0.f, br = 0.f;          // sums and bias of the positions at and behind -R / +R
     float* part = nullptr;
+    float top = 0.f;
+    const int ntop = a.G * ((a.Sq + 31) / 32);
+    const float* tops = a.amax + ((size_t)b * a.H + kh * a.G) * ((a.Sq + 31) / 32);
+    const int at = HALF ? (int)opaque(lane) : 0;           // (opaque: no address kept over the loop)
+    if (HALF && at < ntop) top = tops[at];                 // (used behind the wait that the bias needs anyway)
     if (hg > 0) {
       __syncthreads();                                     // the previous head's tiles, bias and statistics are read
       ql.base += 2 * a.q_sh; ol.base += 2 * DV; stat += (size_t)nq64 * MAPS * 128;
@@ -1059,10 +1102,20 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
     __syncthreads();
     if (hg == 0 && __builtin_amdgcn_readfirstlane(__float_as_int(sAny[0] + sAny[1] + sAny[2] + sAny[3])) == 0) nqt = 0;     // no key of the workgroup is valid
     if constexpr (BIAS) { bl = rlo <= -a.R ? sB[0] : 0.f; br = rhi >= a.R ? sB[rhi - rlo] : 0.f; }
+    float lift = 1.f;                                      // from the largest entry of the group's dO
+    if constexpr (HALF) {
+      for (int i = at + 64; i < ntop; i += 64) top = fmaxf(top, tops[i]);
+      lift = lift_of(top_of_wave(top));
+      drop = inverse_of(lift);
+    }
 #pragma nounroll
     for (int n = 0; n < nqt; n++) {
       const int qt = first + n, buf = n & 1, q0 = qt * 64 + qh * 32;
       dma_wait();
+      if (HALF && wave == 7 && lift != 1.f) {              // (the wave that requested the tile's statistics: r by the lift, too)
+#pragma unroll
+        for (int m = 0; m < MAPS; m++) sStat[buf * 256 + m * 128 + 64 + lane] *= lift;
+      }
       __syncthreads();
       const bool req = n > 0 && n + 1 < nqt;
       const bool work = live && q0 < a.Sq && !(a.causal && q0 + 31 + a.off < k0);
@@ -1145,11 +1198,11 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
               for (int u = 0; u < 2; u++) {
                 const int r = 4 * j + e + u;
                 p[u] = prob(fmaf(s[0][r], cc, cb - L[0][e + u]));
-                d0[u] = p[u] * (dp[r] - r_[0][e + u]);
+                d0[u] = p[u] * (HALF ? fmaf(dp[r], lift, -r_[0][e + u]) : dp[r] - r_[0][e + u]);
                 if constexpr (BIAS) { far += d0[u]; ds0[r - 8 * ps] = d0[u]; }
                 if constexpr (MAPS == 2) {
                   const float p2 = -lam * prob(fmaf(s[MAPS - 1][r], cc, -L[MAPS - 1][e + u]));
-                  d1[u] = p2 * (dp[r] - r_[MAPS - 1][e + u]);
+                  d1[u] = p2 * (HALF ? fmaf(dp[r], lift, -r_[MAPS - 1][e + u]) : dp[r] - r_[MAPS - 1][e + u]);
                   p[u] += p2;
                 }
               }
@@ -1178,6 +1231,7 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
           }
         }
         if constexpr (BIAS) {
+          if constexpr (HALF) { far *= drop; dsum *= drop; }
           if (close) {
             const int rel = rb + lane - 31;                // (the wave's blocks are 64 queries apart: no other one has these positions)
             if (lane < 63) {
@@ -1238,7 +1292,7 @@ __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
     for (int m = 0; m < MAPS; m++) {
 #pragma unroll
       for (int i = 0; i < ND; i++) if (!kok) zero(dk[m][i]);
-      store_rows<HALF, D>(dk[m], a.scale, slab, lane, [=](int row) -> bf16_t* {
+      store_rows<HALF, D>(dk[m], a.scale * drop, slab, lane, [=](int row) -> bf16_t* {
         return k0 + row < a.Sk ? a.dk + ((((size_t)b * a.Sk + k0 + row) * a.Hkv + kh) * MAPS + m) * D : nullptr; });
     }
   } else {
@@ -1275,7 +1329,8 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
   float* sRow = sX + 8 * 768;                              // [8 waves][96] bias gradient of the wave's 95 positions
   float* sEnd = sRow + (BIAS ? 8 * 96 : 0);                // [8 waves][2] its sums at and behind -R, +R
   float* sB = sEnd + (BIAS ? 64 : 0);                      // [256] bias by position
-  bf16_t* sS = DV == 128 ? sV : DV == 32 ? (bf16_t*)sX : (bf16_t*)(sB + (BIAS ? 256 : 0));           // [MAPS][RS][128]
+  float* sTop = sB + (BIAS ? 256 : 0);                     // [8 waves] largest entries of dO (fp16), to the next multiple of 256 bytes
+  bf16_t* sS = DV == 128 ? sV : DV == 32 ? (bf16_t*)sX : (bf16_t*)(sTop + 64);                       // [MAPS][RS][128]
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w4 = wave & 3, half = wave >> 2;
   auto request = [&](int b, int h, int lane) {
 #pragma unroll
@@ -1360,6 +1415,7 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
     bool on[2];                                              // the block has a (query, key) pair
 #pragma unroll
     for (int kb = 0; kb < 2; kb++) on[kb] = live && (unsigned)(mask[half] >> (32 * kb)) != 0 && (!a.causal || min(q0 + 31, a.Sq - 1) + a.off >= key0 + 32 * kb);
+    float top = 0.f, lift = 1.f;
     if (on[0] || on[1]) {
       s16x8 qf[MAPS][NK], of[NV];
 #pragma unroll
@@ -1368,6 +1424,7 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
         for (int ks = 0; ks < NK; ks++) qf[m][ks] = row_frag(lds_at(sQ + m * KT + q0 * D) + koff, ks, 0);
 #pragma unroll
       for (int ks = 0; ks < NV; ks++) of[ks] = row_frag(lds_at(sO + q0 * DV) + voff, ks, 0);
+      if constexpr (HALF) top = top_of_wave(amax_half(of));
       if constexpr (MAPS == 2) {
 #pragma unroll
         for (int ks = NV / 4; ks < 3 * NV / 4; ks++) of[ks] = negated(of[ks]);
@@ -1411,7 +1468,12 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
       rs[m] = half_sum(rs[m]); ps[m] = half_sum(ps[m]);
       sR[((half * MAPS + m) * 2 + g) * 128 + q_raw] = g ? ps[m] : rs[m];
     }
+    if (HALF && lane == 0) sTop[wave] = top;
     __syncthreads();
+    if constexpr (HALF) {
+      const f32x4 x = *(const f32x4*)sTop, y = *(const f32x4*)(sTop + 4);
+      lift = lift_of(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]))));
+    }
 #pragma unroll
     for (int m = 0; m < MAPS; m++) {                         // (divided by the row's sum of p, as in the query kernel)
       const float x = sR[(2 * m + 1) * 128 + q_raw] + sR[(2 * (MAPS + m) + 1) * 128 + q_raw];
@@ -1422,6 +1484,11 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
     if (MAPS == 2 && half == 0 && live) {                    // lam's gradient: the wave's 32 rows, [H][B][32-row block]
       const float w = wave_sum_dpp(g == 0 && q_raw < a.Sq ? rs[MAPS - 1] : 0.f);
       if (lane == 0) a.part[((size_t)h * a.B + b) * ((a.Sq + 31) / 32) + w4] = w;
+    }
+    const float drop = inverse_of(lift);
+    if constexpr (HALF) {
+#pragma unroll
+      for (int m = 0; m < MAPS; m++) rs[m] *= lift;
     }
     // ---- P and dS, packed as operands
     unsigned pp[2][8], pd[MAPS][2][8];
@@ -1441,10 +1508,10 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
 #pragma unroll
         for (int u = 0; u < 2; u++) {
           x[u] = p[0][kb][r + u] * ps[0];
-          d[0][u] = x[u] * (dp[kb][r + u] - rs[0]);
+          d[0][u] = x[u] * (HALF ? fmaf(dp[kb][r + u], lift, -rs[0]) : dp[kb][r + u] - rs[0]);
           if constexpr (MAPS == 2) {
             const float y = ps[MAPS - 1] * p[MAPS - 1][kb][r + u];
-            d[MAPS - 1][u] = y * (dp[kb][r + u] - rs[MAPS - 1]);
+            d[MAPS - 1][u] = y * (HALF ? fmaf(dp[kb][r + u], lift, -rs[MAPS - 1]) : dp[kb][r + u] - rs[MAPS - 1]);
             x[u] += y;
           }
           if constexpr (BIAS) dp[kb][r + u] = d[0][u];
@@ -1471,6 +1538,7 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
           }
+          if constexpr (HALF) v *= drop;
           const int rel = key0 + 32 * kb - q0 - a.off + lane - 31;
           if (lane < 63) {
             if (rel >= a.R) fr += v;
@@ -1593,16 +1661,17 @@ __global__ __launch_bounds__(512, MAPS * D == 32 ? 4 : 2) void maps_bwd_short_ke
     // a row with a NaN has one at every key: not in a masked key's gradients
     const unsigned keep = -(unsigned)((mask[kblk >> 1 & 1] >> (32 * (kblk & 1) + l31)) & 1);
     bf16_t* slab = (bf16_t*)(sX + wave * 768);
+    const float factor = HALF ? a.scale * drop : a.scale;
 #pragma unroll
     for (int j = 0; j < NT; j++) {
       if (32 * qb(j) < a.Sq)
-        store_rows<HALF, 32>(&dq[j], a.scale, slab, lane, [=](int r) -> bf16_t* {
+        store_rows<HALF, 32>(&dq[j], factor, slab, lane, [=](int r) -> bf16_t* {
           return 32 * qb(j) + r < a.Sq ? a.dq + (((size_t)b * a.Sq + 32 * qb(j) + r) * a.H + h) * DV + 32 * qc(j) : nullptr; });
       if (keys) {
         auto rows = [=](bf16_t* base) {
           return [=](int r) -> bf16_t* { return 32 * kblk + r < a.Sk ? base + (((size_t)b * a.Sk + 32 * kblk + r) * a.H + h) * DV + 32 * (kc + j) : nullptr; };
         };
-        store_rows<HALF, 32>(&dk[j], a.scale, slab, lane, rows(a.dk), keep);
+        store_rows<HALF, 32>(&dk[j], factor, slab, lane, rows(a.dk), keep);
         store_rows<HALF, 32>(&dv[j], 1.f, slab, lane, rows(a.dv), keep);
       }
     }
@@ -1749,11 +1818,13 @@ void reachable(const uvtg_attn_dims* d, int& glo, int& gw) {
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 // whole rows in one workgroup: one pass over the operands (256 x 107, 8 heads of 128: 120 us against 221 us of the two passes)
 bool short_rows(const uvtg_attn_dims* d) { return d->Sq <= 128 && d->Sk <= 128 && d->H == d->Hkv; }
-struct BwdWs { size_t rvec, part, sums, total; long long rows; int chunk, chunks, direct; };
+struct BwdWs { size_t rvec, part, sums, amax, total; long long rows; int chunk, chunks, direct; };
 BwdWs bwd_ws(const uvtg_attn_dims* d, int maps) {
   BwdWs w;
   w.rvec = 0;
   size_t at = align256((size_t)d->B * d->H * ((d->Sq + 63) / 64) * maps * 512 + 512);     // (a tile's statistics are fetched 1024 bytes at a time)
+  w.amax = at;
+  if (d->dtype && !short_rows(d)) at += align256((size_t)d->B * d->H * ((d->Sq + 31) / 32) * 4);
   w.part = at;
   if (maps == 1) {
     int glo, gw;
@@ -1824,9 +1895,10 @@ template <bool HALF, int D, int MAPS> int run_bwd(const uvtg_attn_dims* d, MapAr
   const BwdWs w = bwd_ws(d, MAPS);
   a.rvec = (float*)(ws + w.rvec);
   a.part = (float*)(ws + w.part);
+  a.amax = (float*)(ws + w.amax);
   if (MAPS == 1) reachable(d, a.glo, a.gw);
   if (short_rows(d)) {
-    constexpr size_t lds = 4 * 128 * DV * 2 + 4 * MAPS * 512 + DIAG_BYTES + (MAPS == 1 ? 8 * 96 * 4 + 256 + 1024 : 0) + (DV == 64 ? MAPS * 128 * 256 : 0);
+    constexpr size_t lds = 4 * 128 * DV * 2 + 4 * MAPS * 512 + DIAG_BYTES + (MAPS == 1 ? 8 * 96 * 4 + 256 + 1024 : 0) + 256 + (DV == 64 ? MAPS * 128 * 256 : 0);
     // workgroups that stay: one per CU, two where registers allow
     const int wgs = (DV == 32 ? 2 : 1) * persistent_cus();
     hipLaunchKernelGGL((maps_bwd_short_kernel<HALF, D, MAPS>), dim3(d->H * d->B < wgs ? d->H * d->B : wgs), dim3(512), lds, s, a);
