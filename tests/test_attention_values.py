@@ -1,11 +1,12 @@
-"""Values that the attention cores meet at the edges: NaN and infinities that are not masked, rows of a cache that no query sees, small gradients.  The formulas in 64 bits and their tolerances are those of
+"""Values that the attention cores meet at the edges: NaN and infinities that are not masked, rows of a cache that no query sees, small gradients, the
+largest tables.  The formulas in 64 bits and their tolerances are those of
 test_attention_maps."""
 import math
 
 import pytest
 import torch
 
-from test_attention_maps import OPS, check, make, mask, reference, run
+from test_attention_maps import OPS, TYPES, both, check, make, mask, reference, run
 
 
 def _spoil(x, at, value):
@@ -34,12 +35,13 @@ def test_keys_that_no_query_sees_may_hold_anything(op, D, Sq, Sk, seen):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("Sq, Sk, H, Hkv", [(70, 100, 2, 2), (70, 100, 4, 2), (150, 201, 2, 2), (5, 700, 4, 2)])
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
 @pytest.mark.parametrize("what", ["q", "k", "v", "do"])
 @pytest.mark.parametrize("op, D", OPS)
-def test_nan_and_infinity_reach_what_depends_on_them(op, D, what, Sq, Sk, H, Hkv):
+def test_nan_and_infinity_reach_what_depends_on_them(op, D, what, t, Sq, Sk, H, Hkv):
     """One in a query, an unmasked key, a value or an output gradient: none of what the formula makes of it comes out finite, in either backward form; masked
     keys' gradients are zeros, and what does not depend on it keeps its bits."""
-    q, k, v, w, bk, do = make(op, torch.bfloat16, 2, H, Hkv, D, Sq, Sk, seed=31, buckets=8, reach=40)
+    q, k, v, w, bk, do = make(op, TYPES[t], 2, H, Hkv, D, Sq, Sk, seed=31, buckets=8, reach=40)
     kv = mask("holes", 2, Sk)
     kv[:, 3] = 1
     b, h, i, j, R = 1, 1, Sq // 2, 3, 40
@@ -112,3 +114,33 @@ def test_powers_of_two_pass_through(op, D, Sq, Sk):
     for n in ("dq", "dk", "dv"):
         big = one[n].abs() >= 2.0 ** -13
         assert torch.equal(one[n][big], half[n][big] * 2), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [32, 128])
+def test_largest_reach_and_table(D):
+    """The largest window that a workgroup holds, and the most positions and buckets that the table's gradient adds up, one position per bucket."""
+    q, k, v, _, _, do = make("relpos", torch.bfloat16, 1, 1, 1, D, 4300, 4200, seed=35)
+    w = torch.randn(8192, 1, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    bk = torch.arange(2 * 4095 + 1, dtype=torch.int32, device="cuda")
+    both("relpos", q, k, v, w, bk, do, q_offset=-50)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq, Sk", [(1, 900), (20, 3000), (70, 100), (140, 160)])
+@pytest.mark.parametrize("op, D", OPS)
+def test_repeats_and_gradients_that_are_not_asked_for(op, D, Sq, Sk):
+    """Split keys, short rows, two passes: the same bits every time, with and without the gradient of the table or of lam."""
+    from univtg_amd import ops
+    q, k, v, w, bk, do = make(op, torch.float16, 3, 4, 4, D, Sq, Sk, seed=36)
+    opts = dict(kvalid=mask("prefix", 3, Sk), causal=True, q_offset=Sk - Sq)
+    a = run(op, q, k, v, w, bk, do, **opts)
+    for _ in range(3):
+        b = run(op, q, k, v, w, bk, do, **opts)
+        assert all(torch.equal(a[n], b[n]) for n in a)
+    if op == "relpos":
+        got = ops.relpos_attention_bwd(do, q, k, v, w, bk, a["o"], a["lse"], need_dtable=False, **opts)
+    else:
+        o2 = ops.diff_attention_fwd(q, k, v, w, need_o2=True, **opts)[2]
+        got = ops.diff_attention_bwd(do, q, k, v, w, a["o"], o2, a["lse"], need_dlam=False, **opts)
+    assert got[3] is None and all(torch.equal(x, a[n]) for x, n in zip(got, ("dq", "dk", "dv")))
