@@ -37,12 +37,12 @@ def _once(backward):
     guarded = once_differentiable(backward)
 
     def once(ctx, do):
-        _refuse_tangents(do)
+        _check_tangents(do)
         return guarded(ctx, do) if torch.is_grad_enabled() else backward(ctx, do)
     return once
 
 
-def _refuse_tangents(*tensors):
+def _check_tangents(*tensors):
     """Forward-mode differentiation: the kernels would drop the tangents without a word."""
     if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError("attention: forward-mode differentiation is not implemented")
@@ -101,7 +101,7 @@ def _check_capture(leaves, stream):
 
 
 def _needs_grad(*tensors):
-    _refuse_tangents(*tensors)
+    _check_tangents(*tensors)
     return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
