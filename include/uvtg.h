@@ -265,6 +265,10 @@ int uvtg_sine_position(const float* vid_mask, const float* txt_mask, const float
  * Scores, statistics and sums are fp32; probabilities and score gradients are rounded to the operands' type for the products with v, k, q, dO.
  * The backward pass forms the probabilities from lse: their relative error grows with a row's largest score, 2^-23 of it, and none exceeds 1.
  * Results are bit-reproducible for a given set of dims (no floating-point atomics on memory, fixed orders of summation).
+ * fp16 score gradients are formed from dO times a power of two where all of dO's entries are below 1, so that they stay in the type's normal range.
+ * The relpos backward's ws holds 4 bytes for every position within reach (at most 2 reach + 1, Sq + Sk - 1) and 16 keys of every head and sample (one set
+ * per head and sample up to 128 queries and keys), also without dtable: 20 MB for 32 x 1232 keys, 8 heads, reach 128, but 8.6 GB for 32 x 8192 keys,
+ * 16 heads, reach 4095.
  * D: 32, 64, or 128 (relpos only).  ws: uvtg_attn_ws_bytes(dims, maps, backward) bytes, 16-byte aligned, no initial value, may be NULL if 0;
  * maps = 1 relpos, 2 diff.  Calls in flight at the same time need a ws each.  No output may overlap an input. */
 typedef struct uvtg_attn_dims {

@@ -8,6 +8,11 @@
 // Every score tile is computed transposed to the operand that follows it (queries along lanes for o and dq, keys along lanes for dk and dv),
 // so that the probabilities go from the accumulators of one MFMA into the operand of the next without leaving their lane; the operand that has
 // to be transposed is read with ds_read_b64_tr_b16.  Tiles reach LDS by LDS-DMA (16 bytes per lane, no register round trip).
+//
+// Probabilities and score gradients are rounded to the operands' 16 bits, once, where they become operands of the matrix pipe: their products are off by
+// about as much as storing them in 16 bits costs anyway.  Against 64 bits o is 1.3 times (one map) to 1.5 times (two, whose difference cancels) as far off
+// as its own rounding makes it.  A second product with what the rounding left takes that to 1.0, and the forward from 220 to 262 us (32 x 1232, 8 heads of
+// 128), from 388 to 507 (causal 2 x 8191, 16 heads of 64), from 568 to 756 (2 x 6007, 8 heads of two maps of 64): not taken.
 #include "uvtg_kernels.h"
 #include "../../include/uvtg.h"
 #include <string.h>
@@ -343,8 +348,8 @@ __device__ __forceinline__ void mask_scores(f32x16& s, unsigned mask32, int lim,
 //   one pass over the keys: m the running maximum of a row's scores, l = sum exp(x - m), o = sum exp(x - m) v, both times exp(m - m') when m rises
 // Bound by the matrix and the vector pipe by turns: a 64-key tile costs a wave 32 MFMAs of 32 cycles (128 channels) and about as many cycles of vector
 // work, half of it exponentials, and two waves per SIMD (registers) overlap the two in part.  MFMA 35 % and vector 43 % of the busy cycles at 128 channels,
-// 40 % and 71 % with three waves at 64.  Measured: 32 x 1232 (half of the keys valid), 8 heads of 128: 220 us, 680 TF/s; causal 2 x 8191, 16 heads of 64:
-// 395 us, 696 TF/s; two maps of 64, 2 x 6007, 8 heads: 546 us, 515 TF/s.  Row blocks of 256 (8 waves) were 5 - 20 % slower.
+// 40 % and 71 % with three waves at 64.  Measured: 32 x 1232 (half of the keys valid), 8 heads of 128: 227 us, 660 TF/s; causal 2 x 8191, 16 heads of 64:
+// 431 us (399 at best), 640 TF/s; two maps of 64, 2 x 6007, 8 heads: 534 us, 526 TF/s.  Row blocks of 256 (8 waves) were 5 - 20 % slower.
 // ------------------------------------------------------------------------------------------------
 template <bool HALF, int D, int MAPS>
 __global__ __launch_bounds__(256, 2) void maps_fwd_kernel(const MapArgs a) {
@@ -798,8 +803,8 @@ __global__ __launch_bounds__(256) void maps_join_kernel(const MapArgs a) {
 // divided by the row's sum of p, which is 1 up to the rounding of lse (1e-6): the ds of a row then add up to 0, where a bucket that holds nearly all of
 // a row would keep the difference and nothing else.
 // Row statistics leave as [B][H][64-query tile][MAPS][2][64] floats: log2 of the row sum (ROW_OFF for a row without one), r.
-// Bound as the forward: three products per pair of positions instead of two.  32 x 1232, 8 heads of 128: 320 us, 700 TF/s; causal 4 x 4096, 16 heads of
-// two maps of 64: 720 us, 572 TF/s (of which the sums of p and dP's signs, for the precision of r: 3 - 5 %).  (Exponentials placed under the MFMAs of dP by hand were 13 % slower.)
+// Bound as the forward: three products per pair of positions instead of two.  32 x 1232, 8 heads of 128: 330 us, 680 TF/s; causal 4 x 4096, 16 heads of
+// two maps of 64: 762 us (713 at best), 540 TF/s (of which the sums of p and dP's signs, for the precision of r: 3 - 5 %).  (Exponentials placed under the MFMAs of dP by hand were 13 % slower.)
 // ------------------------------------------------------------------------------------------------
 template <bool HALF, int D, int MAPS>
 __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
@@ -1000,7 +1005,7 @@ __global__ __launch_bounds__(256, 2) void maps_bwd_q_kernel(const MapArgs a) {
 // 32 (w & 3) .. and of each tile the queries 32 (w >> 2) .., and the two waves of a key block add up at the end: two waves per SIMD, whose LDS round
 // trips, exponentials and MFMAs overlap (one wave of 4 per SIMD, with everything in 420 registers, spent two thirds of its time waiting).
 // Bound by the pipes and by LDS, of which a block near the diagonal uses twice as much (its score gradients are summed along the diagonals): 32 x 1232,
-// 8 heads of 128: 485 us, 615 TF/s over four products; causal 4 x 4096, 16 heads of two maps of 64: 680 us, 808 TF/s.
+// 8 heads of 128: 500 us, 597 TF/s over four products; causal 4 x 4096, 16 heads of two maps of 64: 694 us, 792 TF/s.
 // ------------------------------------------------------------------------------------------------
 template <bool HALF, int D, int MAPS>
 __global__ __launch_bounds__(512, 2) void maps_bwd_k_kernel(const MapArgs a) {
@@ -1785,7 +1790,8 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // 11 us + 0.08 us per 1000 keys of each of its row blocks.  Measured, row blocks against split, us (8 heads of 128; of two maps of 64):
 //   1 x 128 queries: 512 keys 18, 13; 28, 16   2048 keys 52, 17; 95, 21   4 x 256: 512 keys 19, 24; 29, 30   4096 keys 98, 93; 185, 99
 //   7 x 256, 1024 keys: 31, 54; 52, 63   32 x 128, 2048 keys: 63, 158; 101, 163   64 x 32, 1024 keys: 47, 48; 59, 52   64 x 32, 107 keys: 11, 11; 14, 16
-// (Under 512 keys the gain is 3 - 6 us at most, and a sample's result does not depend on how many others there are.)
+// Under 512 keys the gain is 3 - 6 us at most, and is given up: there, above 32 queries, a sample's bits do not depend on how many others there are.  From
+// 512 keys on, and for up to 32 queries, the number of ranges does depend on the batch, and with it the order of a row's sums.
 // Up to 32 queries the two differ little and the heads of a group share a row block, so that their keys are read once.
 struct SplitPlan { int use, hb, blocks, nsplit; };         // heads packed per row block, row blocks per key head, key ranges
 SplitPlan plan_split(const uvtg_attn_dims* d, int maps) {

@@ -372,7 +372,8 @@ def relpos_attention_fwd(q, k, v, table, buckets, kvalid=None, q_offset=0, causa
 
 
 def relpos_attention_bwd(do, q, k, v, table, buckets, o, lse, kvalid=None, q_offset=0, causal=False, scale=None, need_dtable=True):
-    """Gradients of relpos_attention_fwd from its outputs and do: dq, dk, dv (the operands' type, contiguous) and dtable (fp32, or None)."""
+    """Gradients of relpos_attention_fwd from its outputs and do: dq, dk, dv (the operands' type, contiguous) and dtable (fp32, or None: its last sums are
+    left out then, not its workspace of 4 bytes per position within reach, 16 keys, head and sample)."""
     if _elsewhere(q):
         with torch.cuda.device(q.device):
             return relpos_attention_bwd(do, q, k, v, table, buckets, o, lse, kvalid, q_offset, causal, scale, need_dtable)
