@@ -371,8 +371,8 @@ const float* uvtg_backward_gradnorm2(const uvtg_dims* dm, void* workspace);
 
 
 /* Data-parallel runs: leave k compute units out of every persistent grid (the GEMMs': NT tiles and weight-gradient units are sized for
- * CUs - k; the relpos / diff attention backward of up to 128 positions), so that RCCL's all-reduce kernels on the communication stream always find free CUs while backward runs (the reference
- * gets this from DDP's bucket hooks running beside cuBLAS kernels that do not fill the chip, main/train_vlp_ddp.py:272-275).
+ * CUs - k; the relpos / diff attention backward of up to 128 positions), so that RCCL's all-reduce kernels on the communication stream
+ * always find free CUs while backward runs (the reference gets this from DDP's bucket hooks running beside cuBLAS kernels that do not fill the chip, main/train_vlp_ddp.py:272-275).
  * k = 0 (default): whole chip.  Process-wide; returns the number of CUs the grids will use. */
 int uvtg_set_reserved_cus(int k);
 const char* uvtg_strerror(int code);

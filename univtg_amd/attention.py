@@ -77,8 +77,8 @@ class _DiffAttention(torch.autograd.Function):
 def _apply(function, leaves, *args):
     """function.apply(*args), which differentiates `leaves`.  A gradient accumulator lives as long as some autograd graph of its leaf does, and autograd's
     engine makes the stream it was made on wait for a backward pass: during a capture that joins a stream outside it, which ends the process in
-    capture_end, not in an error.  So every graph made here is noted on its leaves, and a capture is refused while one of another stream is alive.  (Whether a graph of another
-    operation holds a leaf cannot be asked of torch.)"""
+    capture_end, not in an error.  So every graph made here is noted on its leaves, and a capture is refused while one of another stream is alive.
+    (Whether a graph of another operation holds a leaf cannot be asked of torch.)"""
     on_gpu = leaves[0].is_cuda
     stream = ops._stream_of(leaves[0]) if on_gpu else 0
     leaves = [t for t in leaves if t.requires_grad and t.is_leaf]

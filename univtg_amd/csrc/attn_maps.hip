@@ -84,7 +84,7 @@ __device__ __forceinline__ float log2_near_1(float s) {
 // 4 x 3869 queries over 2657 keys, fp16: 1.1e-5 of dlam before, under 1e-6 with it).  ds does not feel a constant in dP.
 __device__ __forceinline__ s16x8 negated(s16x8 x) { return x ^ (short)0x8000; }
 // fp16 score gradients: of a small dO (a mean over a batch, no loss scale) most would fall below the type's normal range (dO of 2^-10 over 4000 keys: dq and
-// dk off by 5e-3 instead of 3e-4).  They are formed from dO times the power of two that brings its largest entry to 1 .. 2, and dq and dk are divided by it
+// dk off by 5e-3, where storing them in 16 bits makes 6e-4).  They are formed from dO times the power of two that brings its largest entry to 1 .. 2, and dq and dk are divided by it
 // in the factor that they are stored with; an entry of 1 or more leaves everything as it is.  (Not further up: |dS| may reach |dO| |v| channels / 2.)
 __device__ __forceinline__ float lift_of(float amax) {                     // (NaN, infinity: 1)
   const int e = (int)((__float_as_uint(amax) >> 23) & 255) - 127;
